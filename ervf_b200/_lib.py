@@ -26,6 +26,13 @@ LAUNCH_PDL = 1
 LAUNCH_IDS_READY = 2
 UP_SWIGLU = 4
 
+F32 = 0
+BF16 = 1
+ACT_NONE = 0
+ACT_RELU2 = 1
+ACT_SILU = 2
+ACT_GELU = 3
+
 _NAMES = {
     ERR_NULL: "null pointer",
     ERR_SHAPE: "unsupported shape",
@@ -41,6 +48,7 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
+_ll = ctypes.c_longlong
 
 # name -> argtypes (all return int)
 SIGNATURES: dict[str, list] = {
@@ -107,12 +115,22 @@ SIGNATURES: dict[str, list] = {
     "ervf_f32_gemv": [_vp, _vp, _vp, _i, _i, _vp],
     "ervf_route_gemv_topk": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _vp, _i, _vp],
     "ervf_cache_assign": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
+    "ervf_linear_bf16": [_vp, _vp, _ll, _vp, _vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, _vp],
+    "ervf_conv1d_prompt": [_vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _ll, _i, _i, _i, _i,
+                           _i, _vp],
+    "ervf_ssm_prompt": [_vp, _ll, _vp, _ll, _vp, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp,
+                        _vp, _i, _vp, _ll, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp],
+    "ervf_ssm_prompt_scratch_bytes": [_i, _i, _i, _i, _i, _i, _i],
+    "ervf_ssm_token": [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _i,
+                       _vp, _vp, _ll, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "ervf_gated_norm": [_vp, _ll, _vp, _ll, _vp, _f, _vp, _ll, _i, _i, _i, _i, _vp],
     "ervf_cache_fetch": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _i, _vp],
 }
 
 SIZE_RESULT = {"ervf_routesum_scratch_bytes", "ervf_nvfp4_gemm_tc_scratch_bytes",
                "ervf_moe_token_scratch_bytes", "ervf_moe_token_ep_scratch_bytes",
-               "ervf_moe_batched_scratch_bytes", "ervf_ep_region_bytes"}
+               "ervf_moe_batched_scratch_bytes", "ervf_ep_region_bytes",
+               "ervf_ssm_prompt_scratch_bytes"}
 
 _lib = None
 

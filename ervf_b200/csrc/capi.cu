@@ -9,6 +9,7 @@
 #include "aux.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "ssm.h"
 
 using namespace ervf;
 
@@ -45,9 +46,10 @@ int ervf_version(void) { return 100; }
 
 int ervf_device_status(void) {
   // read and clear every unit's word; report the first error found
-  const int v[6] = {read_gemv_device_error(true), read_aux_device_error(true),
+  const int v[7] = {read_gemv_device_error(true), read_aux_device_error(true),
                     read_tc_device_error(true), read_ep_device_error(true),
-                    read_mma_device_error(true), read_token_device_error(true)};
+                    read_mma_device_error(true), read_token_device_error(true),
+                    read_linear_device_error(true)};
   for (int e : v)
     if (e) return e;
   return kOk;
@@ -1122,6 +1124,134 @@ int ervf_moe_down_routesum_static(const uint8_t* dn_codes, const uint8_t* dn_sca
   return ervf_moe_down_routesum(dn_codes, dn_scales, dn_code_stride, dn_scale_stride, ids, globals,
                                 route_w, top_k, act, base, resid, out, hidden, inter, scratch,
                                 kStaticScratchBytes, width, flags, stream);
+}
+
+// ---------------------------------------- dense and state-space operators
+
+namespace {
+
+inline bool type_ok(int t) { return t == kTypeF32 || t == kTypeBF16; }
+inline uintptr_t elem(int t) { return t == kTypeBF16 ? 2 : 4; }
+
+int check_packing(const int32_t* cu, int seqs, int n_slots) {
+  if (seqs < 0 || n_slots < 0) return kErrShape;
+  if (!cu && seqs != 1) return kErrArg;
+  return kOk;
+}
+
+}  // namespace
+
+int ervf_linear_bf16(const uint16_t* W, const uint16_t* x, long long x_stride, const float* bias,
+                     const void* resid, long long resid_stride, void* out, long long out_stride,
+                     int out_type, int rows, int cols, int tokens, int act, void* stream) {
+  if (!W || (tokens > 0 && (!x || !out))) return kErrNull;
+  if (rows <= 0 || cols <= 0 || tokens < 0 || cols % 8) return kErrShape;
+  if (x_stride < cols || out_stride < rows || (resid && resid_stride < rows)) return kErrShape;
+  if (!type_ok(out_type) || act < kActNone || act > kActGelu) return kErrArg;
+  if (tokens > 0 && (out == x || (resid == out && resid_stride != out_stride))) return kErrArg;
+  if (!al(W, 16) || !al(x, 16) || x_stride % 8 || !al(bias, 4) || !al(out, elem(out_type)) ||
+      !al(resid, elem(out_type)))
+    return kErrAlign;
+  if (tokens == 0) return kOk;
+  return launch_linear({W, x, bias, resid, out, x_stride, resid_stride, out_stride, rows, cols, tokens, out_type, act},
+                       S(stream));
+}
+
+int ervf_conv1d_prompt(const void* x, long long x_stride, const float* w, const float* bias, void* state,
+                       int n_slots, const int32_t* slots, const uint8_t* has_state, const int32_t* cu_seqlens,
+                       int seqs, void* out, long long out_stride, int type, int tokens, int channels, int width,
+                       int silu, void* stream) {
+  if (!w || (tokens > 0 && (!x || !out))) return kErrNull;
+  if (tokens < 0 || channels <= 0 || width < 2 || width > kMaxConvWidth) return kErrShape;
+  if (x_stride < channels || out_stride < channels) return kErrShape;
+  if (int e = check_packing(cu_seqlens, seqs, n_slots)) return e;
+  if (!type_ok(type) || silu < 0 || silu > 1 || (tokens > 0 && out == x)) return kErrArg;
+  const uintptr_t b = elem(type);
+  if (!al(x, b) || !al(out, b) || !al(state, b) || !al(w, 4) || !al(bias, 4) || !al(cu_seqlens, 4) || !al(slots, 4))
+    return kErrAlign;
+  if (seqs == 0) return kOk;
+  ConvArgs a{{cu_seqlens, slots, has_state, seqs, tokens, n_slots}, x, out, w, bias, state, x_stride, out_stride,
+             type, channels, width, silu};
+  return launch_conv1d_prompt(a, S(stream));
+}
+
+size_t ervf_ssm_prompt_scratch_bytes(int type, int tokens, int seqs, int heads, int head_dim, int groups,
+                                     int d_state) {
+  if (!type_ok(type) || tokens < 0 || seqs < 0 || heads <= 0 || groups <= 0 || heads % groups || head_dim <= 0 ||
+      head_dim > kMaxHeadDim || d_state <= 0 || d_state > kMaxDState)
+    return 0;
+  return ssm_prompt_scratch_bytes(type, tokens, seqs, heads, head_dim, groups, d_state);
+}
+
+int ervf_ssm_prompt(const void* x, long long x_stride, const void* dt, long long dt_stride, const float* A,
+                    const void* B, long long b_stride, const void* C, long long c_stride, const float* D,
+                    const float* dt_bias, float* state, int n_slots, const int32_t* slots, const uint8_t* has_state,
+                    const int32_t* cu_seqlens, int seqs, void* y, long long y_stride, int type, int tokens, int heads,
+                    int head_dim, int groups, int d_state, void* scratch, size_t scratch_bytes, void* stream) {
+  if (!A || (tokens > 0 && (!x || !dt || !B || !C || !y))) return kErrNull;
+  if (tokens < 0 || heads <= 0 || heads > 65535 || groups <= 0 || heads % groups || head_dim <= 0 ||
+      head_dim > kMaxHeadDim || d_state <= 0 || d_state > kMaxDState)
+    return kErrShape;
+  const long long inner = (long long)heads * head_dim, bc = (long long)groups * d_state;
+  if (x_stride < inner || y_stride < inner || dt_stride < heads || b_stride < bc || c_stride < bc) return kErrShape;
+  if (int e = check_packing(cu_seqlens, seqs, n_slots)) return e;
+  if (!type_ok(type) || (tokens > 0 && (y == x || y == dt || y == B || y == C))) return kErrArg;
+  const uintptr_t b = elem(type);
+  if (!al(x, b) || !al(dt, b) || !al(B, b) || !al(C, b) || !al(y, b) || !al(A, 4) || !al(D, 4) || !al(dt_bias, 4) ||
+      !al(state, 4) || !al(cu_seqlens, 4) || !al(slots, 4))
+    return kErrAlign;
+  const size_t need = ssm_prompt_scratch_bytes(type, tokens, seqs, heads, head_dim, groups, d_state);
+  if (need && !scratch) return kErrNull;
+  if (need && !al(scratch, 16)) return kErrAlign;
+  if (scratch_bytes < need) return kErrArg;
+  if (seqs == 0) return kOk;
+  ScanArgs a{{cu_seqlens, slots, has_state, seqs, tokens, n_slots}, x, dt, B, C, y, A, D, dt_bias, state,
+             x_stride, dt_stride, b_stride, c_stride, y_stride, type, heads, head_dim, groups, d_state,
+             scratch, scratch_bytes};
+  return launch_ssm_prompt(a, S(stream));
+}
+
+int ervf_ssm_token(const void* xbc, long long xbc_stride, const void* dt, long long dt_stride, const void* z,
+                   long long z_stride, const float* conv_w, const float* conv_bias, void* conv_state,
+                   const float* A, const float* D, const float* dt_bias, const float* norm_w, float eps,
+                   float* state, int n_slots, const int32_t* slots, void* out, long long out_stride, int type,
+                   int seqs, int heads, int head_dim, int groups, int d_state, int width, void* stream) {
+  if (!conv_w || !A || (seqs > 0 && (!xbc || !dt || !out)) || (n_slots > 0 && (!conv_state || !state)))
+    return kErrNull;
+  if (seqs < 0 || n_slots < 0 || heads <= 0 || groups <= 0 || heads % groups || head_dim <= 0 ||
+      head_dim > kMaxHeadDim || d_state <= 0 || d_state > kMaxDState || d_state % 4 || width < 2 ||
+      width > kMaxConvWidth)
+    return kErrShape;
+  const long long inner = (long long)heads * head_dim, ch = inner + 2LL * groups * d_state;
+  if (xbc_stride < ch || dt_stride < heads || (z && z_stride < inner) || out_stride < inner) return kErrShape;
+  if (!type_ok(type) || (seqs > 0 && (out == xbc || out == dt || out == z)) || !(eps >= 0.0f)) return kErrArg;
+  const uintptr_t b = elem(type);
+  if (!al(xbc, b) || !al(dt, b) || !al(z, b) || !al(conv_state, b) || !al(out, b) || !al(conv_w, 4) ||
+      !al(conv_bias, 4) || !al(A, 4) || !al(D, 4) || !al(dt_bias, 4) || !al(norm_w, 4) || !al(state, 16) ||
+      !al(slots, 4))
+    return kErrAlign;
+  if (seqs == 0) return kOk;
+  TokenArgs a{xbc, dt, z, out, conv_w, conv_bias, conv_state, A, D, dt_bias, norm_w, state, slots,
+              xbc_stride, dt_stride, z_stride, out_stride, eps, type, seqs, n_slots, heads, head_dim, groups,
+              d_state, width};
+  return launch_ssm_token(a, S(stream));
+}
+
+int ervf_gated_norm(const void* y, long long y_stride, const void* z, long long z_stride, const float* w,
+                    float eps, void* out, long long out_stride, int type, int tokens, int groups, int group_size,
+                    void* stream) {
+  if (!w || (tokens > 0 && (!y || !out))) return kErrNull;
+  if (tokens < 0 || groups <= 0 || group_size <= 0) return kErrShape;
+  const long long n = (long long)groups * group_size;
+  if (y_stride < n || (z && z_stride < n) || out_stride < n || (long long)tokens * groups > 0x7fffffffLL)
+    return kErrShape;
+  if (!type_ok(type) || !(eps >= 0.0f)) return kErrArg;
+  if ((out == y && out_stride != y_stride) || (z && out == z && out_stride != z_stride)) return kErrArg;
+  const uintptr_t b = elem(type);
+  if (!al(y, b) || !al(z, b) || !al(out, b) || !al(w, 4)) return kErrAlign;
+  if (tokens == 0) return kOk;
+  return launch_gated_norm({y, z, out, w, y_stride, z_stride, out_stride, eps, type, tokens, groups, group_size},
+                           S(stream));
 }
 
 }  // extern "C"

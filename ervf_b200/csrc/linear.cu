@@ -1,0 +1,361 @@
+// linear.cu -- dense projection with its epilogue on the sm_100a tensor cores:
+//
+//   out[t][r] = act(sum_k W[r][k] x[t][k] + bias[r]) + resid[t][r]
+//
+// W, x bf16, products exact, sums and the whole epilogue in f32, one rounding
+// to the output's type.  Both operands are K-major, so one kernel serves both
+// orientations: the MMA's 128 rows are tokens and its columns features, or
+// (few tokens) its rows are features and its columns tokens.
+//
+// Persistent and warp specialised, one CTA per SM; a k-block is 64 columns
+// (128 bytes of a row, the swizzle's width):
+//   warp 0      producer: TMA of both operands' tiles into a ring of stages
+//   warp 1      one lane issues the tcgen05.mma of each stage into one of two
+//               accumulator buffers in tensor memory
+//   warps 2..5  epilogue: tcgen05.ld of a finished buffer, bias, activation,
+//               residual, store -- while the next tile's MMAs run
+// Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
+// dead, and every role drains before tensor memory is freed.
+#include <cuda.h>  // CUtensorMap and the encode function's types (driver entry point)
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "ssm.h"
+
+namespace ervf {
+
+namespace {
+
+constexpr int kLinM = 128, kLinKB = 64;
+constexpr int kLinThreads = 6 * 32;
+constexpr int kLinATile = kLinM * kLinKB * 2;
+
+template <int BN>
+struct LinShape {
+  static constexpr int kBTile = BN * kLinKB * 2;
+  static constexpr int kStage = kLinATile + kBTile;  // both multiples of 1024 bytes (swizzle period)
+  static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
+  static constexpr int kSmem = 1024 + 1024 + kStages * kStage;  // barriers, alignment slack, ring
+  static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+  static_assert(BN % 16 == 0 && BN <= 256 && (kTmemCols & (kTmemCols - 1)) == 0, "tile");
+};
+
+struct LinTile {
+  const float* bias;
+  const void* resid;
+  void* out;
+  long long resid_stride, out_stride;
+  int rows, cols, tokens;
+  int act;
+  int nkb, mtiles, ntiles;
+};
+
+__device__ __forceinline__ uint64_t lin_desc(uint32_t saddr) {
+  // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void lin_tma(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void lin_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+               ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void lin_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+
+// Bounded wait that also gives up when another role of the CTA died.
+__device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*dead) return false;
+    if (clock64() - t0 > 2000000000LL) {
+      atomicExch(&g_device_error, kErrTimeout);
+      *dead = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ float lin_act(float v, int act) {
+  if (act == kActRelu2) {
+    const float r = v < 0.0f ? 0.0f : v;  // a NaN stays one
+    return r * r;
+  }
+  if (act == kActSilu) return v / (1.0f + expf(-v));
+  if (act == kActGelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float lin_get(const T* p) {
+  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
+  else return *p;
+}
+template <typename T>
+__device__ __forceinline__ void lin_put(T* p, float v) {
+  if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
+  else *p = v;
+}
+
+// N consecutive features r.. of token t.
+template <typename T, int N>
+__device__ __forceinline__ void lin_row(const LinTile& a, size_t t, int r, const float (&acc)[N]) {
+  T* o = static_cast<T*>(a.out) + t * a.out_stride + r;
+  const T* q = a.resid ? static_cast<const T*>(a.resid) + t * a.resid_stride + r : nullptr;
+  constexpr int V = 16 / sizeof(T);
+  const bool whole = r + N <= a.rows && ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(q)) & 15) == 0 &&
+                     (!a.bias || (reinterpret_cast<uintptr_t>(a.bias + r) & 15) == 0);
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+      uint4 rq = q ? *reinterpret_cast<const uint4*>(q + i) : make_uint4(0, 0, 0, 0), oq;
+      const T* re = reinterpret_cast<const T*>(&rq);
+      T* oe = reinterpret_cast<T*>(&oq);
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const float4 b = a.bias ? *reinterpret_cast<const float4*>(a.bias + r + i + j) : make_float4(0, 0, 0, 0);
+        const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float v = lin_act(acc[i + j + k] + bb[k], a.act);
+          lin_put(oe + j + k, q ? v + lin_get(re + j + k) : v);
+        }
+      }
+      *reinterpret_cast<uint4*>(o + i) = oq;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (r + i < a.rows) {
+      const float v = lin_act(acc[i] + (a.bias ? a.bias[r + i] : 0.0f), a.act);
+      lin_put(o + i, q ? v + lin_get(q + i) : v);
+    }
+}
+
+template <int BN, bool SWAP, typename T>
+__global__ void __launch_bounds__(kLinThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, LinTile a) {
+  using Sh = LinShape<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty = full + Sh::kStages;
+  uint64_t* dfull = empty + Sh::kStages;
+  uint64_t* dempty = dfull + 2;
+  uint64_t* mma_done = dempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 512);
+  volatile int* dead = reinterpret_cast<volatile int*>(smem + 516);
+  uint8_t* ring = smem + 1024;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
+                             ((uint32_t)(kLinM >> 4) << 24);
+
+  if (tid == 0) {
+    for (int i = 0; i < Sh::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&dfull[i], 1);
+      mbar_init(&dempty[i], 4);
+    }
+    mbar_init(mma_done, 1);
+    *dead = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(tmem_slot)), "r"(Sh::kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const int units = a.mtiles * a.ntiles;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t gk = 0;
+      for (int u = blockIdx.x; u < units && !*dead; u += gridDim.x) {
+        const int mt = u % a.mtiles, nt = u / a.mtiles;
+        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
+          const int s = (int)(gk % Sh::kStages);
+          if (!lin_wait(&empty[s], ((gk / Sh::kStages) & 1) ^ 1, dead)) break;
+          mbar_arrive_expect_tx(&full[s], Sh::kStage);
+          uint8_t* st = ring + s * Sh::kStage;
+          lin_tma(st, &a_map, kb * kLinKB, mt * kLinM, &full[s]);
+          lin_tma(st + kLinATile, &b_map, kb * kLinKB, nt * BN, &full[s]);
+        }
+      }
+      // leave no tensor copy in flight
+      for (uint32_t k = gk > (uint32_t)Sh::kStages ? gk - Sh::kStages : 0; k < gk; ++k)
+        lin_wait(&full[k % Sh::kStages], (k / Sh::kStages) & 1, dead);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t gk = 0;
+      int nu = 0;
+      for (int u = blockIdx.x; u < units && !*dead; u += gridDim.x, ++nu) {
+        const int d = nu & 1;
+        if (!lin_wait(&dempty[d], ((nu >> 1) & 1) ^ 1, dead)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        bool ok = true;
+        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
+          const int s = (int)(gk % Sh::kStages);
+          if (!lin_wait(&full[s], (gk / Sh::kStages) & 1, dead)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t st = smem_u32(ring + s * Sh::kStage);
+#pragma unroll
+          for (int j = 0; j < kLinKB / 16; ++j) {
+            const uint32_t acc = (kb | j) ? 1u : 0u;
+            asm volatile(
+                "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                ::"r"(tmem + (uint32_t)(d * BN)), "l"(lin_desc(st + 32 * j)),
+                  "l"(lin_desc(st + kLinATile + 32 * j)), "r"(idesc), "r"(acc) : "memory");
+          }
+          lin_commit(&empty[s]);
+        }
+        if (!ok) break;
+        lin_commit(&dfull[d]);
+      }
+      // every MMA is complete before tensor memory is freed
+      lin_commit(mma_done);
+      mbar_wait(mma_done, 0, 2000000000LL);
+    }
+  } else {
+    const int q = warp & 3;  // tensor-memory lanes 32 q ..
+    int nu = 0;
+    for (int u = blockIdx.x; u < units && !*dead; u += gridDim.x, ++nu) {
+      const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
+      const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
+      if (!__all_sync(0xffffffffu, w_ok)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int m = mt * kLinM + 32 * q + lane;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 16) {
+        uint32_t v[16];
+        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        float f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+        if constexpr (SWAP) {
+          if (m < a.rows) {
+            const float b = a.bias ? a.bias[m] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int t = nt * BN + c + i;
+              if (t < a.tokens) {
+                float o = lin_act(f[i] + b, a.act);
+                if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + m);
+                lin_put(static_cast<T*>(a.out) + (size_t)t * a.out_stride + m, o);
+              }
+            }
+          }
+        } else {
+          if (m < a.tokens && nt * BN + c < a.rows) lin_row<T, 16>(a, m, nt * BN + c, f);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&dempty[d]);  // the buffer is read
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kTmemCols) : "memory");
+}
+
+// ------------------------------------------------------------------- host
+
+typedef CUresult (*LinEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+LinEncodeFn lin_encode_fn() {
+  static LinEncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return (LinEncodeFn) nullptr;
+    return reinterpret_cast<LinEncodeFn>(p);
+  }();
+  return fn;
+}
+
+// bf16 [rows][cols] with rows `stride` elements apart, boxes of box_rows x 64
+// columns, 128-byte swizzle, zeros past the edges.
+int lin_map(CUtensorMap* map, const uint16_t* p, int rows, int cols, long long stride, int box_rows) {
+  LinEncodeFn enc = lin_encode_fn();
+  if (!enc) return kErrLaunch;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t box[2] = {kLinKB, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(p), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? kOk
+             : kErrArg;
+}
+
+template <int BN, bool SWAP, typename T>
+int linear_run(const LinearArgs& l, cudaStream_t stream) {
+  using Sh = LinShape<BN>;
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0};
+  a.nkb = (l.cols + kLinKB - 1) / kLinKB;
+  const int ma = SWAP ? l.rows : l.tokens, nb = SWAP ? l.tokens : l.rows;
+  a.mtiles = (ma + kLinM - 1) / kLinM;
+  a.ntiles = (nb + BN - 1) / BN;
+  CUtensorMap wm, xm;
+  if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, SWAP ? kLinM : BN)) return e;
+  if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, SWAP ? BN : kLinM)) return e;
+  auto fn = linear_kernel<BN, SWAP, T>;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
+    return kErrLaunch;
+  const long long units = (long long)a.mtiles * a.ntiles;
+  if (units > 0x7fffffffLL) return kErrShape;
+  const int sms = device_sm_count();
+  fn<<<(unsigned)(units < sms ? units : sms), kLinThreads, Sh::kSmem, stream>>>(SWAP ? wm : xm, SWAP ? xm : wm, a);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <typename T>
+int linear_pick(const LinearArgs& l, cudaStream_t stream) {
+  if (l.tokens <= 32) return linear_run<32, true, T>(l, stream);
+  if (l.tokens <= 128) return linear_run<64, true, T>(l, stream);
+  return linear_run<256, false, T>(l, stream);
+}
+
+}  // namespace
+
+int launch_linear(const LinearArgs& l, cudaStream_t stream) {
+  return l.out_type == kTypeBF16 ? linear_pick<__nv_bfloat16>(l, stream) : linear_pick<float>(l, stream);
+}
+
+int read_linear_device_error(bool clear) { return read_unit_error(clear); }
+
+}  // namespace ervf

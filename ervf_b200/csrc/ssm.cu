@@ -1,0 +1,507 @@
+// ssm.cu -- the state-space layer of the hybrid next to its routed experts:
+// causal convolution, selective scan (token by token), one-token step and
+// gated norm.  The reference runs these one token at a time (conv1d, ssm,
+// softplus, gated_rmsnorm: gpu_kernels.py:77-1515); here prompts are packed
+// sequences, and a decode step is one launch.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "ssm.h"
+
+namespace cg = cooperative_groups;
+
+namespace ervf {
+
+namespace {
+
+// ------------------------------------------------------------ small helpers
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// V consecutive elements as f32.  V is 1 or fills 16 bytes.
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else {
+    static_assert(V * sizeof(T) == 16, "16-byte vectors");
+    uint4 q = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32(e[i]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else {
+    uint4 q;
+    T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = q;
+  }
+}
+
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+// log(1 + exp(v)); above 20 the 1 is below half a unit in the last place
+__device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+
+// Tokens [begin, begin + len) of sequence i, kept inside the token array
+// whatever the offsets say.
+__device__ __forceinline__ void seq_range(const Packing& p, int i, int& begin, int& len) {
+  if (!p.cu) {
+    begin = 0;
+    len = p.tokens;
+    return;
+  }
+  const int b = min(max(p.cu[i], 0), p.tokens), e = min(max(p.cu[i + 1], 0), p.tokens);
+  begin = b;
+  len = max(e - b, 0);
+}
+
+// State slot of sequence i, or -1 for none.
+__device__ __forceinline__ int seq_slot(const Packing& p, int i) {
+  const int s = p.slots ? p.slots[i] : i;
+  return s >= 0 && s < p.n_slots ? s : -1;
+}
+
+// Tile `tile` of the packed sequences, each cut into tiles of `size` tokens
+// from its own first token, an empty one into one: which sequence, and the
+// tile's place in it.  One warp; false past the last tile.
+__device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, int& seq, int& nth) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int i0 = 0; i0 < p.seqs; i0 += 32) {
+    int n = 0;
+    if (i0 + lane < p.seqs) {
+      int b, len;
+      seq_range(p, i0 + lane, b, len);
+      n = max(1, (len + size - 1) / size);
+    }
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, inc, 31);
+    if (tile < base + total) {
+      const unsigned m = __ballot_sync(0xffffffffu, tile < base + inc);
+      const int l = __ffs(m) - 1;
+      seq = i0 + l;
+      nth = tile - base - __shfl_sync(0xffffffffu, inc - n, l);
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+// ------------------------------------------------------------- convolution
+
+// y_t = act(bias + sum_j w[j] x[t - width + 1 + j]) for each channel.  A
+// thread owns V channels of one tile of a sequence and keeps the window in
+// registers.  Bound by HBM: every input is read once (and `width - 1` rows
+// again per tile, from L2), every output written once.  The thread of a
+// sequence's first tile is the only one that touches the carried state: it
+// reads the old inputs, and writes the sequence's last `width - 1` ones.
+constexpr int kConvTile = 32, kConvThreads = 128;
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
+  const int ch = (blockIdx.y * kConvThreads + threadIdx.x) * V;
+  int seq, nth;
+  if (!find_tile(a.pk, blockIdx.x, kConvTile, seq, nth)) return;
+  if (ch >= a.channels) return;
+  int begin, len;
+  seq_range(a.pk, seq, begin, len);
+  const T* x = static_cast<const T*>(a.x) + (size_t)begin * a.x_stride + ch;
+  T* out = static_cast<T*>(a.out) + (size_t)begin * a.out_stride + ch;
+  float w[V][W], bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    bias[v] = a.bias ? a.bias[ch + v] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[v][j] = a.w[(size_t)(ch + v) * W + j];
+  }
+  const int slot = nth == 0 && a.state ? seq_slot(a.pk, seq) : -1;
+  T* state = slot < 0 ? nullptr : static_cast<T*>(a.state) + (size_t)slot * (W - 1) * a.channels + ch;
+  float win[W - 1][V];  // the W - 1 inputs before the next one, oldest first
+  const int t0 = nth * kConvTile, t1 = min(t0 + kConvTile, len);
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) {
+    const int t = t0 - (W - 1) + j;
+    if (t >= 0) {
+      load_vec<T, V>(x + (size_t)t * a.x_stride, win[j]);
+    } else if (state && a.pk.has && a.pk.has[seq]) {
+      load_vec<T, V>(state + (size_t)j * a.channels, win[j]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) win[j][v] = 0.0f;
+    }
+  }
+  if (state) {
+    // last W - 1 inputs of [carried state, sequence]
+    float last[W - 1][V];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      const int t = len - (W - 1) + j;
+      if (t >= 0) {
+        load_vec<T, V>(x + (size_t)t * a.x_stride, last[j]);
+      } else {
+        // win holds the carried inputs at positions -(W - 1) .. -1
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float e = 0.0f;
+#pragma unroll
+          for (int k = 0; k < W - 1; ++k)
+            if (t + (W - 1) == k) e = win[k][v];
+          last[j][v] = e;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) store_vec<T, V>(state + (size_t)j * a.channels, last[j]);
+  }
+#pragma unroll 4
+  for (int t = t0; t < t1; ++t) {
+    float cur[V], y[V];
+    load_vec<T, V>(x + (size_t)t * a.x_stride, cur);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float s = bias[v];
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) s = fmaf(w[v][j], win[j][v], s);
+      s = fmaf(w[v][W - 1], cur[v], s);
+      y[v] = a.silu ? silu(s) : s;
+#pragma unroll
+      for (int j = 0; j + 1 < W - 1; ++j) win[j][v] = win[j + 1][v];
+      win[W - 2][v] = cur[v];
+    }
+    store_vec<T, V>(out + (size_t)t * a.out_stride, y);
+  }
+}
+
+template <typename T, int V>
+int launch_conv(const ConvArgs& a, cudaStream_t stream) {
+  const dim3 grid((unsigned)(a.pk.tokens / kConvTile + a.pk.seqs),
+                  (a.channels + kConvThreads * V - 1) / (kConvThreads * V));
+  if (a.width == 2) conv_prompt_kernel<T, 2, V><<<grid, kConvThreads, 0, stream>>>(a);
+  else if (a.width == 3) conv_prompt_kernel<T, 3, V><<<grid, kConvThreads, 0, stream>>>(a);
+  else conv_prompt_kernel<T, 4, V><<<grid, kConvThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+// 16-byte vectors of V elements fit a row-strided array.
+bool vec_ok(const void* p, long long stride, size_t elem) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((unsigned long long)stride * elem & 15) == 0;
+}
+
+// --------------------------------------------------- scan, token by token
+
+// The recurrence as it stands: S = exp(d A) S + d x B^T, y = S C + D x, with
+// d = softplus(dt + bias).  Four neighbouring lanes share one row p of one
+// head's state, NL columns each (columns n with (n / 4) % 4 == lane part), in
+// registers; B, C, x and the steps of kSeqTile tokens at a time lie in shared
+// memory.  Serves every type and size; its time is the length of a sequence
+// times the latency of one step.
+constexpr int kSeqRows = 32, kSeqThreads = 4 * kSeqRows, kSeqTile = 16;
+
+template <typename T, int NL>
+__global__ void __launch_bounds__(kSeqThreads) scan_seq_kernel(ScanArgs a) {
+  constexpr int N = 4 * NL;
+  __shared__ __align__(16) float sB[kSeqTile][N], sC[kSeqTile][N];
+  __shared__ float sx[kSeqTile][kSeqRows], sd[kSeqTile], sa[kSeqTile];
+  const int seq = blockIdx.x, head = blockIdx.y, p0 = blockIdx.z * kSeqRows;
+  const int tid = threadIdx.x, part = tid & 3, row = tid >> 2, p = p0 + row;
+  const int n_real = a.d_state, grp = head / (a.heads / a.groups);
+  int begin, len;
+  seq_range(a.pk, seq, begin, len);
+  const int slot = a.state ? seq_slot(a.pk, seq) : -1;
+  const bool live = p < a.head_dim;
+  float* state = slot < 0 || !live ? nullptr
+      : a.state + (((size_t)slot * a.heads + head) * a.head_dim + p) * n_real;
+  const bool has = state && a.pk.has && a.pk.has[seq];
+  float s[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int n = (i >> 2) * 16 + part * 4 + (i & 3);
+    s[i] = has && n < n_real ? state[n] : 0.0f;
+  }
+  const float A = a.A[head], D = a.D ? a.D[head] : 0.0f, bias = a.dt_bias ? a.dt_bias[head] : 0.0f;
+  const T* gx = static_cast<const T*>(a.x) + (size_t)begin * a.x_stride + (size_t)head * a.head_dim + p0;
+  const T* gd = static_cast<const T*>(a.dt) + (size_t)begin * a.dt_stride + head;
+  const T* gb = static_cast<const T*>(a.B) + (size_t)begin * a.b_stride + (size_t)grp * n_real;
+  const T* gc = static_cast<const T*>(a.C) + (size_t)begin * a.c_stride + (size_t)grp * n_real;
+  T* gy = static_cast<T*>(a.y) + (size_t)begin * a.y_stride + (size_t)head * a.head_dim + p;
+  for (int t0 = 0; t0 < len; t0 += kSeqTile) {
+    const int m = min(kSeqTile, len - t0);
+    __syncthreads();
+    for (int i = tid; i < m * N; i += kSeqThreads) {
+      const int t = i / N, n = i - t * N;
+      sB[t][n] = n < n_real ? to_f32(gb[(size_t)(t0 + t) * a.b_stride + n]) : 0.0f;
+      sC[t][n] = n < n_real ? to_f32(gc[(size_t)(t0 + t) * a.c_stride + n]) : 0.0f;
+    }
+    for (int i = tid; i < m * kSeqRows; i += kSeqThreads) {
+      const int t = i / kSeqRows, r = i - t * kSeqRows;
+      sx[t][r] = p0 + r < a.head_dim ? to_f32(gx[(size_t)(t0 + t) * a.x_stride + r]) : 0.0f;
+    }
+    if (tid < m) {
+      const float d = softplus(to_f32(gd[(size_t)(t0 + tid) * a.dt_stride]) + bias);
+      sd[tid] = d;
+      sa[tid] = expf(d * A);
+    }
+    __syncthreads();
+    for (int t = 0; t < m; ++t) {
+      const float x = sx[t][row], dx = sd[t] * x, da = sa[t];
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < NL; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(&sB[t][i * 4 + part * 4]);
+        const float4 c = *reinterpret_cast<const float4*>(&sC[t][i * 4 + part * 4]);
+        s[i] = fmaf(dx, b.x, da * s[i]);
+        s[i + 1] = fmaf(dx, b.y, da * s[i + 1]);
+        s[i + 2] = fmaf(dx, b.z, da * s[i + 2]);
+        s[i + 3] = fmaf(dx, b.w, da * s[i + 3]);
+        y[0] = fmaf(s[i], c.x, y[0]);
+        y[1] = fmaf(s[i + 1], c.y, y[1]);
+        y[2] = fmaf(s[i + 2], c.z, y[2]);
+        y[3] = fmaf(s[i + 3], c.w, y[3]);
+      }
+      float v = (y[0] + y[1]) + (y[2] + y[3]);
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (part == 0 && live) gy[(size_t)(t0 + t) * a.y_stride] = from_f32<T>(fmaf(D, x, v));
+    }
+  }
+  if (state) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int n = (i >> 2) * 16 + part * 4 + (i & 3);
+      if (n < n_real) state[n] = s[i];
+    }
+  }
+}
+
+template <typename T>
+int launch_scan_seq(const ScanArgs& a, cudaStream_t stream) {
+  const dim3 grid(a.pk.seqs, a.heads, (a.head_dim + kSeqRows - 1) / kSeqRows);
+  if (a.d_state <= 16) scan_seq_kernel<T, 4><<<grid, kSeqThreads, 0, stream>>>(a);
+  else if (a.d_state <= 64) scan_seq_kernel<T, 16><<<grid, kSeqThreads, 0, stream>>>(a);
+  else if (a.d_state <= 128) scan_seq_kernel<T, 32><<<grid, kSeqThreads, 0, stream>>>(a);
+  else scan_seq_kernel<T, 64><<<grid, kSeqThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+// --------------------------------------------------------- one-token step
+
+// One token of each sequence: convolution, scan step and gated norm in one
+// launch.  A cluster of CTAs owns one (sequence, group): CTA r takes heads
+// r, r + c, ... of the group.  The heads' states are read and written once,
+// which is what the launch costs for a batch (2 x 4 bytes per state element,
+// HBM bound); for one sequence it is latency: one round of loads, the
+// cluster's two barriers, one round of stores.
+//  1. every CTA convolves its heads' x channels and, for itself, the group's
+//     B and C channels (2 d_state of them: recomputing is cheaper than
+//     sending them on);
+//  2. after a cluster barrier (every CTA has read the carried B / C inputs)
+//     CTA 0 shifts those inputs by one token;
+//  3. the states' update and y, one row of d_state per 32 lanes;
+//  4. the CTAs' sums of squares meet in shared memory of each (added in rank
+//     order), then the norm and the output.
+constexpr int kTokThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ float conv_one(const TokenArgs& a, const T* xin, const T* cs, int ch) {
+  float s = a.conv_bias ? a.conv_bias[ch] : 0.0f;
+  const float* w = a.conv_w + (size_t)ch * a.width;
+  for (int j = 0; j < a.width - 1; ++j)
+    s = fmaf(w[j], cs ? to_f32(cs[(size_t)j * (a.heads * a.head_dim + 2 * a.groups * a.d_state) + ch]) : 0.0f, s);
+  return silu(fmaf(w[a.width - 1], to_f32(xin[ch]), s));
+}
+
+template <typename T>
+__device__ __forceinline__ void conv_shift(const TokenArgs& a, const T* xin, T* cs, int ch) {
+  const size_t pitch = (size_t)a.heads * a.head_dim + 2 * (size_t)a.groups * a.d_state;
+  for (int j = 0; j + 1 < a.width - 1; ++j) cs[j * pitch + ch] = cs[(j + 1) * pitch + ch];
+  cs[(size_t)(a.width - 2) * pitch + ch] = xin[ch];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTokThreads) ssm_token_kernel(TokenArgs a) {
+  extern __shared__ __align__(16) float sm[];
+  cg::cluster_group cl = cg::this_cluster();
+  const int c = (int)cl.num_blocks(), r = (int)cl.block_rank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int unit = blockIdx.x / c, seq = unit / a.groups, grp = unit - seq * a.groups;
+  const int hpg = a.heads / a.groups, P = a.head_dim, N = a.d_state;
+  const int mine = (hpg - r + c - 1) / c;  // heads of this CTA: r, r + c, ...
+  float* sBC = sm;                         // B then C of the group
+  float* sy = sBC + 2 * N;                 // [mine][P]: x, then the gated output
+  float* red = sy + ((hpg + c - 1) / c) * P;  // per-warp sums, then this CTA's sum
+  const int s0 = a.slots ? a.slots[seq] : seq;
+  const int slot = s0 >= 0 && s0 < a.n_slots ? s0 : -1;
+  const T* xin = static_cast<const T*>(a.xbc) + (size_t)seq * a.xbc_stride;
+  const size_t channels = (size_t)a.heads * P + 2 * (size_t)a.groups * N;
+  T* cs = slot < 0 ? nullptr : static_cast<T*>(a.conv_state) + (size_t)slot * (a.width - 1) * channels;
+  for (int i = tid; i < 2 * N; i += kTokThreads) {
+    const int ch = a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N);
+    sBC[i] = conv_one(a, xin, cs, ch);
+  }
+  for (int i = tid; i < mine * P; i += kTokThreads) {
+    const int k = i / P, ch = (grp * hpg + r + k * c) * P + i - k * P;
+    sy[i] = conv_one(a, xin, cs, ch);
+    if (cs) conv_shift(a, xin, cs, ch);
+  }
+  cl.sync();  // B / C inputs read by every CTA; also this CTA's __syncthreads
+  if (r == 0 && cs)
+    for (int i = tid; i < 2 * N; i += kTokThreads)
+      conv_shift(a, xin, cs, a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N));
+  float ss = 0.0f;
+  for (int k = 0; k < mine; ++k) {
+    const int head = grp * hpg + r + k * c;
+    const float d = softplus(to_f32(static_cast<const T*>(a.dt)[(size_t)seq * a.dt_stride + head]) +
+                             (a.dt_bias ? a.dt_bias[head] : 0.0f));
+    const float da = expf(d * a.A[head]), D = a.D ? a.D[head] : 0.0f;
+    float* st = slot < 0 ? nullptr : a.state + ((size_t)slot * a.heads + head) * P * N;
+    for (int p = warp; p < P; p += kTokThreads / 32) {
+      const float x = sy[k * P + p], dx = d * x;
+      float y = 0.0f;
+      for (int n = lane * 4; n < N; n += 128) {
+        float4 v = st ? *reinterpret_cast<const float4*>(st + (size_t)p * N + n) : make_float4(0, 0, 0, 0);
+        const float4 b = *reinterpret_cast<const float4*>(sBC + n);
+        const float4 cc = *reinterpret_cast<const float4*>(sBC + N + n);
+        v.x = fmaf(dx, b.x, da * v.x);
+        v.y = fmaf(dx, b.y, da * v.y);
+        v.z = fmaf(dx, b.z, da * v.z);
+        v.w = fmaf(dx, b.w, da * v.w);
+        if (st) *reinterpret_cast<float4*>(st + (size_t)p * N + n) = v;
+        y += (v.x * cc.x + v.y * cc.y) + (v.z * cc.z + v.w * cc.w);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      y = fmaf(D, x, y);
+      if (a.z) y *= silu(to_f32(static_cast<const T*>(a.z)[(size_t)seq * a.z_stride + head * P + p]));
+      __syncwarp();
+      if (lane == 0) sy[k * P + p] = y;
+      ss = fmaf(y, y, ss);
+    }
+  }
+  float scale = 1.0f;
+  if (a.norm_w) {
+    if (lane == 0) red[warp] = ss;
+    __syncthreads();
+    if (tid == 0) {
+      float t = 0.0f;
+      for (int i = 0; i < kTokThreads / 32; ++i) t += red[i];
+      red[kTokThreads / 32] = t;
+    }
+    cl.sync();
+    float t = 0.0f;
+    for (int i = 0; i < c; ++i) t += *cl.map_shared_rank(red + kTokThreads / 32, i);
+    scale = rsqrtf(t / (float)(hpg * P) + a.eps);
+  } else {
+    __syncthreads();
+  }
+  T* out = static_cast<T*>(a.out) + (size_t)seq * a.out_stride;
+  for (int i = tid; i < mine * P; i += kTokThreads) {
+    const int k = i / P, ch = (grp * hpg + r + k * c) * P + i - k * P;
+    const float v = sy[i] * scale;
+    out[ch] = from_f32<T>(a.norm_w ? v * a.norm_w[ch] : v);
+  }
+  if (a.norm_w) cl.sync();  // the others' sums are read before a CTA leaves
+}
+
+// -------------------------------------------------------------- gated norm
+
+// g = y silu(z), out = w g / sqrt(mean(g^2) + eps) per group of channels; one
+// CTA per (token, group), two passes over rows that stay in L1.
+constexpr int kNormThreads = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads) gated_norm_kernel(NormArgs a) {
+  __shared__ float red[kNormThreads / 32];
+  const long long unit = blockIdx.x;
+  const long long t = unit / a.groups;
+  const int grp = (int)(unit - t * a.groups), tid = threadIdx.x;
+  const size_t off = (size_t)grp * a.group_size;
+  const T* y = static_cast<const T*>(a.y) + (size_t)t * a.y_stride + off;
+  const T* z = a.z ? static_cast<const T*>(a.z) + (size_t)t * a.z_stride + off : nullptr;
+  T* out = static_cast<T*>(a.out) + (size_t)t * a.out_stride + off;
+  float ss = 0.0f;
+  for (int i = tid; i < a.group_size; i += kNormThreads) {
+    const float g = to_f32(y[i]) * (z ? silu(to_f32(z[i])) : 1.0f);
+    ss = fmaf(g, g, ss);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if ((tid & 31) == 0) red[tid >> 5] = ss;
+  __syncthreads();
+  ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNormThreads / 32; ++i) ss += red[i];
+  const float scale = rsqrtf(ss / (float)a.group_size + a.eps);
+  for (int i = tid; i < a.group_size; i += kNormThreads) {
+    const float g = to_f32(y[i]) * (z ? silu(to_f32(z[i])) : 1.0f);
+    out[i] = from_f32<T>(g * scale * a.w[off + i]);
+  }
+}
+
+}  // namespace
+
+int launch_conv1d_prompt(const ConvArgs& a, cudaStream_t stream) {
+  const size_t e = a.type == kTypeBF16 ? 2 : 4;
+  const int v = (int)(16 / e);
+  const bool vec = a.channels % v == 0 && vec_ok(a.x, a.x_stride, e) && vec_ok(a.out, a.out_stride, e) &&
+                   vec_ok(a.state, a.channels, e);
+  if (a.type == kTypeBF16)
+    return vec ? launch_conv<__nv_bfloat16, 8>(a, stream) : launch_conv<__nv_bfloat16, 1>(a, stream);
+  return vec ? launch_conv<float, 4>(a, stream) : launch_conv<float, 1>(a, stream);
+}
+
+size_t ssm_prompt_scratch_bytes(int, int, int, int, int, int, int) { return 0; }
+
+int launch_ssm_prompt(const ScanArgs& a, cudaStream_t stream) {
+  return a.type == kTypeBF16 ? launch_scan_seq<__nv_bfloat16>(a, stream) : launch_scan_seq<float>(a, stream);
+}
+
+int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
+  const int hpg = a.heads / a.groups, c = hpg < 8 ? hpg : 8;
+  const size_t smem = (2 * (size_t)a.d_state + (size_t)((hpg + c - 1) / c) * a.head_dim + kTokThreads / 32 + 1) * 4;
+  const void* fn = a.type == kTypeBF16 ? (const void*)ssm_token_kernel<__nv_bfloat16>
+                                       : (const void*)ssm_token_kernel<float>;
+  if (smem > 48 * 1024) return kErrShape;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.seqs * a.groups * c));
+  cfg.blockDim = dim3(kTokThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = c;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TokenArgs copy = a;
+  void* args[] = {&copy};
+  return cudaLaunchKernelExC(&cfg, fn, args) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+int launch_gated_norm(const NormArgs& a, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((long long)a.tokens * a.groups);
+  if (a.type == kTypeBF16) gated_norm_kernel<__nv_bfloat16><<<grid, kNormThreads, 0, stream>>>(a);
+  else gated_norm_kernel<float><<<grid, kNormThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+}  // namespace ervf

@@ -570,6 +570,95 @@ ERVF_API int ervf_cache_fetch(const uint8_t* bank_c, const uint8_t* bank_s, uint
                      const int32_t* need, size_t code_bytes, size_t scale_bytes, int top_k,
                      void* stream);
 
+/* ---- dense and state-space operators of the hybrid's other layers ----
+ * Element types of activations, and activations of ervf_linear_bf16. */
+#define ERVF_F32 0
+#define ERVF_BF16 1
+#define ERVF_ACT_NONE 0
+#define ERVF_ACT_RELU2 1 /* relu(v)^2 */
+#define ERVF_ACT_SILU 2  /* v / (1 + exp(-v)) */
+#define ERVF_ACT_GELU 3  /* v (1 + erf(v / sqrt 2)) / 2 */
+
+/* Dense projection of any number of tokens, on the tensor cores:
+ * out[t][r] = act(sum_k W[r][k] x[t][k] + bias[r]) + resid[t][r].
+ * W bf16 [rows][cols]; x bf16, out and resid of out_type, their rows *_stride
+ * elements apart; bias f32.  bias, resid may be NULL; resid may be out
+ * itself (then with its stride), x must not overlap out.  Sums and epilogue
+ * in f32, one rounding to out_type, the same bits on every call.  cols and
+ * x_stride multiples of 8, W and x 16-byte aligned.  tokens = 0 does nothing.
+ * The reference projects one token at a time (gpu_kernels.py:21-49). */
+ERVF_API int ervf_linear_bf16(const uint16_t* W, const uint16_t* x, long long x_stride, const float* bias,
+                              const void* resid, long long resid_stride, void* out, long long out_stride,
+                              int out_type, int rows, int cols, int tokens, int act, void* stream);
+
+/* Packed sequences, for the prompt entry points: sequence i is tokens
+ * [cu_seqlens[i], cu_seqlens[i+1]) (int32, device, not decreasing, within
+ * [0, tokens]; it may be empty).  cu_seqlens NULL: one sequence of all tokens
+ * (seqs = 1).  Tokens of no sequence are neither read nor written.  Sequence
+ * i carries state slot slots[i] (int32, device; NULL: slot i), read only
+ * where has_state[i] is not zero (u8, device; NULL: nowhere) and left holding
+ * the state behind the sequence's last token.  A slot outside [0, n_slots)
+ * means none: a zero state, and nothing is stored.  No two sequences of one
+ * call may name the same slot. */
+
+/* Causal depthwise convolution of packed prompts: out[t][c] = act(bias[c] +
+ * sum_j w[c][j] x[t-width+1+j][c]), act = silu or none.  x, out, state of
+ * `type`; w f32 [channels][width], width 2..4; bias f32 or NULL; state
+ * [n_slots][width-1][channels], the last inputs, oldest first, or NULL (no
+ * sequence carries any).  out must not overlap x.  The reference: conv1d, one
+ * token at a time (gpu_kernels.py:77-1515). */
+ERVF_API int ervf_conv1d_prompt(const void* x, long long x_stride, const float* w, const float* bias,
+                                void* state, int n_slots, const int32_t* slots, const uint8_t* has_state,
+                                const int32_t* cu_seqlens, int seqs, void* out, long long out_stride, int type,
+                                int tokens, int channels, int width, int silu, void* stream);
+
+/* Selective state-space scan of packed prompts.  Per head h with group
+ * g = h / (heads / groups): d_t = softplus(dt[t][h] + dt_bias[h]),
+ * S_t = exp(d_t A[h]) S_{t-1} + d_t x[t][h] B[t][g]^T, y[t][h] = S_t C[t][g] +
+ * D[h] x[t][h].  x, y [tokens][heads][head_dim], B, C [tokens][groups][d_state]
+ * and dt [tokens][heads] of `type`, their token rows *_stride elements apart;
+ * A (not above 0), D, dt_bias f32 [heads], D and dt_bias may be NULL; state f32
+ * [n_slots][heads][head_dim][d_state] or NULL.  head_dim and d_state <= 256.
+ * scratch: ervf_ssm_prompt_scratch_bytes bytes, 16-byte aligned, need not be
+ * cleared; calls that share it must not overlap on the GPU.  y must not
+ * overlap an input.  The reference: softplus and ssm, one token at a time. */
+ERVF_API int ervf_ssm_prompt(const void* x, long long x_stride, const void* dt, long long dt_stride,
+                             const float* A, const void* B, long long b_stride, const void* C,
+                             long long c_stride, const float* D, const float* dt_bias, float* state, int n_slots,
+                             const int32_t* slots, const uint8_t* has_state, const int32_t* cu_seqlens, int seqs,
+                             void* y, long long y_stride, int type, int tokens, int heads, int head_dim,
+                             int groups, int d_state, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Bytes of scratch ervf_ssm_prompt uses for these sizes (0: none). */
+ERVF_API size_t ervf_ssm_prompt_scratch_bytes(int type, int tokens, int seqs, int heads, int head_dim,
+                                              int groups, int d_state);
+
+/* One token of each sequence through a state-space layer's convolution, scan
+ * and gated norm, one launch.  Row i of xbc holds x [heads * head_dim], B and C
+ * [groups * d_state] before the convolution (with silu); conv_state
+ * [n_slots][width-1][channels] as ervf_conv1d_prompt leaves it and state as
+ * ervf_ssm_prompt leaves it are updated in place.  y is multiplied by silu(z)
+ * (z NULL: not) and normalised per group of heads * head_dim / groups channels
+ * as ervf_gated_norm does (norm_w NULL: not).  Everything between the inputs
+ * and the output's one rounding is f32.  slots as above; d_state a multiple
+ * of 4, state 16-byte aligned.  out must not overlap an input.  The
+ * reference: conv1d, softplus, ssm, gated_rmsnorm (gpu_kernels.py:77-1515). */
+ERVF_API int ervf_ssm_token(const void* xbc, long long xbc_stride, const void* dt, long long dt_stride,
+                            const void* z, long long z_stride, const float* conv_w, const float* conv_bias,
+                            void* conv_state, const float* A, const float* D, const float* dt_bias,
+                            const float* norm_w, float eps, float* state, int n_slots, const int32_t* slots,
+                            void* out, long long out_stride, int type, int seqs, int heads, int head_dim,
+                            int groups, int d_state, int width, void* stream);
+
+/* Gated RMS norm: g = y silu(z) (z NULL: y), out = w g / sqrt(mean(g^2) + eps),
+ * the mean per group of group_size channels.  y, z, out of `type`, rows
+ * *_stride elements apart; w f32 [groups * group_size].  out may be y or z
+ * itself (with its stride).  The reference: gated_rmsnorm, one token at a
+ * time (gpu_kernels.py:77-1515). */
+ERVF_API int ervf_gated_norm(const void* y, long long y_stride, const void* z, long long z_stride,
+                             const float* w, float eps, void* out, long long out_stride, int type, int tokens,
+                             int groups, int group_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,144 @@
+"""The dense projection with its epilogue against 64 bits.
+
+Tolerance: bf16 products are exact in f32; a sum of `cols` of them in any
+order is off by at most cols * 2^-23 of the sum of their magnitudes (a step
+that truncates instead of rounding loses a whole unit in the last place), the
+epilogue's operations by a few 2^-24 of their values, the output by half a
+step of its type."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import hybrid_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(out, size, cols, dtype):
+    return ref.HALF[dtype] * out.abs() + (2 * cols + 32) * ref.U * size + 1e-30
+
+
+def make(rows, cols, tokens, dtype, bias, resid, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    W = (torch.randn(rows, cols, generator=g) * 0.1).bfloat16()
+    x = torch.randn(tokens, cols, generator=g).bfloat16()
+    b = torch.randn(rows, generator=g) if bias else None
+    r = torch.randn(tokens, rows, generator=g).to(dtype) if resid else None
+    return W, x, b, r
+
+
+def put(v, dev):
+    return None if v is None else v.to(dev)
+
+
+@pytest.fixture(scope="module")
+def k(cuda):
+    from ervf_b200 import GPUKernels
+
+    return GPUKernels()
+
+
+@pytest.mark.parametrize("rows,cols,tokens", [
+    (1, 8, 1), (7, 16, 3), (128, 64, 1), (129, 72, 33), (300, 1000, 17), (256, 4104, 2),
+    (1000, 264, 128), (257, 520, 129), (513, 136, 300), (2688, 4096, 1), (2688, 1856, 8),
+    (640, 328, 257), (1111, 88, 511), (20000, 64, 5), (96, 8192, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear(k, cuda, rows, cols, tokens, dtype):
+    W, x, b, r = make(rows, cols, tokens, dtype, True, True)
+    out = torch.full((tokens, rows), float("nan"), dtype=dtype, device=cuda)
+    k.linear_bf16(out, put(W, cuda), put(x, cuda), rows, cols, tokens, bias=put(b, cuda), act="silu",
+                  resid=put(r, cuda))
+    want, size = ref.linear(W, x, b, "silu", r)
+    ref.within(out, want, bound(want, size, cols, dtype))
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu"])
+@pytest.mark.parametrize("bias,resid", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("tokens", [3, 140])
+def test_epilogue(k, cuda, act, bias, resid, tokens):
+    W, x, b, r = make(200, 96, tokens, torch.float32, bias, resid, seed=1)
+    out = torch.empty(tokens, 200, device=cuda)
+    k.linear_bf16(out, put(W, cuda), put(x, cuda), 200, 96, tokens, bias=put(b, cuda), act=act, resid=put(r, cuda))
+    want, size = ref.linear(W, x, b, act, r)
+    ref.within(out, want, bound(want, size, 96, torch.float32))
+
+
+@pytest.mark.parametrize("tokens", [5, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_guards_and_residual_in_place(k, cuda, tokens, dtype):
+    """x and out are slices of wider rows; the bytes beside them stay as they were; resid is out."""
+    rows, cols = 331, 136
+    W, x, b, r = make(rows, cols, tokens, dtype, True, True, seed=2)
+    wide_x = torch.full((tokens, 200), float("nan"), dtype=torch.bfloat16, device=cuda)
+    wide_x[:, 32:32 + cols] = x.to(cuda)
+    wide = torch.full((tokens + 1, 400), 7.0, dtype=dtype, device=cuda)
+    view = wide[:tokens, 3:3 + rows]
+    view.copy_(r)
+    k.linear_bf16(view, put(W, cuda), wide_x[:, 32:32 + cols], rows, cols, tokens, bias=put(b, cuda), resid=view)
+    want, size = ref.linear(W, x, b, "none", r)
+    ref.within(view, want, bound(want, size, cols, dtype))
+    assert (wide[:, :3] == 7).all() and (wide[:, 3 + rows:] == 7).all() and (wide[tokens] == 7).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 200])
+def test_same_bits_every_call(k, cuda, tokens):
+    W, x, _, _ = make(2688, 4096, tokens, torch.float32, False, False, seed=3)
+    W, x = W.to(cuda), x.to(cuda)
+    outs = [torch.empty(tokens, 2688, device=cuda) for _ in range(3)]
+    for o in outs:
+        k.linear_bf16(o, W, x, 2688, 4096, tokens)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_infinities_stay_in_their_rows(k, cuda):
+    W, x, _, _ = make(130, 64, 150, torch.float32, False, False, seed=4)
+    x[17, 5], x[140, 9] = float("inf"), float("nan")
+    out = torch.empty(150, 130, device=cuda)
+    k.linear_bf16(out, put(W, cuda), put(x, cuda), 130, 64, 150, act="relu2")
+    clean = torch.isfinite(out).all(1).cpu()
+    assert [int(v) for v in (~clean).nonzero().flatten()] == [17, 140]
+    assert torch.isnan(out[140]).all()
+
+
+def test_no_tokens(k, cuda):
+    W = torch.zeros(16, 16, dtype=torch.bfloat16, device=cuda)
+    k.linear_bf16(torch.empty(0, 16, device=cuda), W, torch.empty(0, 16, dtype=torch.bfloat16, device=cuda), 16, 16, 0)
+
+
+def test_captured_and_replayed(k, cuda):
+    W, x, _, _ = make(384, 256, 70, torch.bfloat16, False, False, seed=5)
+    W, x = W.to(cuda), x.to(cuda)
+    out = torch.zeros(70, 384, dtype=torch.bfloat16, device=cuda)
+    want = torch.empty_like(out)
+    k.linear_bf16(want, W, x, 384, 256, 70)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        k.linear_bf16(out, W, x, 384, 256, 70)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    x.neg_()
+    k.linear_bf16(want, W, x, 384, 256, 70)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_wrong_arrays_are_refused(k, cuda):
+    W, x, _, _ = make(32, 64, 4, torch.float32, False, False)
+    W, x, out = W.to(cuda), x.to(cuda), torch.zeros(4, 32, device=cuda)
+    for bad in (dict(act="tanh"), dict(resid=torch.zeros(4, 32, device=cuda).bfloat16()),
+                dict(bias=torch.zeros(31, device=cuda)), dict(bias=torch.zeros(32)), ):
+        with pytest.raises(ValueError):
+            k.linear_bf16(out, W, x, 32, 64, 4, **bad)
+    with pytest.raises(ValueError):
+        k.linear_bf16(out, W, x.float(), 32, 64, 4)
+    with pytest.raises(ValueError):
+        k.linear_bf16(out, W, x, 32, 64, 5)
+    with pytest.raises(ValueError):
+        k.linear_bf16(out, W, x[:, 1:], 32, 56, 4)       # not 16-byte aligned
+    with pytest.raises(ValueError):
+        k.linear_bf16(out.half(), W, x, 32, 64, 4)
+    assert (out == 0).all()
