@@ -46,10 +46,10 @@ int ervf_version(void) { return 100; }
 
 int ervf_device_status(void) {
   // read and clear every unit's word; report the first error found
-  const int v[7] = {read_gemv_device_error(true), read_aux_device_error(true),
+  const int v[8] = {read_gemv_device_error(true), read_aux_device_error(true),
                     read_tc_device_error(true), read_ep_device_error(true),
                     read_mma_device_error(true), read_token_device_error(true),
-                    read_linear_device_error(true)};
+                    read_linear_device_error(true), read_scan_device_error(true)};
   for (int e : v)
     if (e) return e;
   return kOk;

@@ -178,6 +178,7 @@ int read_ep_device_error(bool clear);
 int read_mma_device_error(bool clear);
 int read_token_device_error(bool clear);
 int read_linear_device_error(bool clear);
+int read_scan_device_error(bool clear);
 
 // One decode token through every routed MoE layer in one launch
 // (moe_token.cu).  layer_ptrs: device array [5][n_layers] (+2 rows with the

@@ -8,6 +8,7 @@
 
 #include "common.cuh"
 #include "ssm.h"
+#include "ssm_dev.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -52,61 +53,6 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
   }
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
-// log(1 + exp(v)); above 20 the 1 is below half a unit in the last place
-__device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
-
-// Tokens [begin, begin + len) of sequence i, kept inside the token array
-// whatever the offsets say.
-__device__ __forceinline__ void seq_range(const Packing& p, int i, int& begin, int& len) {
-  if (!p.cu) {
-    begin = 0;
-    len = p.tokens;
-    return;
-  }
-  const int b = min(max(p.cu[i], 0), p.tokens), e = min(max(p.cu[i + 1], 0), p.tokens);
-  begin = b;
-  len = max(e - b, 0);
-}
-
-// State slot of sequence i, or -1 for none.
-__device__ __forceinline__ int seq_slot(const Packing& p, int i) {
-  const int s = p.slots ? p.slots[i] : i;
-  return s >= 0 && s < p.n_slots ? s : -1;
-}
-
-// Tile `tile` of the packed sequences, each cut into tiles of `size` tokens
-// from its own first token, an empty one into one: which sequence, and the
-// tile's place in it.  One warp; false past the last tile.
-__device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, int& seq, int& nth) {
-  const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int i0 = 0; i0 < p.seqs; i0 += 32) {
-    int n = 0;
-    if (i0 + lane < p.seqs) {
-      int b, len;
-      seq_range(p, i0 + lane, b, len);
-      n = max(1, (len + size - 1) / size);
-    }
-    int inc = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    const int total = __shfl_sync(0xffffffffu, inc, 31);
-    if (tile < base + total) {
-      const unsigned m = __ballot_sync(0xffffffffu, tile < base + inc);
-      const int l = __ffs(m) - 1;
-      seq = i0 + l;
-      nth = tile - base - __shfl_sync(0xffffffffu, inc - n, l);
-      return true;
-    }
-    base += total;
-  }
-  return false;
-}
-
 // ------------------------------------------------------------- convolution
 
 // y_t = act(bias + sum_j w[j] x[t - width + 1 + j]) for each channel.  A
@@ -120,8 +66,8 @@ constexpr int kConvTile = 32, kConvThreads = 128;
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
   const int ch = (blockIdx.y * kConvThreads + threadIdx.x) * V;
-  int seq, nth;
-  if (!find_tile(a.pk, blockIdx.x, kConvTile, seq, nth)) return;
+  int seq, nth, total;
+  if (!find_tile(a.pk, blockIdx.x, kConvTile, 1, seq, nth, total)) return;
   if (ch >= a.channels) return;
   int begin, len;
   seq_range(a.pk, seq, begin, len);
@@ -469,9 +415,7 @@ int launch_conv1d_prompt(const ConvArgs& a, cudaStream_t stream) {
   return vec ? launch_conv<float, 4>(a, stream) : launch_conv<float, 1>(a, stream);
 }
 
-size_t ssm_prompt_scratch_bytes(int, int, int, int, int, int, int) { return 0; }
-
-int launch_ssm_prompt(const ScanArgs& a, cudaStream_t stream) {
+int launch_scan_tokens(const ScanArgs& a, cudaStream_t stream) {
   return a.type == kTypeBF16 ? launch_scan_seq<__nv_bfloat16>(a, stream) : launch_scan_seq<float>(a, stream);
 }
 

@@ -59,6 +59,7 @@ struct ScanArgs {
 };
 size_t ssm_prompt_scratch_bytes(int type, int tokens, int seqs, int heads, int head_dim, int groups, int d_state);
 int launch_ssm_prompt(const ScanArgs& a, cudaStream_t stream);
+int launch_scan_tokens(const ScanArgs& a, cudaStream_t stream);  // token by token, any type and size
 
 struct TokenArgs {
   const void *xbc, *dt, *z;

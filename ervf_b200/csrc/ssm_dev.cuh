@@ -1,0 +1,68 @@
+// ssm_dev.cuh -- device helpers shared by the state-space kernels: packed
+// sequences and the scalar functions of the scan.
+#pragma once
+
+#include "common.cuh"
+#include "ssm.h"
+
+namespace ervf {
+
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+// log(1 + exp(v)); above 20 the 1 is below half a unit in the last place
+__device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+
+// Tokens [begin, begin + len) of sequence i, kept inside the token array
+// whatever the offsets say.
+__device__ __forceinline__ void seq_range(const Packing& p, int i, int& begin, int& len) {
+  if (!p.cu) {
+    begin = 0;
+    len = p.tokens;
+    return;
+  }
+  const int b = min(max(p.cu[i], 0), p.tokens), e = min(max(p.cu[i + 1], 0), p.tokens);
+  begin = b;
+  len = max(e - b, 0);
+}
+
+// State slot of sequence i, or -1 for none.
+__device__ __forceinline__ int seq_slot(const Packing& p, int i) {
+  const int s = p.slots ? p.slots[i] : i;
+  return s >= 0 && s < p.n_slots ? s : -1;
+}
+
+// Tile `tile` of the packed sequences, each cut into tiles of `size` tokens
+// from its own first token, an empty one into `empty` (0 or 1): which
+// sequence, and the tile's place in it.  One warp; false past the last tile,
+// with `total` the number of tiles.
+__device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, int empty, int& seq, int& nth,
+                                          int& total) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int i0 = 0; i0 < p.seqs; i0 += 32) {
+    int n = 0;
+    if (i0 + lane < p.seqs) {
+      int b, len;
+      seq_range(p, i0 + lane, b, len);
+      n = max(empty, (len - 1) / size + (len > 0));
+    }
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const int sum = __shfl_sync(0xffffffffu, inc, 31);
+    if (tile >= 0 && tile < base + sum) {
+      const unsigned m = __ballot_sync(0xffffffffu, tile < base + inc);
+      const int l = __ffs(m) - 1;
+      seq = i0 + l;
+      nth = tile - base - __shfl_sync(0xffffffffu, inc - n, l);
+      return true;
+    }
+    base += sum;
+  }
+  total = base;
+  return false;
+}
+
+}  // namespace ervf

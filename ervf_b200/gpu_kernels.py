@@ -36,6 +36,11 @@ _BF16 = (torch.bfloat16, torch.uint16, torch.int16)
 _CODE_TYPES = {_lib.F32: _F32, _lib.BF16: _BF16}
 
 
+# handle of torch's current stream on a device, without making a Stream object
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: int(torch.cuda.current_stream(index).cuda_stream))
+
+
 def _type_of(a, dtype, what: str) -> int:
     """Element type code of an activation array (f32, or bf16 as such or as its bits)."""
     if isinstance(a, torch.Tensor):
@@ -57,6 +62,7 @@ class GPUKernels:
             else torch.device(device)
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
         self.stream = None
 
     def _s(self) -> int:
@@ -95,20 +101,23 @@ class GPUKernels:
         _lib.call("ervf_f32_gemv", ptr(W), ptr(x), ptr(out), int(rows), int(cols), self._s())
 
     # ------------------------------------------------ argument checks
+    # A call's checks are part of a decode step's latency: the accepted case
+    # is decided with few attribute reads, the error text made afterwards.
     def _rows(self, a, rows: int, cols: int, code, what: str) -> tuple[int, int]:
         """Address and row stride of an activation array of `rows` rows."""
+        if a is None:
+            return 0, cols
         if isinstance(a, torch.Tensor):
-            if a.device != self.device:
-                raise ValueError(f"{what} is on {a.device}, this object launches on {self.device}")
-            if _TYPES.get(a.dtype) != code:
-                raise ValueError(f"{what}: elements of type {a.dtype} do not fit the other arrays")
-            if a.dim() == 2 and a.shape[0] >= rows and a.shape[1] >= cols and (cols == 1 or a.stride(1) == 1):
-                return a.data_ptr(), a.stride(0) if rows > 1 else cols
-            if a.numel() < rows * cols:
-                raise ValueError(f"{what} holds {a.numel()} elements, needs {rows * cols}")
-            if not a.is_contiguous():
-                raise ValueError(f"{what}: rows of contiguous elements are needed")
-        elif a is not None and not isinstance(a, int):
+            if a.get_device() == self._index and _TYPES.get(a.dtype) == code:
+                if a.dim() == 2:
+                    r, c = a.shape
+                    stride = a.stride()
+                    if r >= rows and c >= cols and (stride[1] == 1 or cols == 1):
+                        return a.data_ptr(), stride[0] if rows > 1 else cols
+                if a.numel() >= rows * cols and a.is_contiguous():
+                    return a.data_ptr(), cols
+            self._refuse(a, rows * cols, _CODE_TYPES[code], what)
+        if not isinstance(a, int):
             if _type_of(a, None, what) != code:
                 raise ValueError(f"{what}: its elements do not fit the other arrays")
             if a.__cuda_array_interface__.get("strides") is not None:
@@ -118,19 +127,25 @@ class GPUKernels:
 
     def _flat(self, a, n: int, dtypes, what: str) -> int:
         """Address of a contiguous parameter, state or index array (None: 0)."""
+        if a is None:
+            return 0
         if isinstance(a, torch.Tensor):
-            if a.device != self.device:
-                raise ValueError(f"{what} is on {a.device}, this object launches on {self.device}")
-            if a.dtype not in dtypes:
-                raise ValueError(f"{what}: elements of type {a.dtype} do not fit")
-            if a.numel() < n:
-                raise ValueError(f"{what} holds {a.numel()} elements, needs {n}")
-            if not a.is_contiguous():
-                raise ValueError(f"{what}: a contiguous array is needed")
-            return a.data_ptr()
-        if a is not None and not isinstance(a, int):
+            if (a.get_device() == self._index and a.dtype in dtypes and a.numel() >= n
+                    and a.is_contiguous()):
+                return a.data_ptr()
+            self._refuse(a, n, dtypes, what)
+        if not isinstance(a, int):
             _need(a, n, what)
         return ptr(a)
+
+    def _refuse(self, a, n: int, dtypes, what: str):
+        if a.get_device() != self._index:
+            raise ValueError(f"{what} is on {a.device}, this object launches on {self.device}")
+        if a.dtype not in dtypes:
+            raise ValueError(f"{what}: elements of type {a.dtype} do not fit, one of {dtypes} is needed")
+        if a.numel() < n:
+            raise ValueError(f"{what} holds {a.numel()} elements, needs {n}")
+        raise ValueError(f"{what}: rows of contiguous elements, {n} in all, are needed")
 
     @staticmethod
     def _slots_of(state, per_slot: int, n_slots, what: str) -> int:
@@ -143,11 +158,12 @@ class GPUKernels:
         return state.numel() // per_slot
 
     def _launch(self, name: str, *args) -> None:
-        if torch.cuda.current_device() == self.device.index:
-            _lib.call(name, *args, self._s())
+        stream = _raw_stream(self._index) if self.stream is None else int(self.stream.cuda_stream)
+        if torch.cuda.current_device() == self._index:
+            _lib.call(name, *args, stream)
         else:
             with torch.cuda.device(self.device):
-                _lib.call(name, *args, self._s())
+                _lib.call(name, *args, stream)
 
     # ------------------------------------------------ dense projection
     def linear_bf16(self, out, W, x, rows: int, cols: int, tokens: int, bias=None, act: str = "none",
