@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "kernels.h"
 #include "ssm.h"
 #include "ssm_dev.cuh"
 
@@ -56,15 +57,36 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
 // ------------------------------------------------------------- convolution
 
 // y_t = act(bias + sum_j w[j] x[t - width + 1 + j]) for each channel.  A
-// thread owns V channels of one tile of a sequence and keeps the window in
-// registers.  Bound by HBM: every input is read once (and `width - 1` rows
-// again per tile, from L2), every output written once.  The thread of a
-// sequence's first tile is the only one that touches the carried state: it
-// reads the old inputs, and writes the sequence's last `width - 1` ones.
-constexpr int kConvTile = 32, kConvThreads = 128;
+// thread owns V channels of one tile of a sequence, keeps the window in
+// registers and four tokens' loads in flight ahead of the four it works on.
+// Bound by HBM: every input is read once (and `width - 1` rows again per
+// tile, from L2), every output written once.  The thread of a sequence's
+// first tile is the only one that touches the carried state: it reads the old
+// inputs, and writes the sequence's last `width - 1` ones.
+constexpr int kConvTile = 32, kConvThreads = 128, kConvAhead = 4;
+
+// V elements as they lie in memory.
+template <typename T, int V>
+struct Raw {
+  static constexpr int kWords = V == 1 ? 1 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) {
+      if constexpr (sizeof(T) == 2) w[0] = *reinterpret_cast<const uint16_t*>(p);
+      else w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      const uint4 q = *reinterpret_cast<const uint4*>(p);
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  }
+};
 
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, 4) conv_prompt_kernel(ConvArgs a) {
   const int ch = (blockIdx.y * kConvThreads + threadIdx.x) * V;
   int seq, nth, total;
   if (!find_tile(a.pk, blockIdx.x, kConvTile, 1, seq, nth, total)) return;
@@ -73,17 +95,14 @@ __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
   seq_range(a.pk, seq, begin, len);
   const T* x = static_cast<const T*>(a.x) + (size_t)begin * a.x_stride + ch;
   T* out = static_cast<T*>(a.out) + (size_t)begin * a.out_stride + ch;
-  float w[V][W], bias[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    bias[v] = a.bias ? a.bias[ch + v] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[v][j] = a.w[(size_t)(ch + v) * W + j];
-  }
   const int slot = nth == 0 && a.state ? seq_slot(a.pk, seq) : -1;
   T* state = slot < 0 ? nullptr : static_cast<T*>(a.state) + (size_t)slot * (W - 1) * a.channels + ch;
-  float win[W - 1][V];  // the W - 1 inputs before the next one, oldest first
   const int t0 = nth * kConvTile, t1 = min(t0 + kConvTile, len);
+  Raw<T, V> next[kConvAhead];
+#pragma unroll
+  for (int u = 0; u < kConvAhead; ++u)
+    if (t0 + u < t1) next[u].load(x + (size_t)(t0 + u) * a.x_stride);
+  float win[W - 1][V];  // the W - 1 inputs before the next one, oldest first
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
     const int t = t0 - (W - 1) + j;
@@ -95,6 +114,13 @@ __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) win[j][v] = 0.0f;
     }
+  }
+  float w[V][W], bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    bias[v] = a.bias ? a.bias[ch + v] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[v][j] = a.w[(size_t)(ch + v) * W + j];
   }
   if (state) {
     // last W - 1 inputs of [carried state, sequence]
@@ -119,22 +145,31 @@ __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) store_vec<T, V>(state + (size_t)j * a.channels, last[j]);
   }
-#pragma unroll 4
-  for (int t = t0; t < t1; ++t) {
-    float cur[V], y[V];
-    load_vec<T, V>(x + (size_t)t * a.x_stride, cur);
+  for (int t = t0; t < t1; t += kConvAhead) {
+    Raw<T, V> cur[kConvAhead];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float s = bias[v];
+    for (int u = 0; u < kConvAhead; ++u) cur[u] = next[u];
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) s = fmaf(w[v][j], win[j][v], s);
-      s = fmaf(w[v][W - 1], cur[v], s);
-      y[v] = a.silu ? silu(s) : s;
+    for (int u = 0; u < kConvAhead; ++u)
+      if (t + kConvAhead + u < t1) next[u].load(x + (size_t)(t + kConvAhead + u) * a.x_stride);
 #pragma unroll
-      for (int j = 0; j + 1 < W - 1; ++j) win[j][v] = win[j + 1][v];
-      win[W - 2][v] = cur[v];
+    for (int u = 0; u < kConvAhead; ++u) {
+      if (t + u >= t1) break;
+      float y[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float c = cur[u].get(v);
+        float sum = bias[v];
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) sum = fmaf(w[v][j], win[j][v], sum);
+        sum = fmaf(w[v][W - 1], c, sum);
+        y[v] = a.silu ? silu(sum) : sum;
+#pragma unroll
+        for (int j = 0; j + 1 < W - 1; ++j) win[j][v] = win[j + 1][v];
+        win[W - 2][v] = c;
+      }
+      store_vec<T, V>(out + (size_t)(t + u) * a.out_stride, y);
     }
-    store_vec<T, V>(out + (size_t)t * a.out_stride, y);
   }
 }
 
@@ -257,12 +292,14 @@ int launch_scan_seq(const ScanArgs& a, cudaStream_t stream) {
 // which is what the launch costs for a batch (2 x 4 bytes per state element,
 // HBM bound); for one sequence it is latency: one round of loads, the
 // cluster's two barriers, one round of stores.
+//  0. the first rows of the first head's state start on their way;
 //  1. every CTA convolves its heads' x channels and, for itself, the group's
 //     B and C channels (2 d_state of them: recomputing is cheaper than
 //     sending them on);
 //  2. after a cluster barrier (every CTA has read the carried B / C inputs)
 //     CTA 0 shifts those inputs by one token;
-//  3. the states' update and y, one row of d_state per 32 lanes;
+//  3. the states' update and y: L lanes share a row of d_state, a warp works
+//     on 8 rows a lane at a time (128 bytes in flight each);
 //  4. the CTAs' sums of squares meet in shared memory of each (added in rank
 //     order), then the norm and the output.
 constexpr int kTokThreads = 256;
@@ -283,8 +320,11 @@ __device__ __forceinline__ void conv_shift(const TokenArgs& a, const T* xin, T* 
   cs[(size_t)(a.width - 2) * pitch + ch] = xin[ch];
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kTokThreads) ssm_token_kernel(TokenArgs a) {
+// L lanes of four columns each share a row, NV times over.
+template <typename T, int L, int NV>
+__global__ void __launch_bounds__(kTokThreads, 3) ssm_token_kernel(TokenArgs a) {
+  constexpr int kRows = 8 / NV;                              // rows of a lane at a time
+  constexpr int kStep = kTokThreads / L, kBatch = kRows * kStep;  // rows of the CTA
   extern __shared__ __align__(16) float sm[];
   cg::cluster_group cl = cg::this_cluster();
   const int c = (int)cl.num_blocks(), r = (int)cl.block_rank();
@@ -299,6 +339,23 @@ __global__ void __launch_bounds__(kTokThreads) ssm_token_kernel(TokenArgs a) {
   const int slot = s0 >= 0 && s0 < a.n_slots ? s0 : -1;
   const T* xin = static_cast<const T*>(a.xbc) + (size_t)seq * a.xbc_stride;
   const size_t channels = (size_t)a.heads * P + 2 * (size_t)a.groups * N;
+  const int sub = tid / L, n0 = (tid % L) * 4;
+  float4 v[kRows][NV];
+  // rows p0 + sub, p0 + sub + kStep, ... of a head's state
+  auto load = [&](const float* st, int p0) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int p = p0 + i * kStep + sub, n = n0 + k * 4 * L;
+        v[i][k] = st && p < P && n < N ? *reinterpret_cast<const float4*>(st + (size_t)p * N + n)
+                                       : make_float4(0, 0, 0, 0);
+      }
+  };
+  auto state_of = [&](int k) {
+    return slot < 0 ? nullptr : a.state + ((size_t)slot * a.heads + grp * hpg + r + k * c) * P * N;
+  };
+  load(state_of(0), 0);
   T* cs = slot < 0 ? nullptr : static_cast<T*>(a.conv_state) + (size_t)slot * (a.width - 1) * channels;
   for (int i = tid; i < 2 * N; i += kTokThreads) {
     const int ch = a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N);
@@ -319,30 +376,45 @@ __global__ void __launch_bounds__(kTokThreads) ssm_token_kernel(TokenArgs a) {
     const float d = softplus(to_f32(static_cast<const T*>(a.dt)[(size_t)seq * a.dt_stride + head]) +
                              (a.dt_bias ? a.dt_bias[head] : 0.0f));
     const float da = expf(d * a.A[head]), D = a.D ? a.D[head] : 0.0f;
-    float* st = slot < 0 ? nullptr : a.state + ((size_t)slot * a.heads + head) * P * N;
-    for (int p = warp; p < P; p += kTokThreads / 32) {
-      const float x = sy[k * P + p], dx = d * x;
-      float y = 0.0f;
-      for (int n = lane * 4; n < N; n += 128) {
-        float4 v = st ? *reinterpret_cast<const float4*>(st + (size_t)p * N + n) : make_float4(0, 0, 0, 0);
-        const float4 b = *reinterpret_cast<const float4*>(sBC + n);
-        const float4 cc = *reinterpret_cast<const float4*>(sBC + N + n);
-        v.x = fmaf(dx, b.x, da * v.x);
-        v.y = fmaf(dx, b.y, da * v.y);
-        v.z = fmaf(dx, b.z, da * v.z);
-        v.w = fmaf(dx, b.w, da * v.w);
-        if (st) *reinterpret_cast<float4*>(st + (size_t)p * N + n) = v;
-        y += (v.x * cc.x + v.y * cc.y) + (v.z * cc.z + v.w * cc.w);
-      }
+    float* st = state_of(k);
+    for (int p0 = 0; p0 < P; p0 += kBatch) {
+      if (k + p0 > 0) load(st, p0);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-      y = fmaf(D, x, y);
-      if (a.z) y *= silu(to_f32(static_cast<const T*>(a.z)[(size_t)seq * a.z_stride + head * P + p]));
-      __syncwarp();
-      if (lane == 0) sy[k * P + p] = y;
-      ss = fmaf(y, y, ss);
+      for (int i = 0; i < kRows; ++i) {
+        const int p = p0 + i * kStep + sub;
+        const float x = p < P ? sy[k * P + p] : 0.0f, dx = d * x;
+        float y = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int n = n0 + j * 4 * L;
+          if (n < N) {
+            const float4 b = *reinterpret_cast<const float4*>(sBC + n);
+            const float4 cc = *reinterpret_cast<const float4*>(sBC + N + n);
+            float4 q = v[i][j];
+            q.x = fmaf(dx, b.x, da * q.x);
+            q.y = fmaf(dx, b.y, da * q.y);
+            q.z = fmaf(dx, b.z, da * q.z);
+            q.w = fmaf(dx, b.w, da * q.w);
+            if (st && p < P) *reinterpret_cast<float4*>(st + (size_t)p * N + n) = q;
+            y += (q.x * cc.x + q.y * cc.y) + (q.z * cc.z + q.w * cc.w);
+          }
+        }
+#pragma unroll
+        for (int o = L / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+        if (p < P) {
+          y = fmaf(D, x, y);
+          if (a.z) y *= silu(to_f32(static_cast<const T*>(a.z)[(size_t)seq * a.z_stride + head * P + p]));
+          if (n0 == 0) {
+            ss = fmaf(y, y, ss);
+            sy[k * P + p] = y;  // its x was read by this row's lanes, together
+          }
+        }
+        __syncwarp();
+      }
     }
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   float scale = 1.0f;
   if (a.norm_w) {
     if (lane == 0) red[warp] = ss;
@@ -368,12 +440,76 @@ __global__ void __launch_bounds__(kTokThreads) ssm_token_kernel(TokenArgs a) {
   if (a.norm_w) cl.sync();  // the others' sums are read before a CTA leaves
 }
 
+template <typename T>
+const void* token_kernel(int d_state) {
+  if (d_state <= 32) return (const void*)ssm_token_kernel<T, 8, 1>;
+  if (d_state <= 64) return (const void*)ssm_token_kernel<T, 16, 1>;
+  if (d_state <= 128) return (const void*)ssm_token_kernel<T, 32, 1>;
+  return (const void*)ssm_token_kernel<T, 32, 2>;
+}
+
 // -------------------------------------------------------------- gated norm
 
-// g = y silu(z), out = w g / sqrt(mean(g^2) + eps) per group of channels; one
-// CTA per (token, group), two passes over rows that stay in L1.
+// g = y silu(z), out = w g / sqrt(mean(g^2) + eps) per group of channels.
+// Bound by HBM.  A warp holds one group's row in registers (NV vectors of 16
+// bytes a lane) and its weights for all the tokens that it walks.
 constexpr int kNormThreads = 128;
 
+template <typename T, int NV>
+__global__ void __launch_bounds__(kNormThreads) gated_norm_warp_kernel(NormArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, grp = blockIdx.y;
+  const size_t off = (size_t)grp * a.group_size;
+  const T* y = static_cast<const T*>(a.y) + off;
+  const T* z = a.z ? static_cast<const T*>(a.z) + off : nullptr;
+  T* out = static_cast<T*>(a.out) + off;
+  float w[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const int i = (k * 32 + lane) * V + j;
+      const float4 q = i < a.group_size ? make_float4(a.w[off + i], a.w[off + i + 1], a.w[off + i + 2], a.w[off + i + 3])
+                                        : make_float4(0, 0, 0, 0);
+      w[k][j] = q.x; w[k][j + 1] = q.y; w[k][j + 2] = q.z; w[k][j + 3] = q.w;
+    }
+  const long long step = (long long)gridDim.x * (kNormThreads / 32);
+  for (long long t = (long long)blockIdx.x * (kNormThreads / 32) + (threadIdx.x >> 5); t < a.tokens; t += step) {
+    Raw<T, V> ry[NV], rz[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * 32 + lane) * V;
+      if (i < a.group_size) {
+        ry[k].load(y + (size_t)t * a.y_stride + i);
+        if (z) rz[k].load(z + (size_t)t * a.z_stride + i);
+      }
+    }
+    float g[NV][V], ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if ((k * 32 + lane) * V < a.group_size) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          g[k][j] = z ? ry[k].get(j) * silu(rz[k].get(j)) : ry[k].get(j);
+          ss = fmaf(g[k][j], g[k][j], ss);
+        }
+      }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float scale = rsqrtf(ss / (float)a.group_size + a.eps);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * 32 + lane) * V;
+      if (i < a.group_size) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[k][j] *= scale * w[k][j];
+        store_vec<T, V>(out + (size_t)t * a.out_stride + i, g[k]);
+      }
+    }
+  }
+}
+
+// Any size and alignment: one CTA per (token, group), two passes over a row.
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads) gated_norm_kernel(NormArgs a) {
   __shared__ float red[kNormThreads / 32];
@@ -399,8 +535,28 @@ __global__ void __launch_bounds__(kNormThreads) gated_norm_kernel(NormArgs a) {
   const float scale = rsqrtf(ss / (float)a.group_size + a.eps);
   for (int i = tid; i < a.group_size; i += kNormThreads) {
     const float g = to_f32(y[i]) * (z ? silu(to_f32(z[i])) : 1.0f);
-    out[i] = from_f32<T>(g * scale * a.w[off + i]);
+    out[i] = from_f32<T>(g * (scale * a.w[off + i]));
   }
+}
+
+template <typename T>
+int launch_norm(const NormArgs& a, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int nv = (a.group_size + 32 * V - 1) / (32 * V);
+  // a row of up to four vectors a lane stays in registers
+  if (a.group_size % V == 0 && nv <= 4 && a.groups <= 65535 && vec_ok(a.y, a.y_stride, sizeof(T)) &&
+      vec_ok(a.z, a.z ? a.z_stride : 0, sizeof(T)) && vec_ok(a.out, a.out_stride, sizeof(T))) {
+    const long long rows = ((long long)a.tokens + kNormThreads / 32 - 1) / (kNormThreads / 32);
+    const long long most = (8LL * device_sm_count() + a.groups - 1) / a.groups;  // 32 warps a SM, walking
+    const dim3 grid((unsigned)(rows < most ? rows : most), a.groups);
+    if (nv == 1) gated_norm_warp_kernel<T, 1><<<grid, kNormThreads, 0, stream>>>(a);
+    else if (nv == 2) gated_norm_warp_kernel<T, 2><<<grid, kNormThreads, 0, stream>>>(a);
+    else if (nv == 3) gated_norm_warp_kernel<T, 3><<<grid, kNormThreads, 0, stream>>>(a);
+    else gated_norm_warp_kernel<T, 4><<<grid, kNormThreads, 0, stream>>>(a);
+  } else {
+    gated_norm_kernel<T><<<(unsigned)((long long)a.tokens * a.groups), kNormThreads, 0, stream>>>(a);
+  }
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace
@@ -422,8 +578,7 @@ int launch_scan_tokens(const ScanArgs& a, cudaStream_t stream) {
 int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
   const int hpg = a.heads / a.groups, c = hpg < 8 ? hpg : 8;
   const size_t smem = (2 * (size_t)a.d_state + (size_t)((hpg + c - 1) / c) * a.head_dim + kTokThreads / 32 + 1) * 4;
-  const void* fn = a.type == kTypeBF16 ? (const void*)ssm_token_kernel<__nv_bfloat16>
-                                       : (const void*)ssm_token_kernel<float>;
+  const void* fn = a.type == kTypeBF16 ? token_kernel<__nv_bfloat16>(a.d_state) : token_kernel<float>(a.d_state);
   if (smem > 48 * 1024) return kErrShape;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.seqs * a.groups * c));
@@ -442,10 +597,7 @@ int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
 }
 
 int launch_gated_norm(const NormArgs& a, cudaStream_t stream) {
-  const unsigned grid = (unsigned)((long long)a.tokens * a.groups);
-  if (a.type == kTypeBF16) gated_norm_kernel<__nv_bfloat16><<<grid, kNormThreads, 0, stream>>>(a);
-  else gated_norm_kernel<float><<<grid, kNormThreads, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  return a.type == kTypeBF16 ? launch_norm<__nv_bfloat16>(a, stream) : launch_norm<float>(a, stream);
 }
 
 }  // namespace ervf

@@ -1,14 +1,15 @@
 // ssm_chunk.cu -- the selective scan of bf16 prompts on the sm_100a tensor
 // cores, in chunks of Q = 128 tokens:
 //
-//   P[t][s] = (C_t . B_s) exp(c_t - c_s) d_s  for s <= t, + D on the diagonal
-//   y_t     = sum_s P[t][s] x_s + exp(c_t) S C_t
+//   P[t][s] = (C_t . B_s) exp(c_t - c_s) d_s  for s <= t
+//   y_t     = sum_s P[t][s] x_s + exp(c_t) S C_t + D x_t
 //   S'      = exp(c_Q) S + sum_s exp(c_Q - c_s) d_s x_s B_s^T
 //
 // with c the running sum of d A inside the chunk and S the state before it.
 // One CTA per SM walks a list of (head pair, sequence, chunk) steps and carries
 // the two heads' state in registers; C B^T is shared by the pair.  The list
 // is cut into equal pieces, one per CTA, wherever the cuts fall:
+//   pass 0  softplus, running sums and weights of every (head, chunk)
 //   pass 1  (WHOLE = false) a CTA whose piece ends inside a sequence computes
 //           the state that its own part of that sequence adds, and its decay;
 //   pass 2  joins these along each sequence, in order;
@@ -16,22 +17,29 @@
 // Exponents are sums of numbers of one sign (distances within blocks of 32
 // tokens plus whole blocks), so no difference of two long sums is taken but
 // inside a block.  Products meet the tensor cores in bf16: B, C and x are bf16
-// already; P and S are split into two bf16 numbers (off by 2^-16 of the
-// value, the output's own rounding is 2^-8), the state's new terms into three
-// (2^-24: states stay f32).
+// already.  The in-chunk weights P are rounded to bf16 once (2^-8 of each
+// term at most, as the output's own rounding; two parts would cost the tensor
+// memory that lets both heads' P be in work at once); D x is added in f32.  S is split into two
+// bf16 numbers for S C (2^-16), the state's new terms into three (2^-24: states
+// stay f32).
 //
-// Warps, and what bounds them at 128 state columns (clocks per step of two
-// heads, measured tcgen05 rates):
-//   0..3   P: C B^T from tensor memory, weighted, split, back to tensor memory
-//          as an A operand; scales S C by exp(c_t) in tensor memory
-//   4..11  states: x scaled and split into the B operand of the state's new
-//          terms; the f32 state (64 registers a thread), split for S C
-//   12..15 y: tensor memory -> bf16 -> coalesced rows
-//   16     TMA of the B, C and x tiles
-//   17     all MMAs: C B^T 8 x 65, S C 16 x 69, P x 32 x 68, states 24 x 69
-//          = 5460 clocks, which is the step's bound
-//   18     steps: softplus, running sums, weights; clears rows behind a
-//          sequence's end, so that a neighbour's NaN meets no zero weight
+// Warps (a warpgroup's register share in brackets), and what bounds them at
+// 128 state columns (clocks per step of two heads, measured tcgen05 rates):
+//   0..7   P [80]: C B^T from tensor memory, weighted, back to tensor memory
+//          as an A operand; S C to exp(c_t) S C + D x in tensor memory
+//   8..15  states [96]: the f32 state, 64 registers a thread; split for S C
+//   16..23 W [56]: x scaled to the chunk's end and split into three, 32 tokens
+//          at a time, as the B operand of the state's new terms; then y, tensor
+//          memory -> bf16 -> rows, while the next x tile is on its way
+//   24     TMA of the B, C and x tiles and of the steps
+//   25     MMAs of y: C B^T 8 x 65, S C 16 x 69, P x 16 x 68
+//   26     MMAs of the state's new terms: 24 x 69; with 25's, 4370 clocks
+//   27     clears rows behind a sequence's end, so that a neighbour's NaN meets
+//          no zero weight
+// Both operands of a 128-column MMA in shared memory take its whole bandwidth
+// (128 bytes a clock); with W, the split state and the tiles a step moves 800 KB
+// there, 6250 clocks.
+// In pass 1 warps 0..7 do W's work too.
 // Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
 // dead, and every role leaves; copies and MMAs are drained first.
 #include <cuda.h>  // CUtensorMap and the encode function's types (driver entry point)
@@ -46,11 +54,29 @@ namespace {
 
 constexpr int kQ = 128, kP = 64;          // tokens per chunk, head_dim
 constexpr int kPanel = kQ * 128;          // 128 rows of 64 bf16, 128-byte swizzle
-constexpr int kHalfPanel = 64 * 128;
-constexpr int kChWarps = 19, kChThreads = kChWarps * 32;
+constexpr int kWRows = 32, kWPanel = kWRows * 128;  // tokens of a W buffer, one part of one head of it
+constexpr int kChWarps = 28, kChThreads = kChWarps * 32;
+// registers a thread at launch, and each warpgroup's after its split: the
+// shares must not exceed what the block was launched with
+constexpr int kRegs = 72, kRegP = 80, kRegS = 96, kRegW = 56, kRegMisc = 40;
+static_assert(2 * kRegP + 2 * kRegS + 2 * kRegW + kRegMisc <= 7 * kRegs, "register shares");
 constexpr int kMaxCtas = 148;
 // tensor-memory columns
-constexpr int kTmCB = 0, kTmP = 128, kTmY = 256, kTmS = 384;
+constexpr int kTmCB = 0, kTmP = 128, kTmY = 256, kTmS = 384;  // P: 64 columns a head
+
+// Per-token numbers of one head in one chunk, base-2 exponents.
+struct alignas(16) Steps {
+  float lp[kQ];  // running sum inside the token's block of 32, inclusive
+  float d[kQ];   // softplus step, 0 behind the end
+  float v[kQ];   // d exp2(distance to the end of the token's block)
+  float w[kQ];   // d exp2(distance to the end of the chunk)
+  float blk[4];  // sums of the blocks
+  float all;     // exp2(sum of the chunk)
+  float sum;     // sum of the chunk
+  float D;
+  float pad;
+};
+static_assert(sizeof(Steps) % 16 == 0, "bulk copies");
 
 struct ChunkArgs {
   Packing pk;
@@ -61,43 +87,45 @@ struct ChunkArgs {
   long long dt_stride, y_stride;
   int heads, hpg, ppg, pairs;  // heads, heads and pairs per group, pairs in all
   int n;                       // d_state
+  Steps* steps;                // [pair][chunk][2]
   float* local;                // [ctas][2][kP][n]: pass 1's states, joined in place by pass 2
   float* init;                 // [ctas][2][kP][n]: carried states of sequences that are cut
   float* decay;                // [ctas][2]
-  int* meta;                   // [ctas]: 0 no cut, 1 from a sequence's start, 2 continued
+  int* meta;                   // [ctas]: 0 no cut, else pair * 4 + (1 from a sequence's start, 2 continued)
+};
+
+// kStages tiles of B and x: pass 1 has the room of C, S and y.  Two teams scale
+// x, each into a W buffer of its own (a team may run a step ahead of the
+// other: buffers taken in turns would need more than a parity to tell their
+// rounds apart).
+template <bool WHOLE>
+struct Depth {
+  static constexpr int kStages = WHOLE ? 1 : 2, kWBufs = 2, kTeam = WHOLE ? 128 : 256;
 };
 
 struct Barriers {
-  uint64_t raw_b, raw_c, raw_x;   // TMA bytes landed
-  uint64_t rdy_b, rdy_x;          // and rows behind the end cleared
+  uint64_t raw_b[2], raw_c, raw_x[2];  // TMA bytes landed
+  uint64_t rdy_b[2], rdy_x[2];         // and rows behind the end cleared
   uint64_t sc_full[2], sc_free[2];
-  uint64_t cb_full, cb_free, cs_done, p_full, px_done[2], y_free;
-  uint64_t w_full[3], w_free[3], ds_done, ds_free, s_full, x_read, mma_done;
+  uint64_t cb_full, cb_free, cs_done, p_full[2], px_done[2], y_free;
+  uint64_t w_full[2], w_free[2], ds_done, ds_free, b_free[2], s_full, x_read[2], mma_done;
 };
 
-// Per-token numbers of one head, base-2 exponents.
-struct alignas(16) Steps {
-  float lp[kQ];  // running sum inside the token's block of 32, inclusive
-  float d[kQ];   // softplus step, 0 behind the end
-  float v[kQ];   // d exp2(distance to the end of the token's block)
-  float w[kQ];   // d exp2(distance to the end of the chunk)
-  float blk[4];  // sums of the blocks
-  float all;     // exp2(sum of the chunk)
-};
-
-template <int N>
+template <int N, bool WHOLE>
 struct ChunkSmem {
+  using Dp = Depth<WHOLE>;
   static constexpr int kTile = N / 64 * kPanel;    // B or C
-  static constexpr int kB = 0, kC = kB + kTile, kX = kC + kTile;
-  static constexpr int kS = kX + 2 * kPanel;       // [hi, lo][head][N rows]
+  static constexpr int kB = 0, kX = kB + Dp::kStages * kTile;
+  static constexpr int kW = kX + Dp::kStages * 2 * kPanel;  // [buffer][part][head][rows]
+  static constexpr int kC = kW + Dp::kWBufs * 6 * kWPanel;
+  static constexpr int kS = kC + (WHOLE ? kTile : 0);       // [hi, lo][head][N rows]
   static constexpr int kSPanel = N * 128;
-  static constexpr int kW = kS + 4 * kSPanel;      // 3 parts x [head][64 rows]
-  static constexpr int kY = kW + 6 * kHalfPanel;   // 4 warps x 2 KB
-  static constexpr int kSteps = kY + 4 * 2048;     // [2 buffers][2 heads]
-  static constexpr int kBar = (kSteps + 4 * (int)sizeof(Steps) + 15) / 16 * 16;
+  static constexpr int kY = kS + (WHOLE ? 4 * kSPanel : 0); // 8 warps x 1 KB
+  static constexpr int kSteps = kY + (WHOLE ? 8 * 1024 : 0);  // [2 buffers][2 heads]
+  static constexpr int kBar = kSteps + 4 * (int)sizeof(Steps);
   static constexpr int kBytes = 1024 + kBar + 512;
 };
-static_assert(ChunkSmem<128>::kBytes <= 232448, "shared memory");
+static_assert(ChunkSmem<128, true>::kBytes <= 232448 && ChunkSmem<128, false>::kBytes <= 232448, "shared memory");
 
 __device__ __forceinline__ float ex2(float v) {
   float r;
@@ -160,12 +188,25 @@ __device__ __forceinline__ void tm_st32(uint32_t t, const uint32_t (&v)[32]) {
         "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void tm_ld16(uint32_t t, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(t));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tm_st16(uint32_t t, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
         "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+__device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -178,19 +219,30 @@ __device__ __forceinline__ void ch_tma(void* dst, const CUtensorMap* map, int x,
       ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
 
-// Bounded wait of one thread; gives up too when another role died.
+// The box into L2 ahead of its load.
+__device__ __forceinline__ void ch_prefetch(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+
+__device__ __noinline__ void ch_timeout(volatile int* dead) {
+  atomicExch(&g_device_error, kErrTimeout);
+  *dead = 1;
+}
+
+// Bounded wait of one thread: kChTries tries, each of which the hardware may
+// suspend for up to 20 us; gives up too when another role died.  Small on
+// purpose: with some forty waits in line, a clock to watch in each made the
+// kernel 97 KB long, and its warps waited for instructions.
+constexpr int kChTries = 100000;
+
 __device__ __forceinline__ bool ch_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait_sleep(bar, parity, 200)) {
+#pragma unroll 1
+  for (int i = 0; i < kChTries; ++i) {
+    if (mbar_try_wait_sleep(bar, parity, 20000)) return true;
     if (*dead) return false;
-    if (clock64() - t0 > 2000000000LL) {
-      atomicExch(&g_device_error, kErrTimeout);
-      *dead = 1;
-      return false;
-    }
   }
-  return true;
+  ch_timeout(dead);
+  return false;
 }
 // The same for a whole warp: one decision.
 __device__ __forceinline__ bool ch_wait_w(uint64_t* bar, uint32_t parity, volatile int* dead) {
@@ -230,21 +282,90 @@ struct Walk {
   __device__ int valid() const { return min(kQ, len - chunk * kQ); }
 };
 
+// Heads of a pair; an odd group's last pair has its head twice.
+struct Heads {
+  int grp, h[2];
+  __device__ Heads(const ChunkArgs& a, int pair) {
+    grp = pair / a.ppg;
+    const int k = (pair - grp * a.ppg) * 2;
+    h[0] = grp * a.hpg + k;
+    h[1] = k + 1 < a.hpg ? h[0] + 1 : h[0];
+  }
+};
+
 // First and one-past-last step of CTA c out of g.
 __device__ __forceinline__ long long cut(long long steps, int c, int g) { return steps * c / g; }
+
+// Two f32 to their bf16 rounding and to the bf16 rounding of what it leaves.
+__device__ __forceinline__ void split2(float e, float o, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(e, o);
+  lo = pack2(e - lo_f(hi), o - hi_f(hi));
+}
+
+// W: a team scales x of step `it` to the chunk's end and splits it into three,
+// kWRows tokens of both heads at a time: every second such quarter of the chunk.
+template <int N, bool WHOLE>
+__device__ __forceinline__ bool scale_x(uint8_t* smem, Barriers& br, int team, int it, volatile int* dead) {
+  using Sm = ChunkSmem<N, WHOLE>;
+  constexpr int STG = Depth<WHOLE>::kStages, NT = Depth<WHOLE>::kTeam;
+  const Steps* st = reinterpret_cast<const Steps*>(smem + Sm::kSteps) + 2 * (it & 1);
+  const int stg = it % STG, wt = threadIdx.x & (NT - 1);
+  if (!ch_wait_w(&br.sc_full[it & 1], (it >> 1) & 1, dead)) return false;
+  if (!ch_wait_w(&br.rdy_x[stg], (it / STG) & 1, dead)) return false;
+  const uint8_t* xt = smem + Sm::kX + stg * 2 * kPanel;
+#pragma unroll 1
+  for (int qt = team; qt < kQ / kWRows; qt += 2) {
+    // the buffer's rounds 2 it, 2 it + 1
+    if (!ch_wait_w(&br.w_free[team], (qt >> 1) ^ 1, dead)) return false;
+    uint8_t* wb = smem + Sm::kW + team * 6 * kWPanel;
+#pragma unroll 2
+    for (int i = 0; i < 2 * kWRows * 8 / NT; ++i) {
+      const int id = i * NT + wt, h = id >> 8, r = (id >> 3) & 31, ch = id & 7;
+      const int row = kWRows * qt + r;
+      const float w = st[h].w[row];
+      const uint32_t off = (uint32_t)((ch ^ (r & 7)) << 4);
+      const uint4 xv = *reinterpret_cast<const uint4*>(xt + h * kPanel + row * 128 + off);
+      const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
+      uint32_t p0[4], p1[4], p2[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float e = lo_f(xs[j]) * w, o = hi_f(xs[j]) * w;
+        p0[j] = pack2(e, o);
+        e -= lo_f(p0[j]);
+        o -= hi_f(p0[j]);
+        split2(e, o, p1[j], p2[j]);
+      }
+      uint8_t* dst = wb + h * kWPanel + r * 128 + off;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+      *reinterpret_cast<uint4*>(dst + 2 * kWPanel) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+      *reinterpret_cast<uint4*>(dst + 4 * kWPanel) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
+    }
+    to_async();
+    ch_arrive_w(&br.w_full[team]);
+  }
+  ch_arrive_w(&br.x_read[stg]);
+  ch_arrive_w(&br.sc_free[it & 1]);
+  return true;
+}
+
+template <int R>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
 template <int N, bool WHOLE>
 __global__ void __launch_bounds__(kChThreads, 1)
     scan_chunk_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap b_map,
                       const __grid_constant__ CUtensorMap c_map, ChunkArgs a) {
-  using Sm = ChunkSmem<N>;
+  using Sm = ChunkSmem<N, WHOLE>;
+  constexpr int STG = Depth<WHOLE>::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   Barriers& br = *reinterpret_cast<Barriers*>(smem + Sm::kBar);
   static_assert(sizeof(Barriers) <= 400, "barrier block");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Sm::kBar + 400);
   volatile int* dead = reinterpret_cast<volatile int*>(smem + Sm::kBar + 404);
-  int* first = reinterpret_cast<int*>(smem + Sm::kBar + 408);  // pair, seq, chunk, steps, piece before
+  int* first = reinterpret_cast<int*>(smem + Sm::kBar + 408);  // pair, seq, chunk, steps, piece before, chunks, chunk of all
   Steps* steps = reinterpret_cast<Steps*>(smem + Sm::kSteps);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, ctas = gridDim.x;
@@ -283,37 +404,41 @@ __global__ void __launch_bounds__(kChThreads, 1)
       first[2] = nth;
       first[3] = n;
       first[4] = before;
-      if (!WHOLE) a.meta[cta] = n == 0 ? 0 : nth == 0 ? 1 : 2;
-      const int cons = WHOLE ? 12 : 8;  // warps that read the steps
-      mbar_init(&br.raw_b, 1);
-      mbar_init(&br.raw_c, 1);
-      mbar_init(&br.raw_x, 1);
-      mbar_init(&br.rdy_b, 1);
-      mbar_init(&br.rdy_x, 1);
+      first[5] = total;
+      first[6] = (int)((WHOLE ? f0 : f1 - n) % max(total, 1));
+      if (!WHOLE) a.meta[cta] = n == 0 ? 0 : (pair << 2) + (nth == 0 ? 1 : 2);
+      // warps that scale x, and that read the steps
+      const int scalers = WHOLE ? 8 : 16, cons = 8 + scalers + (WHOLE ? 8 : 0);
       for (int i = 0; i < 2; ++i) {
+        mbar_init(&br.raw_b[i], 1);
+        mbar_init(&br.raw_x[i], 1);
+        mbar_init(&br.rdy_b[i], 1);
+        mbar_init(&br.rdy_x[i], 1);
         mbar_init(&br.sc_full[i], 1);
         mbar_init(&br.sc_free[i], cons);
         mbar_init(&br.px_done[i], 1);
+        mbar_init(&br.b_free[i], 1);
+        mbar_init(&br.x_read[i], scalers);
+        mbar_init(&br.p_full[i], 8);
       }
-      mbar_init(&br.cb_full, 1);
-      mbar_init(&br.cb_free, 4);
-      mbar_init(&br.cs_done, 1);
-      mbar_init(&br.p_full, 4);
-      mbar_init(&br.y_free, 4);
-      for (int i = 0; i < 3; ++i) {
-        mbar_init(&br.w_full[i], 8);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&br.w_full[i], Depth<WHOLE>::kTeam / 32);
         mbar_init(&br.w_free[i], 1);
       }
+      mbar_init(&br.raw_c, 1);
+      mbar_init(&br.cb_full, 1);
+      mbar_init(&br.cb_free, 8);
+      mbar_init(&br.cs_done, 1);
+      mbar_init(&br.y_free, 8);
       mbar_init(&br.ds_done, 1);
       mbar_init(&br.ds_free, 8);
       mbar_init(&br.s_full, 8);
-      mbar_init(&br.x_read, 8);
-      mbar_init(&br.mma_done, 1);
+      mbar_init(&br.mma_done, 2);
       *dead = 0;
       fence_mbar_init();
     }
   }
-  if (warp == 17) {
+  if (warp == 25) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -325,347 +450,330 @@ __global__ void __launch_bounds__(kChThreads, 1)
   const int count = first[3];
   Walk wk;
   if (count > 0) wk.at(a.pk, first[0], first[1], first[2]);
-  // heads of a pair; an odd group's last pair has its head twice
-  auto head_of = [&](int pair, int h) {
-    const int grp = pair / a.ppg, k = (pair - grp * a.ppg) * 2 + h;
-    return grp * a.hpg + min(k, a.hpg - 1);
-  };
-  auto two = [&](int pair) { return (pair % a.ppg) * 2 + 1 < a.hpg; };
+  const int q = warp & 3;  // tensor-memory lanes 32 q ..
+  const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ------------------------------------------------------------------ P
-    if (WHOLE && count > 0) {
-      const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
-      {
+    // Lanes are tokens t; the two warps of a lane quarter share its blocks of
+    // 32 tokens s: q, q - 2 for the first, q - 1, q - 3 for the second (of two
+    // below the diagonal, the second takes both).
+    regs_up<kRegP>();
+    if (!WHOLE) {
+      for (int it = 0; it < count; ++it)
+        if (!scale_x<N, WHOLE>(smem, br, 0, it, dead)) break;
+    } else if (count > 0) {
+      const int side = warp >> 2, t = 32 * q + lane;
+      if (side == 1) {
         // columns behind the diagonal block stay zero
-        uint32_t z[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = 0;
-        for (int j = warp + 1; j < 4; ++j) {
-          tm_st16(lanes + kTmP + 16 * j, z);
-          tm_st16(lanes + kTmP + 64 + 16 * j, z);
+        const uint32_t z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int c = 16 * (q + 1); c < 64; c += 8) {
+          tm_st8(lanes + kTmP + c, z);
+          tm_st8(lanes + kTmP + 64 + c, z);
         }
         tm_wait_st();
       }
       for (int it = 0; it < count; ++it) {
         const uint32_t ph = it & 1;
-        const Steps* st2 = steps + 2 * ph;
         if (!ch_wait_w(&br.sc_full[ph], (it >> 1) & 1, dead)) break;
         if (!ch_wait_w(&br.cb_full, ph, dead)) break;
-        tc_after();
         bool ok = true;
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          const Steps& st = st2[h];
-          const int t = 32 * warp + lane;
-          const float lp = st.lp[t];
-          // the P buffer is free: the last product of it is done
-          if (!ch_wait_w(&br.px_done[h ^ 1], h ? ph : ph ^ 1, dead)) {
+          const Steps& st = steps[2 * ph + h];
+          const float lp = st.lp[t], b1 = st.blk[1], b2 = st.blk[2];
+          // this head's P buffer is free: its last product is done
+          if (!ch_wait_w(&br.px_done[h], ph ^ 1, dead)) {
             ok = false;
             break;
           }
           tc_after();
-          float before = lp;  // distance from the end of block j to t
-          for (int j = warp; j >= 0; --j) {
-            uint32_t v[32], hi[16], lo[16];
+#pragma unroll 1
+          for (int j = q - side; j >= 0; j -= (q == 2 && side == 1) ? 1 : 2) {
+            if (q == 2 && j == 0 && side == 0) break;
+            uint32_t v[32];
             tm_ld32(lanes + kTmCB + 32 * j, v);
-            if (j == warp) {
-              const float D = a.D ? a.D[head_of(wk.pair, h)] : 0.0f;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float p = __uint_as_float(v[i]) * (st.d[32 * j + i] * ex2(lp - st.lp[32 * j + i]));
-                v[i] = __float_as_uint(i < lane ? p : i == lane ? p + D : 0.0f);
-              }
-            } else {
-              const float u = ex2(before);
-              before += st.blk[j];
+            uint32_t o[16];
+            if (j == q) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(&st.v[32 * j + i]);
-                v[i] = __float_as_uint(__uint_as_float(v[i]) * (u * q.x));
-                v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) * (u * q.y));
-                v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) * (u * q.z));
-                v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) * (u * q.w));
+                const float4 ls = *reinterpret_cast<const float4*>(&st.lp[32 * j + i]);
+                const float4 ds = *reinterpret_cast<const float4*>(&st.d[32 * j + i]);
+                const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {ds.x, ds.y, ds.z, ds.w};
+                float p[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  p[k] = __uint_as_float(v[i + k]) * (dv[k] * ex2(lp - lv[k]));
+                  if (i + k > lane) p[k] = 0.0f;
+                }
+                o[i / 2] = pack2(p[0], p[1]);
+                o[i / 2 + 1] = pack2(p[2], p[3]);
+              }
+            } else {
+              // from the end of block j to t: whole blocks between, then t's own part
+              const float u = ex2(lp + (j + 1 < q ? (j == 0 ? b1 : b2) : 0.0f) + (j + 2 < q ? b2 : 0.0f));
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(&st.v[32 * j + i]);
+                o[i / 2] = pack2(__uint_as_float(v[i]) * (u * w.x), __uint_as_float(v[i + 1]) * (u * w.y));
+                o[i / 2 + 1] = pack2(__uint_as_float(v[i + 2]) * (u * w.z), __uint_as_float(v[i + 3]) * (u * w.w));
               }
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e = __uint_as_float(v[2 * i]), o = __uint_as_float(v[2 * i + 1]);
-              hi[i] = pack2(e, o);
-              lo[i] = pack2(e - lo_f(hi[i]), o - hi_f(hi[i]));
-            }
-            tm_st16(lanes + kTmP + 16 * j, hi);
-            tm_st16(lanes + kTmP + 64 + 16 * j, lo);
+            tm_st16(lanes + kTmP + 64 * h + 16 * j, o);
           }
           if (h == 1) {
             tc_before();
             ch_arrive_w(&br.cb_free);
           }
-          // S C of this head times exp(c_t)
-          if (h == 0 && !ch_wait_w(&br.cs_done, ph, dead)) {
-            ok = false;
-            break;
-          }
+          // half of this head's row: S C times exp(c_t), plus D x
+          if (h == 0) ok = ch_wait_w(&br.cs_done, ph, dead) && ch_wait_w(&br.rdy_x[0], ph, dead);
+          if (!ok) break;
           tc_after();
-          const float e = ex2(before);  // every block before t's, and t's own part
-#pragma unroll
-          for (int c = 0; c < 64; c += 32) {
+          {
+            const float e = ex2(lp + (q > 0 ? st.blk[0] : 0.0f) + (q > 1 ? b1 : 0.0f) + (q > 2 ? b2 : 0.0f));
+            const float D = st.D;
             uint32_t v[32];
-            tm_ld32(lanes + kTmY + 64 * h + c, v);
+            tm_ld32(lanes + kTmY + 64 * h + 32 * side, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * e);
-            tm_st32(lanes + kTmY + 64 * h + c, v);
+            for (int c = 0; c < 4; ++c) {
+              const uint4 xv = *reinterpret_cast<const uint4*>(smem + Sm::kX + h * kPanel + t * 128 +
+                                                               (((4 * side + c) ^ (t & 7)) << 4));
+              const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                v[8 * c + 2 * i] = __float_as_uint(fmaf(D, lo_f(xs[i]), __uint_as_float(v[8 * c + 2 * i]) * e));
+                v[8 * c + 2 * i + 1] =
+                    __float_as_uint(fmaf(D, hi_f(xs[i]), __uint_as_float(v[8 * c + 2 * i + 1]) * e));
+              }
+            }
+            tm_st32(lanes + kTmY + 64 * h + 32 * side, v);
           }
           tm_wait_st();
           tc_before();
-          ch_arrive_w(&br.p_full);
+          ch_arrive_w(&br.p_full[h]);
         }
         if (!ok) break;
         ch_arrive_w(&br.sc_free[ph]);
-        if (it + 1 < count) wk.next(a.pk);
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // ------------------------------------------------------------- states
-    const int q = warp & 3, half = (warp - 4) >> 2;  // state rows 32 q .., columns 32 half ..
-    const int n = 32 * q + lane, wt = tid - 128;
+    regs_up<kRegS>();
+    const int half = (warp - 8) >> 2;  // state rows 32 q .., columns 32 half ..
+    const int n = 32 * q + lane;
     const bool own = n < N;
     float s[2][32];
-    auto put_s = [&]() {
-      // both parts of both heads' state as the B operand of S C
-      if (own) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float e = s[h][8 * c + 2 * i], o = s[h][8 * c + 2 * i + 1];
-              hi[i] = pack2(e, o);
-              lo[i] = pack2(e - lo_f(hi[i]), o - hi_f(hi[i]));
-            }
-            uint8_t* p = smem + Sm::kS + h * Sm::kSPanel + n * 128 + (((4 * half + c) ^ (n & 7)) << 4);
-            *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(p + 2 * Sm::kSPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-      }
-      to_async();
-      ch_arrive_w(&br.s_full);
-    };
-    // this thread's elements of a pair of states [2][kP][N] or of the heads' slots
-    auto elem = [&](float* base, int h, int i) { return base + ((size_t)h * kP + 32 * half + i) * N + n; };
+    // offset of this thread's element i of a head's [kP][N] state
+    auto at = [&](int i) { return (size_t)(32 * half + i) * N + n; };
     for (int it = 0; it < count; ++it) {
       const uint32_t ph = it & 1;
-      const Steps* st2 = steps + 2 * ph;
       if (wk.chunk == 0 || it == 0) {
         // where the state before this chunk comes from
         const int slot = a.state ? seq_slot(a.pk, wk.seq) : -1;
-        const bool carried = slot >= 0 && a.pk.has && a.pk.has[wk.seq];
+        const Heads hd(a, wk.pair);
         const float* src = nullptr;
         bool slots = false;
         if (wk.chunk > 0) {
           if (WHOLE) src = a.local + (size_t)first[4] * 2 * kP * N;
-        } else if (carried) {
+        } else if (slot >= 0 && a.pk.has && a.pk.has[wk.seq]) {
           // a sequence that another CTA finishes may already have its new state in the slot
-          const bool is_cut = WHOLE && wk.nch - wk.chunk > count - it;
-          if (is_cut) src = a.init + (size_t)cta * 2 * kP * N;
+          if (WHOLE && wk.nch > count - it) src = a.init + (size_t)cta * 2 * kP * N;
           else slots = true;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float* p = slots ? a.state + ((size_t)slot * a.heads + head_of(wk.pair, h)) * kP * N
+          const float* p = slots ? a.state + ((size_t)slot * a.heads + hd.h[h]) * kP * N
                                  : src ? src + (size_t)h * kP * N : nullptr;
+          if (p && own) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[h][i] = p && own ? p[(size_t)(32 * half + i) * N + n] : 0.0f;
-          if (!WHOLE && slots && own) {
+            for (int i = 0; i < 32; ++i) s[h][i] = p[at(i)];
+            if (!WHOLE) {
+              float* o = a.init + ((size_t)cta * 2 + h) * kP * N;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) *elem(a.init + (size_t)cta * 2 * kP * N, h, i) = s[h][i];
+              for (int i = 0; i < 32; ++i) o[at(i)] = s[h][i];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[h][i] = 0.0f;
           }
-        }
-        if (WHOLE) {
-          if (!ch_wait_w(&br.cs_done, ph ^ 1, dead)) break;
-          put_s();
         }
       }
-      if (!ch_wait_w(&br.sc_full[ph], (it >> 1) & 1, dead)) break;
-      if (!ch_wait_w(&br.rdy_x, ph, dead)) break;
-      bool ok = true;
-      for (int hf = 0; hf < 2; ++hf) {
-        // x rows 64 hf .., scaled to the chunk's end, in three bf16 parts
-        for (int i = 0; i < 3 && ok; ++i) ok = ch_wait_w(&br.w_free[i], hf ^ 1, dead);
-        if (!ok) break;
+      if (WHOLE) {
+        // both parts of both heads' state as the B operand of S C
+        if (!ch_wait_w(&br.cs_done, ph ^ 1, dead)) break;
+        if (own) {
+          uint8_t* row = smem + Sm::kS + n * 128;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int id = i * 256 + wt, h = id >> 9, r = (id >> 3) & 63, ch = id & 7;
-          const int row = 64 * hf + r;
-          const float w = st2[h].w[row];
-          const uint32_t at = (uint32_t)((ch ^ (r & 7)) << 4);
-          const uint4 xv = *reinterpret_cast<const uint4*>(smem + Sm::kX + h * kPanel + row * 128 + at);
-          const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
-          uint32_t p0[4], p1[4], p2[4];
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float e = lo_f(xs[j]) * w, o = hi_f(xs[j]) * w;
-            p0[j] = pack2(e, o);
-            e -= lo_f(p0[j]);
-            o -= hi_f(p0[j]);
-            p1[j] = pack2(e, o);
-            e -= lo_f(p1[j]);
-            o -= hi_f(p1[j]);
-            p2[j] = pack2(e, o);
-          }
-          uint8_t* dst = smem + Sm::kW + h * kHalfPanel + r * 128 + at;
-          *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-          *reinterpret_cast<uint4*>(dst + 2 * kHalfPanel) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
-          *reinterpret_cast<uint4*>(dst + 4 * kHalfPanel) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) split2(s[h][8 * c + 2 * i], s[h][8 * c + 2 * i + 1], hi[i], lo[i]);
+              uint8_t* p = row + h * Sm::kSPanel + (((4 * half + c) ^ (n & 7)) << 4);
+              *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4*>(p + 2 * Sm::kSPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
         }
         to_async();
-        __syncwarp();
-        if (lane == 0)
-          for (int i = 0; i < 3; ++i) mbar_arrive(&br.w_full[i]);
+        ch_arrive_w(&br.s_full);
       }
-      if (!ok) break;
-      ch_arrive_w(&br.x_read);
+      if (!ch_wait_w(&br.sc_full[ph], (it >> 1) & 1, dead)) break;
+      const float d0 = steps[2 * ph].all, d1 = steps[2 * ph + 1].all;
+      ch_arrive_w(&br.sc_free[ph]);
       if (!ch_wait_w(&br.ds_done, ph, dead)) break;
       tc_after();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t v[32];
-        __syncwarp();
-        tm_ld32(tmem + ((uint32_t)(32 * q) << 16) + kTmS + 64 * h + 32 * half, v);
-        const float da = st2[h].all;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s[h][i] = fmaf(da, s[h][i], __uint_as_float(v[i]));
-      }
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[16];
+          tm_ld16(lanes + kTmS + 64 * h + 32 * half + 16 * c, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[h][16 * c + i] = fmaf(h ? d1 : d0, s[h][16 * c + i], __uint_as_float(v[i]));
+        }
       tc_before();
       ch_arrive_w(&br.ds_free);
-      ch_arrive_w(&br.sc_free[ph]);
       if (WHOLE && wk.chunk == wk.nch - 1) {
         const int slot = a.state ? seq_slot(a.pk, wk.seq) : -1;
+        const Heads hd(a, wk.pair);
         if (slot >= 0 && own)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            if (h == 0 || two(wk.pair)) {
-              float* p = a.state + ((size_t)slot * a.heads + head_of(wk.pair, h)) * kP * N;
+            if (h == 0 || hd.h[1] != hd.h[0]) {
+              float* o = a.state + ((size_t)slot * a.heads + hd.h[h]) * kP * N;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) *elem(p, 0, i) = s[h][i];
+              for (int i = 0; i < 32; ++i) o[at(i)] = s[h][i];
             }
       }
-      if (it + 1 < count) {
-        wk.next(a.pk);
-        if (WHOLE && wk.chunk > 0) {
-          if (!ch_wait_w(&br.cs_done, ph, dead)) break;
-          put_s();
-        }
-      }
+      if (it + 1 < count) wk.next(a.pk);
     }
     if (!WHOLE && count > 0 && own) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        float* o = a.local + ((size_t)cta * 2 + h) * kP * N;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) *elem(a.local + (size_t)cta * 2 * kP * N, h, i) = s[h][i];
-    }
-  } else if (warp < 16) {
-    // ------------------------------------------------------------------ y
-    if (WHOLE) {
-      const int q = warp & 3;
-      uint8_t* stage = smem + Sm::kY + q * 2048;
-      for (int it = 0; it < count; ++it) {
-        const uint32_t ph = it & 1;
-        bool ok = true;
-        for (int h = 0; h < 2; ++h) {
-          if (!ch_wait_w(&br.px_done[h], ph, dead)) {
-            ok = false;
-            break;
-          }
-          tc_after();
-          uint32_t o[32];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t v[32];
-            tm_ld32(tmem + ((uint32_t)(32 * q) << 16) + kTmY + 64 * h + 32 * c, v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              o[16 * c + i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-          }
-          if (h == 1) {
-            tc_before();
-            ch_arrive_w(&br.y_free);
-          }
-          if (h == 1 && !two(wk.pair)) continue;
-          const int left = wk.valid() - 32 * q;  // rows of this warp inside the sequence
-          __nv_bfloat16* y = a.y + (size_t)(wk.row0() + 32 * q) * a.y_stride + (size_t)head_of(wk.pair, h) * kP;
-          // 16 rows at a time through shared memory: eight lanes store one row's 128 bytes
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            __syncwarp();
-            if ((lane >> 4) == g) {
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(stage + (lane & 15) * 128 + ((c ^ (lane & 7)) << 4)) =
-                    make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = 4 * k + (lane >> 3), c = lane & 7;
-              const uint4 val = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
-              if (16 * g + r < left)
-                *reinterpret_cast<uint4*>(y + (size_t)(16 * g + r) * a.y_stride + 8 * c) = val;
-            }
-          }
-        }
-        if (!ok) break;
-        if (it + 1 < count) wk.next(a.pk);
+        for (int i = 0; i < 32; ++i) o[at(i)] = s[h][i];
       }
     }
-  } else if (warp == 16) {
-    // ---------------------------------------------------------------- TMA
-    if (lane == 0) {
-      int it = 0;
-      for (; it < count; ++it) {
-        const uint32_t ph = it & 1;
-        const int grp = wk.pair / a.ppg, row = wk.row0();
-        if (WHOLE) {
-          if (!ch_wait(&br.cs_done, ph ^ 1, dead)) break;
-          mbar_arrive_expect_tx(&br.raw_c, Sm::kTile);
+  } else if (warp < 24) {
+    // ------------------------------------------------------------ W, then y
+    regs_down<kRegW>();
+    const int side = (warp - 16) >> 2;
+    uint8_t* stage = smem + Sm::kY + (warp - 16) * 1024;
+    for (int it = 0; it < count; ++it) {
+      if (!scale_x<N, WHOLE>(smem, br, WHOLE ? side : 1, it, dead)) break;
+      if (!WHOLE) continue;
+      const int left = wk.valid() - 32 * q;  // rows of this warp inside the sequence
+      const Heads hd(a, wk.pair);
+      __nv_bfloat16* rows = a.y + (size_t)(wk.row0() + 32 * q) * a.y_stride + 32 * side;
+      bool ok = true;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if (!ch_wait_w(&br.px_done[h], it & 1, dead)) {
+          ok = false;
+          break;
+        }
+        tc_after();
+        uint32_t v[32];
+        tm_ld32(lanes + kTmY + 64 * h + 32 * side, v);
+        if (h == 1) {
+          tc_before();
+          ch_arrive_w(&br.y_free);
+          if (hd.h[1] == hd.h[0]) break;
+        }
+        __nv_bfloat16* y = rows + (size_t)(h ? hd.h[1] : hd.h[0]) * kP;
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        // 16 rows of 64 bytes at a time through shared memory: four lanes store one row's
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          __syncwarp();
+          if ((lane >> 4) == g) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(stage + (lane & 15) * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int r = 8 * k + (lane >> 2), i = lane & 3;
+            const uint4 val = *reinterpret_cast<const uint4*>(stage + r * 64 + ((i ^ ((r >> 1) & 3)) << 4));
+            if (16 * g + r < left) *reinterpret_cast<uint4*>(y + (size_t)(16 * g + r) * a.y_stride + 8 * i) = val;
+          }
+        }
+      }
+      if (!ok) break;
+      if (it + 1 < count) wk.next(a.pk);
+    }
+  } else {
+    regs_down<kRegMisc>();
+    if (warp == 24) {
+      // -------------------------------------------------------------- TMA
+      if (lane == 0) {
+        // the list walks the chunks pair after pair, as the steps lie
+        const Steps* src = a.steps + 2 * ((size_t)first[0] * first[5] + first[6]);
+        for (int it = 0; it < count; ++it) {
+          const uint32_t ph = it & 1, sph = (it / STG) & 1;
+          const Heads hd(a, wk.pair);
+          const int grp = hd.grp, row = wk.row0(), stg = it % STG;
+          if (!ch_wait(&br.sc_free[ph], ((it >> 1) & 1) ^ 1, dead)) break;
+          mbar_arrive_expect_tx(&br.sc_full[ph], 2 * sizeof(Steps));
+          bulk_g2s(steps + 2 * ph, src, 2 * sizeof(Steps), &br.sc_full[ph]);
+          src += 2;
+          if (WHOLE) {
+            if (!ch_wait(&br.cs_done, ph ^ 1, dead)) break;
+            mbar_arrive_expect_tx(&br.raw_c, Sm::kTile);
+            for (int i = 0; i < N / 64; ++i)
+              ch_tma(smem + Sm::kC + i * kPanel, &c_map, grp * N + 64 * i, row, &br.raw_c);
+          }
+          if (WHOLE && !ch_wait(&br.cb_full, ph ^ 1, dead)) break;
+          if (!ch_wait(&br.b_free[stg], sph ^ 1, dead)) break;
+          mbar_arrive_expect_tx(&br.raw_b[stg], Sm::kTile);
           for (int i = 0; i < N / 64; ++i)
-            ch_tma(smem + Sm::kC + i * kPanel, &c_map, grp * N + 64 * i, row, &br.raw_c);
+            ch_tma(smem + Sm::kB + stg * Sm::kTile + i * kPanel, &b_map, grp * N + 64 * i, row, &br.raw_b[stg]);
+          if (WHOLE && !ch_wait(&br.px_done[1], ph ^ 1, dead)) break;
+          if (!ch_wait(&br.x_read[stg], sph ^ 1, dead)) break;
+          mbar_arrive_expect_tx(&br.raw_x[stg], 2 * kPanel);
+          for (int h = 0; h < 2; ++h)
+            ch_tma(smem + Sm::kX + (2 * stg + h) * kPanel, &x_map, hd.h[h] * kP, row, &br.raw_x[stg]);
+          if (it + 1 < count) {
+            wk.next(a.pk);
+            const Heads nx(a, wk.pair);
+            for (int i = 0; i < N / 64; ++i) {
+              if (WHOLE) ch_prefetch(&c_map, nx.grp * N + 64 * i, wk.row0());
+              ch_prefetch(&b_map, nx.grp * N + 64 * i, wk.row0());
+            }
+            for (int h = 0; h < 2; ++h) ch_prefetch(&x_map, nx.h[h] * kP, wk.row0());
+          }
         }
-        if (!ch_wait(&br.ds_done, ph ^ 1, dead)) break;
-        mbar_arrive_expect_tx(&br.raw_b, Sm::kTile);
-        for (int i = 0; i < N / 64; ++i)
-          ch_tma(smem + Sm::kB + i * kPanel, &b_map, grp * N + 64 * i, row, &br.raw_b);
-        if (WHOLE && !ch_wait(&br.px_done[1], ph ^ 1, dead)) break;
-        if (!ch_wait(&br.x_read, ph ^ 1, dead)) break;
-        mbar_arrive_expect_tx(&br.raw_x, 2 * kPanel);
-        for (int h = 0; h < 2; ++h)
-          ch_tma(smem + Sm::kX + h * kPanel, &x_map, head_of(wk.pair, h) * kP, row, &br.raw_x);
-        if (it + 1 < count) wk.next(a.pk);
-      }
-      // no copy is left in flight: wait for every one that was started (a
-      // dead CTA's waits return at once, so these go by the clock alone)
-      if (*dead) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000) {
+        // no copy is left in flight: wait for the last ones (a dead CTA's
+        // waits return at once, so there a millisecond by the clock)
+        if (*dead) {
+          const long long t0 = clock64();
+          while (clock64() - t0 < 2000000) {
+          }
+        } else {
+          for (int it = count > STG ? count - STG : 0; it < count; ++it) {
+            const uint32_t sph = (it / STG) & 1;
+            if (WHOLE) ch_wait(&br.raw_c, it & 1, dead);
+            ch_wait(&br.raw_b[it % STG], sph, dead);
+            ch_wait(&br.raw_x[it % STG], sph, dead);
+            ch_wait(&br.sc_full[it & 1], (it >> 1) & 1, dead);
+          }
         }
-      } else if (count > 0) {
-        const uint32_t ph = (count - 1) & 1;
-        if (WHOLE) ch_wait(&br.raw_c, ph, dead);
-        ch_wait(&br.raw_b, ph, dead);
-        ch_wait(&br.raw_x, ph, dead);
       }
-    }
-  } else if (warp == 17) {
-    // --------------------------------------------------------------- MMAs
-    if (lane == 0) {
-      const uint32_t base = smem_u32(smem);
-      constexpr uint32_t id_cb = ch_idesc(128, false, false), id_cs = ch_idesc(128, false, true),
-                         id_px = ch_idesc(64, false, true), id_ds = ch_idesc(128, true, true);
-      for (int it = 0; it < count; ++it) {
-        const uint32_t ph = it & 1;
-        if (!ch_wait(&br.rdy_b, ph, dead)) break;
-        if (WHOLE) {
+    } else if (warp == 25) {
+      // -------------------------------------------------------- MMAs of y
+      if (lane == 0) {
+        const uint32_t base = smem_u32(smem);
+        constexpr uint32_t id_cb = ch_idesc(128, false, false), id_cs = ch_idesc(128, false, true),
+                           id_px = ch_idesc(64, false, true);
+        for (int it = 0; WHOLE && it < count; ++it) {
+          const uint32_t ph = it & 1;
+          if (!ch_wait(&br.rdy_b[0], ph, dead)) break;
           if (!ch_wait(&br.raw_c, ph, dead)) break;
           if (!ch_wait(&br.cb_free, ph ^ 1, dead)) break;
           tc_after();
@@ -685,147 +793,163 @@ __global__ void __launch_bounds__(kChThreads, 1)
               mma_ss(tmem + kTmY, sw_desc(base + Sm::kC + (k >> 2) * kPanel + (k & 3) * 32, 16),
                      sw_desc(base + Sm::kS + part * 2 * Sm::kSPanel + k * 2048, Sm::kSPanel), id_cs, part + k > 0);
           ch_commit(&br.cs_done);
-          if (!ch_wait(&br.rdy_x, ph, dead)) break;
-          if (!ch_wait(&br.p_full, 0, dead)) break;  // phases 2 it, 2 it + 1
-          tc_after();
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mma_ts(tmem + kTmY, tmem + kTmP + 64 * part + 8 * k, sw_desc(base + Sm::kX + k * 2048, 16), id_px);
-          ch_commit(&br.px_done[0]);
-        }
-        if (!ch_wait(&br.ds_free, ph ^ 1, dead)) break;
-        bool ok = true;
-        for (int hf = 0; hf < 2 && ok; ++hf)
-          for (int part = 0; part < 3; ++part) {
-            if (!ch_wait(&br.w_full[part], hf, dead)) {
+          if (!ch_wait(&br.rdy_x[0], ph, dead)) break;
+          bool ok = true;
+          for (int h = 0; h < 2; ++h) {
+            if (!ch_wait(&br.p_full[h], ph, dead)) {
               ok = false;
               break;
             }
             tc_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              // fewer than 128 state columns: the rows behind them repeat the first (panel stride 0)
-              mma_ss(tmem + kTmS, sw_desc(base + Sm::kB + (64 * hf + 16 * k) * 128, N == 128 ? kPanel : 0),
-                     sw_desc(base + Sm::kW + part * 2 * kHalfPanel + k * 2048, kHalfPanel), id_ds,
-                     hf + part + k > 0);
-            ch_commit(&br.w_free[part]);
-          }
-        if (!ok) break;
-        ch_commit(&br.ds_done);
-        if (WHOLE) {
-          if (!ch_wait(&br.p_full, 1, dead)) break;
-          tc_after();
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
             for (int k = 0; k < 8; ++k)
-              mma_ts(tmem + kTmY + 64, tmem + kTmP + 64 * part + 8 * k,
-                     sw_desc(base + Sm::kX + kPanel + k * 2048, 16), id_px);
-          ch_commit(&br.px_done[1]);
+              mma_ts(tmem + kTmY + 64 * h, tmem + kTmP + 64 * h + 8 * k,
+                     sw_desc(base + Sm::kX + h * kPanel + k * 2048, 16), id_px);
+            ch_commit(&br.px_done[h]);
+          }
+          if (!ok) break;
         }
+        // every MMA is complete before tensor memory is freed
+        ch_commit(&br.mma_done);
+        mbar_wait(&br.mma_done, 0, 2000000000LL);
       }
-      // every MMA is complete before tensor memory is freed
-      ch_commit(&br.mma_done);
-      mbar_wait(&br.mma_done, 0, 2000000000LL);
-    }
-  } else {
-    // -------------------------------------------------------------- steps
-    const float log2e = 1.4426950408889634f;
-    float sum[2] = {0.0f, 0.0f};  // pass 1: exponent of the whole part
-    for (int it = 0; it < count; ++it) {
-      const uint32_t ph = it & 1;
-      const int valid = wk.valid(), row = wk.row0();
-      float d[2][4];
+    } else if (warp == 26) {
+      // --------------------------------------- MMAs of the state's new terms
+      if (lane == 0) {
+        const uint32_t base = smem_u32(smem);
+        constexpr uint32_t id_ds = ch_idesc(128, true, true);
+        for (int it = 0; it < count; ++it) {
+          const int stg = it % STG;
+          if (!ch_wait(&br.rdy_b[stg], (it / STG) & 1, dead)) break;
+          if (!ch_wait(&br.ds_free, (it & 1) ^ 1, dead)) break;
+          bool ok = true;
+          for (int qt = 0; qt < kQ / kWRows; ++qt) {
+            const int buf = qt & 1;
+            if (!ch_wait(&br.w_full[buf], qt >> 1, dead)) {
+              ok = false;
+              break;
+            }
+            tc_after();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int head = head_of(wk.pair, h);
-        const float bias = a.dt_bias ? a.dt_bias[head] : 0.0f;
+            for (int part = 0; part < 3; ++part)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 4 * lane + i;
-          d[h][i] = t < valid
-                        ? softplus(__bfloat162float(a.dt[(size_t)(row + t) * a.dt_stride + head]) + bias)
-                        : 0.0f;
+              for (int k = 0; k < kWRows / 16; ++k)
+                // fewer than 128 state columns: the rows behind them repeat the first (panel stride 0)
+                mma_ss(tmem + kTmS,
+                       sw_desc(base + Sm::kB + stg * Sm::kTile + (kWRows * qt + 16 * k) * 128, N == 128 ? kPanel : 0),
+                       sw_desc(base + Sm::kW + (6 * buf + 2 * part) * kWPanel + k * 2048, kWPanel), id_ds,
+                       qt + part + k > 0);
+            ch_commit(&br.w_free[buf]);
+          }
+          if (!ok) break;
+          ch_commit(&br.b_free[stg]);
+          ch_commit(&br.ds_done);
         }
+        ch_commit(&br.mma_done);
+        mbar_wait(&br.mma_done, 0, 2000000000LL);
       }
-      if (!ch_wait_w(&br.sc_free[ph], ((it >> 1) & 1) ^ 1, dead)) break;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        Steps& st = steps[2 * ph + h];
-        const float A2 = a.A[head_of(wk.pair, h)] * log2e;
-        float e[4], suf[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = d[h][i] * A2;
-        const float own = (e[0] + e[1]) + (e[2] + e[3]);
-        // over the eight lanes of a block of 32 tokens
-        float pre = own, post = own;
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          const float u = __shfl_up_sync(0xffffffffu, pre, o), v = __shfl_down_sync(0xffffffffu, post, o);
-          if ((lane & 7) >= o) pre += u;
-          if ((lane & 7) + o < 8) post += v;
-        }
-        float ex = __shfl_up_sync(0xffffffffu, pre, 1), sx = __shfl_down_sync(0xffffffffu, post, 1);
-        if ((lane & 7) == 0) ex = 0.0f;
-        if ((lane & 7) == 7) sx = 0.0f;
-        const float b0 = __shfl_sync(0xffffffffu, pre, 7), b1 = __shfl_sync(0xffffffffu, pre, 15),
-                    b2 = __shfl_sync(0xffffffffu, pre, 23), b3 = __shfl_sync(0xffffffffu, pre, 31);
-        const int blk = lane >> 3;
-        const float after = blk == 0 ? b1 + b2 + b3 : blk == 1 ? b2 + b3 : blk == 2 ? b3 : 0.0f;
-        suf[3] = sx;
-        suf[2] = suf[3] + e[3];
-        suf[1] = suf[2] + e[2];
-        suf[0] = suf[1] + e[1];
-        float run = ex;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 4 * lane + i;
-          run += e[i];
-          st.lp[t] = run;
-          st.d[t] = d[h][i];
-          st.v[t] = d[h][i] * ex2(suf[i]);
-          st.w[t] = d[h][i] * ex2(suf[i] + after);
-        }
-        const float all = (b0 + b1) + (b2 + b3);
-        sum[h] += all;
-        if (lane == 0) {
-          st.blk[0] = b0;
-          st.blk[1] = b1;
-          st.blk[2] = b2;
-          st.blk[3] = b3;
-          st.all = ex2(all);
-        }
-      }
-      ch_arrive_w(&br.sc_full[ph]);
-      if (!ch_wait_w(&br.raw_b, ph, dead)) break;
+    } else {
+      // ------------------------------------------- rows behind an end
+      float sum0 = 0.0f, sum1 = 0.0f;  // pass 1: exponent of the whole part
+      const Steps* src = a.steps + 2 * ((size_t)first[0] * first[5] + first[6]);
       const uint4 zero = make_uint4(0, 0, 0, 0);
-      if (valid < kQ) {
-        for (int i = lane; i < (kQ - valid) * 8; i += 32)
+      for (int it = 0; it < count; ++it) {
+        const uint32_t sph = (it / STG) & 1;
+        const int valid = wk.valid(), stg = it % STG;
+        if (!WHOLE) {
+          sum0 += src[2 * it].sum;
+          sum1 += src[2 * it + 1].sum;
+        }
+        if (!ch_wait_w(&br.raw_b[stg], sph, dead)) break;
+        if (valid < kQ) {
+          for (int i = lane; i < (kQ - valid) * 8; i += 32)
 #pragma unroll
-          for (int p = 0; p < N / 64; ++p)
-            *reinterpret_cast<uint4*>(smem + Sm::kB + p * kPanel + valid * 128 + i * 16) = zero;
-        to_async();
-      }
-      ch_arrive_w(&br.rdy_b);
-      if (!ch_wait_w(&br.raw_x, ph, dead)) break;
-      if (valid < kQ) {
-        for (int i = lane; i < (kQ - valid) * 8; i += 32)
+            for (int p = 0; p < N / 64; ++p)
+              *reinterpret_cast<uint4*>(smem + Sm::kB + stg * Sm::kTile + p * kPanel + valid * 128 + i * 16) = zero;
+          to_async();
+        }
+        ch_arrive_w(&br.rdy_b[stg]);
+        if (!ch_wait_w(&br.raw_x[stg], sph, dead)) break;
+        if (valid < kQ) {
+          for (int i = lane; i < (kQ - valid) * 8; i += 32)
 #pragma unroll
-          for (int p = 0; p < 2; ++p)
-            *reinterpret_cast<uint4*>(smem + Sm::kX + p * kPanel + valid * 128 + i * 16) = zero;
-        to_async();
+            for (int p = 0; p < 2; ++p)
+              *reinterpret_cast<uint4*>(smem + Sm::kX + (2 * stg + p) * kPanel + valid * 128 + i * 16) = zero;
+          to_async();
+        }
+        ch_arrive_w(&br.rdy_x[stg]);
+        if (it + 1 < count) wk.next(a.pk);
       }
-      ch_arrive_w(&br.rdy_x);
-      if (it + 1 < count) wk.next(a.pk);
+      if (!WHOLE && count > 0 && lane < 2) a.decay[2 * cta + lane] = ex2(lane ? sum1 : sum0);
     }
-    if (!WHOLE && count > 0 && lane < 2) a.decay[2 * cta + lane] = ex2(lane ? sum[1] : sum[0]);
   }
   tc_before();
   __syncthreads();
-  if (warp == 17)
+  if (warp == 25)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Pass 0: one warp computes the steps of one head of a pair in one chunk; a
+// lane holds four tokens, eight lanes a block of 32.
+constexpr int kStepThreads = 256;
+
+__global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a) {
+  const int lane = threadIdx.x & 31, chunk = blockIdx.x;
+  const int ph = blockIdx.y * (kStepThreads / 32) + (threadIdx.x >> 5);  // pair and head
+  int seq = 0, nth = 0, total = 0;
+  if (!find_tile(a.pk, chunk, kQ, 0, seq, nth, total) || ph >= 2 * a.pairs) return;
+  int seq_, nth_;
+  find_tile(a.pk, -1, kQ, 0, seq_, nth_, total);
+  Walk wk;
+  wk.at(a.pk, ph >> 1, seq, nth);
+  const int head = Heads(a, ph >> 1).h[ph & 1], valid = wk.valid(), row = wk.row0();
+  const float bias = a.dt_bias ? a.dt_bias[head] : 0.0f, A2 = a.A[head] * 1.4426950408889634f;
+  float d[4], e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 4 * lane + i;
+    d[i] = t < valid ? softplus(__bfloat162float(a.dt[(size_t)(row + t) * a.dt_stride + head]) + bias) : 0.0f;
+    e[i] = d[i] * A2;
+  }
+  const float own = (e[0] + e[1]) + (e[2] + e[3]);
+  float pre = own, post = own;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const float u = __shfl_up_sync(0xffffffffu, pre, o), v = __shfl_down_sync(0xffffffffu, post, o);
+    if ((lane & 7) >= o) pre += u;
+    if ((lane & 7) + o < 8) post += v;
+  }
+  float run = __shfl_up_sync(0xffffffffu, pre, 1), suf = __shfl_down_sync(0xffffffffu, post, 1);
+  if ((lane & 7) == 0) run = 0.0f;
+  if ((lane & 7) == 7) suf = 0.0f;
+  const float b0 = __shfl_sync(0xffffffffu, pre, 7), b1 = __shfl_sync(0xffffffffu, pre, 15),
+              b2 = __shfl_sync(0xffffffffu, pre, 23), b3 = __shfl_sync(0xffffffffu, pre, 31);
+  const int blk = lane >> 3;
+  const float after = blk == 0 ? b1 + b2 + b3 : blk == 1 ? b2 + b3 : blk == 2 ? b3 : 0.0f;
+  float lp[4], v[4], w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    run += e[i];
+    lp[i] = run;
+  }
+#pragma unroll
+  for (int i = 3; i >= 0; --i) {
+    v[i] = d[i] * ex2(suf);
+    w[i] = d[i] * ex2(suf + after);
+    suf += e[i];
+  }
+  Steps& st = a.steps[2 * ((size_t)(ph >> 1) * total + chunk) + (ph & 1)];
+  *reinterpret_cast<float4*>(&st.lp[4 * lane]) = make_float4(lp[0], lp[1], lp[2], lp[3]);
+  *reinterpret_cast<float4*>(&st.d[4 * lane]) = make_float4(d[0], d[1], d[2], d[3]);
+  *reinterpret_cast<float4*>(&st.v[4 * lane]) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(&st.w[4 * lane]) = make_float4(w[0], w[1], w[2], w[3]);
+  if (lane == 0) {
+    const float all = (b0 + b1) + (b2 + b3);
+    *reinterpret_cast<float4*>(st.blk) = make_float4(b0, b1, b2, b3);
+    st.all = ex2(all);
+    st.sum = all;
+    st.D = a.D ? a.D[head] : 0.0f;
+  }
 }
 
 // Pass 2: along each head pair's pieces, in order, state after piece c =
@@ -834,31 +958,39 @@ __global__ void __launch_bounds__(kChThreads, 1)
 constexpr int kJoinThreads = 256;
 
 __global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(ChunkArgs a, int ctas) {
-  __shared__ int s_total;
-  if (threadIdx.x < 32) {
-    int seq, nth, total = 0;
-    find_tile(a.pk, -1, kQ, 0, seq, nth, total);
-    if (threadIdx.x == 0) s_total = total;
-  }
+  __shared__ int list[kMaxCtas], count[kJoinThreads / 32];
+  const int pair = blockIdx.y, tid = threadIdx.x, size = 2 * kP * a.n;
+  // this pair's pieces, in order
+  const int m = tid < ctas ? a.meta[tid] : 0;
+  const bool mine = (m & 3) && (m >> 2) == pair;
+  const unsigned votes = __ballot_sync(0xffffffffu, mine);
+  if ((tid & 31) == 0) count[tid >> 5] = __popc(votes);
   __syncthreads();
-  const int total = s_total, size = 2 * kP * a.n, pair = blockIdx.y;
-  const int e = blockIdx.x * kJoinThreads + threadIdx.x;
-  if (total > 0 && e < size) {
-    const long long all = (long long)total * a.pairs, lo = (long long)pair * total, hi = lo + total;
+  int at = 0, total = 0;
+  for (int i = 0; i < kJoinThreads / 32; ++i) {
+    if (i < (tid >> 5)) at += count[i];
+    total += count[i];
+  }
+  if (mine) list[at + __popc(votes & ((1u << (tid & 31)) - 1))] = tid * 4 + (m & 3);
+  __syncthreads();
+  const int e = (blockIdx.x * kJoinThreads + tid) * 4;
+  if (e < size) {
     const int h = e / (kP * a.n);
-    int c = (int)(lo * ctas / all);
-    while (c > 0 && cut(all, c, ctas) > lo) --c;
-    float carry = 0.0f;
-    // pieces that end inside this pair's steps
-    for (; c < ctas; ++c) {
-      const long long f1 = cut(all, c + 1, ctas);
-      if (f1 <= lo) continue;
-      if (f1 > hi || cut(all, c, ctas) >= hi) break;
-      const int m = a.meta[c];
-      if (m == 0) continue;
-      float* p = a.local + (size_t)c * size + e;
-      carry = m == 2 ? fmaf(a.decay[2 * c + h], carry, *p) : *p;
-      *p = carry;
+    float4 carry = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int i = 0; i < total; ++i) {
+      const int c = list[i] >> 2;
+      float4* p = reinterpret_cast<float4*>(a.local + (size_t)c * size + e);
+      float4 v = *p;
+      if ((list[i] & 3) == 2) {
+        const float d = a.decay[2 * c + h];
+        v.x = fmaf(d, carry.x, v.x);
+        v.y = fmaf(d, carry.y, v.y);
+        v.z = fmaf(d, carry.z, v.z);
+        v.w = fmaf(d, carry.w, v.w);
+      }
+      carry = v;
+      *p = v;
     }
   }
   if (a.state && a.pk.seqs) {
@@ -918,6 +1050,14 @@ bool chunk_sizes(int type, int tokens, int head_dim, int d_state) {
   return type == kTypeBF16 && head_dim == kP && (d_state == 64 || d_state == 128) && tokens > 32;
 }
 
+// The register shares need every register that the block is launched with: a
+// build that gave the kernel fewer must not run, its warps would wait for ever.
+bool chunk_kernel_ok(const void* fn, int smem) {
+  cudaFuncAttributes at;
+  return cudaFuncGetAttributes(&at, fn) == cudaSuccess && at.numRegs >= kRegs &&
+         cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
+}
+
 template <int N>
 int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   ChunkArgs a{};
@@ -936,7 +1076,9 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   a.pairs = a.ppg * s.groups;
   a.n = N;
   const size_t part = (size_t)kMaxCtas * 2 * kP * N;
-  a.local = static_cast<float*>(s.scratch);
+  const long long chunks = (long long)s.pk.tokens / kQ + s.pk.seqs;  // at most
+  a.steps = static_cast<Steps*>(s.scratch);
+  a.local = reinterpret_cast<float*>(a.steps + 2 * chunks * a.pairs);
   a.init = a.local + part;
   a.decay = a.init + part;
   a.meta = reinterpret_cast<int*>(a.decay + 2 * kMaxCtas);
@@ -946,25 +1088,26 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   if (int e = ch_map(&cm, s.C, s.pk.tokens, s.groups * N, s.c_stride)) return e;
   auto pass1 = scan_chunk_kernel<N, false>;
   auto pass3 = scan_chunk_kernel<N, true>;
-  constexpr int smem = ChunkSmem<N>::kBytes;
-  if (cudaFuncSetAttribute(pass1, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-      cudaFuncSetAttribute(pass3, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return kErrLaunch;
-  const long long most = ((long long)s.pk.tokens / kQ + s.pk.seqs) * a.pairs;  // steps, at most
+  constexpr int smem1 = ChunkSmem<N, false>::kBytes, smem3 = ChunkSmem<N, true>::kBytes;
+  if (!chunk_kernel_ok((const void*)pass1, smem1) || !chunk_kernel_ok((const void*)pass3, smem3)) return kErrLaunch;
+  const long long most = chunks * a.pairs;
   int ctas = device_sm_count();
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (most < ctas) ctas = (int)most;
-  pass1<<<ctas, kChThreads, smem, stream>>>(xm, bm, cm, a);
-  scan_join_kernel<<<dim3((2 * kP * N + kJoinThreads - 1) / kJoinThreads, a.pairs), kJoinThreads, 0, stream>>>(a, ctas);
-  pass3<<<ctas, kChThreads, smem, stream>>>(xm, bm, cm, a);
+  scan_steps_kernel<<<dim3((unsigned)chunks, (2 * a.pairs + kStepThreads / 32 - 1) / (kStepThreads / 32)), kStepThreads, 0,
+                      stream>>>(a);
+  pass1<<<ctas, kChThreads, smem1, stream>>>(xm, bm, cm, a);
+  scan_join_kernel<<<dim3((2 * kP * N / 4 + kJoinThreads - 1) / kJoinThreads, a.pairs), kJoinThreads, 0, stream>>>(a, ctas);
+  pass3<<<ctas, kChThreads, smem3, stream>>>(xm, bm, cm, a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace
 
-size_t ssm_prompt_scratch_bytes(int type, int tokens, int, int, int head_dim, int, int d_state) {
+size_t ssm_prompt_scratch_bytes(int type, int tokens, int seqs, int heads, int head_dim, int groups, int d_state) {
   if (!chunk_sizes(type, tokens, head_dim, d_state)) return 0;
-  return (size_t)kMaxCtas * (4 * kP * d_state * 4 + 16);
+  const size_t pairs = (size_t)(heads / groups + 1) / 2 * groups;
+  return ((size_t)tokens / kQ + seqs) * pairs * 2 * sizeof(Steps) + (size_t)kMaxCtas * (4 * kP * d_state * 4 + 16);
 }
 
 int launch_ssm_prompt(const ScanArgs& a, cudaStream_t stream) {

