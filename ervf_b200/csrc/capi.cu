@@ -1171,7 +1171,7 @@ int ervf_conv1d_prompt(const void* x, long long x_stride, const float* w, const 
     return kErrAlign;
   if (seqs == 0) return kOk;
   ConvArgs a{{cu_seqlens, slots, has_state, seqs, tokens, n_slots}, x, out, w, bias, state, x_stride, out_stride,
-             type, channels, width, silu};
+             type, channels, width, silu, 0};
   return launch_conv1d_prompt(a, S(stream));
 }
 

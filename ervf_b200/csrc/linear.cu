@@ -7,17 +7,30 @@
 // orientations: the MMA's 128 rows are tokens and its columns features, or
 // (few tokens) its rows are features and its columns tokens.
 //
-// Persistent and warp specialised, one CTA per SM; a k-block is 64 columns
-// (128 bytes of a row, the swizzle's width):
+// Warp specialised, one CTA per SM; a k-block is 64 columns (128 bytes of a
+// row, the swizzle's width):
 //   warp 0      producer: TMA of both operands' tiles into a ring of stages
 //   warp 1      one lane issues the tcgen05.mma of each stage into one of two
 //               accumulator buffers in tensor memory
 //   warps 2..5  epilogue: tcgen05.ld of a finished buffer, bias, activation,
 //               residual, store -- while the next tile's MMAs run
+// Three forms of it:
+//   few tokens (rows = features): bound by reading W from HBM.  Each of a
+//     k-block's four MMAs has an accumulator of its own, added in the epilogue:
+//     the tensor core's sums lose a little with every step (rel. 3e-6 over 4096
+//     columns in one chain).
+//   few tiles: the k-blocks of a tile are dealt to a cluster of CTAs, whose
+//     sums meet in shared memory and are added in rank order.
+//   many tokens: a pair of CTAs computes a 256 x 256 tile (cta_group::2); each
+//     holds its 128 rows of x and half of W's.  Bound by the tensor cores and
+//     by what L2 delivers: 64 bytes a clock and SM at full rate, where a single
+//     CTA's 128 x 256 tile takes 96.
 // Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
 // dead, and every role drains before tensor memory is freed.
 #include <cuda.h>  // CUtensorMap and the encode function's types (driver entry point)
 #include <cuda_bf16.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -31,14 +44,16 @@ constexpr int kLinM = 128, kLinKB = 64;
 constexpr int kLinThreads = 6 * 32;
 constexpr int kLinATile = kLinM * kLinKB * 2;
 
-template <int BN>
+template <int BN, int CH>
 struct LinShape {
   static constexpr int kBTile = BN * kLinKB * 2;
   static constexpr int kStage = kLinATile + kBTile;  // both multiples of 1024 bytes (swizzle period)
   static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
   static constexpr int kSmem = 1024 + 1024 + kStages * kStage;  // barriers, alignment slack, ring
-  static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
-  static_assert(BN % 16 == 0 && BN <= 256 && (kTmemCols & (kTmemCols - 1)) == 0, "tile");
+  static constexpr int kTmemCols = 2 * CH * BN;  // buffer d, chain c at columns (d CH + c) BN
+  static_assert(BN % 16 == 0 && BN <= 256 && kTmemCols >= 32 && kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0,
+                "tile");
+  static_assert(BN * kLinM * 4 <= kStages * kStage, "a split's sums fit the ring");
 };
 
 struct LinTile {
@@ -48,7 +63,7 @@ struct LinTile {
   long long resid_stride, out_stride;
   int rows, cols, tokens;
   int act;
-  int nkb, mtiles, ntiles;
+  int nkb, mtiles, ntiles, splits;
 };
 
 __device__ __forceinline__ uint64_t lin_desc(uint32_t saddr) {
@@ -148,10 +163,41 @@ __device__ __forceinline__ void lin_row(const LinTile& a, size_t t, int r, const
     }
 }
 
-template <int BN, bool SWAP, typename T>
+// 16 columns c.. of a tile from row lane `m`: tokens (SWAP) or features.
+template <bool SWAP, typename T>
+__device__ __forceinline__ void lin_store(const LinTile& a, int m, int n, const float (&f)[16]) {
+  if constexpr (SWAP) {
+    if (m < a.rows) {
+      const float b = a.bias ? a.bias[m] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n + i < a.tokens) {
+          float o = lin_act(f[i] + b, a.act);
+          if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)(n + i) * a.resid_stride + m);
+          lin_put(static_cast<T*>(a.out) + (size_t)(n + i) * a.out_stride + m, o);
+        }
+    }
+  } else {
+    if (m < a.tokens && n < a.rows) lin_row<T, 16>(a, m, n, f);
+  }
+}
+
+__device__ __forceinline__ float lin_remote(const float* p, int rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// CH accumulator chains a buffer; SPLIT: a cluster shares one tile's k-blocks.
+template <int BN, int CH, bool SWAP, bool SPLIT, typename T>
 __global__ void __launch_bounds__(kLinThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, LinTile a) {
-  using Sh = LinShape<BN>;
+  using Sh = LinShape<BN, CH>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
@@ -188,14 +234,18 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
-  const int units = a.mtiles * a.ntiles;
+  // SPLIT: one unit a cluster, this CTA's share of its k-blocks
+  const int rank = SPLIT ? (int)(blockIdx.x % a.splits) : 0;
+  const int units = a.mtiles * a.ntiles, u0 = SPLIT ? blockIdx.x / a.splits : blockIdx.x;
+  const int step = SPLIT ? units : (int)gridDim.x;
+  const int kb0 = SPLIT ? a.nkb * rank / a.splits : 0, kb1 = SPLIT ? a.nkb * (rank + 1) / a.splits : a.nkb;
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t gk = 0;
-      for (int u = blockIdx.x; u < units && !*dead; u += gridDim.x) {
+      for (int u = u0; u < units && !*dead; u += step) {
         const int mt = u % a.mtiles, nt = u / a.mtiles;
-        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
+        for (int kb = kb0; kb < kb1; ++kb, ++gk) {
           const int s = (int)(gk % Sh::kStages);
           if (!lin_wait(&empty[s], ((gk / Sh::kStages) & 1) ^ 1, dead)) break;
           mbar_arrive_expect_tx(&full[s], Sh::kStage);
@@ -212,12 +262,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     if (lane == 0) {
       uint32_t gk = 0;
       int nu = 0;
-      for (int u = blockIdx.x; u < units && !*dead; u += gridDim.x, ++nu) {
+      for (int u = u0; u < units && !*dead; u += step, ++nu) {
         const int d = nu & 1;
         if (!lin_wait(&dempty[d], ((nu >> 1) & 1) ^ 1, dead)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool ok = true;
-        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
+        for (int kb = kb0; kb < kb1; ++kb, ++gk) {
           const int s = (int)(gk % Sh::kStages);
           if (!lin_wait(&full[s], (gk / Sh::kStages) & 1, dead)) {
             ok = false;
@@ -227,11 +277,11 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           const uint32_t st = smem_u32(ring + s * Sh::kStage);
 #pragma unroll
           for (int j = 0; j < kLinKB / 16; ++j) {
-            const uint32_t acc = (kb | j) ? 1u : 0u;
+            const uint32_t acc = kb > kb0 || j >= CH ? 1u : 0u;
             asm volatile(
                 "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                ::"r"(tmem + (uint32_t)(d * BN)), "l"(lin_desc(st + 32 * j)),
+                ::"r"(tmem + (uint32_t)((d * CH + j % CH) * BN)), "l"(lin_desc(st + 32 * j)),
                   "l"(lin_desc(st + kLinATile + 32 * j)), "r"(idesc), "r"(acc) : "memory");
           }
           lin_commit(&empty[s]);
@@ -245,36 +295,34 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
   } else {
     const int q = warp & 3;  // tensor-memory lanes 32 q ..
+    // 16 columns of buffer d, its chains added in order
+    auto sums = [&](int d, int c, float (&f)[16]) {
+#pragma unroll
+      for (int h = 0; h < CH; ++h) {
+        uint32_t v[16];
+        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)((d * CH + h) * BN + c), v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = h ? f[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+      }
+    };
     int nu = 0;
-    for (int u = blockIdx.x; u < units && !*dead; u += gridDim.x, ++nu) {
+    for (int u = u0; u < units && !*dead; u += step, ++nu) {
       const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
       const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
       if (!__all_sync(0xffffffffu, w_ok)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int m = mt * kLinM + 32 * q + lane;
 #pragma unroll 1
       for (int c = 0; c < BN; c += 16) {
-        uint32_t v[16];
-        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         float f[16];
+        sums(d, c, f);
+        if constexpr (SPLIT) {
+          // all MMAs are done: the ring holds the sums, [column][row]
+          float* part = reinterpret_cast<float*>(ring) + (size_t)c * kLinM + 32 * q + lane;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-        if constexpr (SWAP) {
-          if (m < a.rows) {
-            const float b = a.bias ? a.bias[m] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int t = nt * BN + c + i;
-              if (t < a.tokens) {
-                float o = lin_act(f[i] + b, a.act);
-                if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + m);
-                lin_put(static_cast<T*>(a.out) + (size_t)t * a.out_stride + m, o);
-              }
-            }
-          }
+          for (int i = 0; i < 16; ++i) part[i * kLinM] = f[i];
         } else {
-          if (m < a.tokens && nt * BN + c < a.rows) lin_row<T, 16>(a, m, nt * BN + c, f);
+          lin_store<SWAP, T>(a, mt * kLinM + 32 * q + lane, nt * BN + c, f);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -282,10 +330,204 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       if (lane == 0) mbar_arrive(&dempty[d]);  // the buffer is read
     }
   }
+  if constexpr (SPLIT) {
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2) {
+      // this rank's share of the tile: every splits'th column (of tokens) or 16 of them (of features)
+      const int q = warp & 3, mt = u0 % a.mtiles, nt = u0 / a.mtiles, m = mt * kLinM + 32 * q + lane;
+      const float* part = reinterpret_cast<const float*>(ring) + 32 * q + lane;
+      if constexpr (SWAP) {
+        const int cols = min(BN, a.tokens - nt * BN);
+        for (int c = rank; c < cols; c += a.splits) {
+          float f = 0.0f;
+          for (int r = 0; r < a.splits; ++r) f += lin_remote(part + (size_t)c * kLinM, r);
+          if (m < a.rows) {
+            const size_t t = (size_t)(nt * BN + c);
+            float o = lin_act(f + (a.bias ? a.bias[m] : 0.0f), a.act);
+            if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + t * a.resid_stride + m);
+            lin_put(static_cast<T*>(a.out) + t * a.out_stride + m, o);
+          }
+        }
+      } else {
+        for (int c = 16 * rank; c < BN; c += 16 * a.splits) {
+          float f[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = 0.0f;
+          for (int r = 0; r < a.splits; ++r) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] += lin_remote(part + (size_t)(c + i) * kLinM, r);
+          }
+          lin_store<SWAP, T>(a, m, nt * BN + c, f);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // the others have read this CTA's sums
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kTmemCols) : "memory");
+}
+
+// ------------------------------------------------------- a pair of CTAs
+
+// One 256 x 256 tile by two CTAs: each loads its 128 rows of x and 128 of the
+// tile's 256 rows of W; the even one issues the MMAs of both.
+constexpr int kPairTile = 128 * kLinKB * 2;    // one operand's part in one CTA
+constexpr int kPairStage = 2 * kPairTile, kPairStages = 6;
+constexpr int kPairSmem = 2048 + kPairStages * kPairStage;
+
+__device__ __forceinline__ uint32_t lead_addr(const void* p) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(0));
+  return at;
+}
+// This GPU's own memory only, into this CTA; the bytes count at the even CTA's barrier.
+__device__ __forceinline__ void pair_tma(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+// Arrives at the same barrier of both CTAs.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, LinTile a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);  // counted at the even CTA
+  uint64_t* empty = full + kPairStages;                // one each
+  uint64_t* dfull = empty + kPairStages;               // one each
+  uint64_t* dempty = dfull + 2;                        // counted at the even CTA
+  uint64_t* mma_done = dempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 512);
+  volatile int* dead = reinterpret_cast<volatile int*>(smem + 516);
+  uint8_t* ring = smem + 1024;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1;
+  constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (32u << 17) | (16u << 24);  // N 256, M 256
+
+  if (tid == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&dfull[i], 1);
+      mbar_init(&dempty[i], 8);
+    }
+    mbar_init(mma_done, 1);
+    *dead = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // the other CTA's barriers are there
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const int units = a.mtiles * a.ntiles, u0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t gk = 0;
+      for (int u = u0; u < units && !*dead; u += step) {
+        const int mt = u % a.mtiles, nt = u / a.mtiles;
+        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
+          const int s = (int)(gk % kPairStages);
+          if (!lin_wait(&empty[s], ((gk / kPairStages) & 1) ^ 1, dead)) break;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);
+          const uint32_t bar = lead_addr(&full[s]);
+          uint8_t* st = ring + s * kPairStage;
+          pair_tma(st, &x_map, kb * kLinKB, (2 * mt + rank) * 128, bar);
+          pair_tma(st + kPairTile, &w_map, kb * kLinKB, (2 * nt + rank) * 128, bar);
+        }
+      }
+      // leave no tensor copy in flight: each stage's release follows its arrival
+      for (uint32_t k = gk > (uint32_t)kPairStages ? gk - kPairStages : 0; k < gk; ++k)
+        lin_wait(&empty[k % kPairStages], (k / kPairStages) & 1, dead);
+      if (*dead) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      uint32_t gk = 0;
+      int nu = 0;
+      for (int u = u0; u < units && !*dead; u += step, ++nu) {
+        const int d = nu & 1;
+        if (!lin_wait(&dempty[d], ((nu >> 1) & 1) ^ 1, dead)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        bool ok = true;
+        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
+          const int s = (int)(gk % kPairStages);
+          if (!lin_wait(&full[s], (gk / kPairStages) & 1, dead)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t st = smem_u32(ring + s * kPairStage);
+#pragma unroll
+          for (int j = 0; j < kLinKB / 16; ++j) {
+            asm volatile(
+                "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
+                ::"r"(tmem + (uint32_t)(d * 256)), "l"(lin_desc(st + 32 * j)),
+                  "l"(lin_desc(st + kPairTile + 32 * j)), "r"(idesc), "r"((uint32_t)(kb | j)) : "memory");
+          }
+          pair_commit(&empty[s]);
+        }
+        if (!ok) break;
+        pair_commit(&dfull[d]);
+      }
+      // every MMA is complete before tensor memory is freed
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                   ::"r"(smem_u32(mma_done)) : "memory");
+      mbar_wait(mma_done, 0, 2000000000LL);
+    }
+  } else {
+    const int q = warp & 3;  // tensor-memory lanes 32 q ..
+    int nu = 0;
+    for (int u = u0; u < units && !*dead; u += step, ++nu) {
+      const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
+      const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
+      if (!__all_sync(0xffffffffu, w_ok)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int m = (2 * mt + rank) * 128 + 32 * q + lane;
+#pragma unroll 1
+      for (int c = 0; c < 256; c += 16) {
+        uint32_t v[16];
+        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * 256 + c), v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        float f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+        lin_store<false, T>(a, m, nt * 256 + c, f);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)  // the buffer is read
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_addr(&dempty[d])) : "memory");
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  __syncwarp();
+  cluster_sync();  // nothing of the other CTA reads or signals here any more
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ------------------------------------------------------------------- host
@@ -322,10 +564,10 @@ int lin_map(CUtensorMap* map, const uint16_t* p, int rows, int cols, long long s
              : kErrArg;
 }
 
-template <int BN, bool SWAP, typename T>
-int linear_run(const LinearArgs& l, cudaStream_t stream) {
-  using Sh = LinShape<BN>;
-  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0};
+template <int BN, int CH, bool SWAP, bool SPLIT, typename T>
+int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
+  using Sh = LinShape<BN, CH>;
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits};
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   const int ma = SWAP ? l.rows : l.tokens, nb = SWAP ? l.tokens : l.rows;
   a.mtiles = (ma + kLinM - 1) / kLinM;
@@ -333,21 +575,100 @@ int linear_run(const LinearArgs& l, cudaStream_t stream) {
   CUtensorMap wm, xm;
   if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, SWAP ? kLinM : BN)) return e;
   if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, SWAP ? BN : kLinM)) return e;
-  auto fn = linear_kernel<BN, SWAP, T>;
+  auto fn = linear_kernel<BN, CH, SWAP, SPLIT, T>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
     return kErrLaunch;
   const long long units = (long long)a.mtiles * a.ntiles;
   if (units > 0x7fffffffLL) return kErrShape;
   const int sms = device_sm_count();
-  fn<<<(unsigned)(units < sms ? units : sms), kLinThreads, Sh::kSmem, stream>>>(SWAP ? wm : xm, SWAP ? xm : wm, a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(SPLIT ? units * splits : units < sms ? units : sms));
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = Sh::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = SPLIT ? splits : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, fn, SWAP ? wm : xm, SWAP ? xm : wm, a) == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <typename T>
+int linear_pair(const LinearArgs& l, cudaStream_t stream) {
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, 1};
+  a.nkb = (l.cols + kLinKB - 1) / kLinKB;
+  a.mtiles = (l.tokens + 255) / 256;
+  a.ntiles = (l.rows + 255) / 256;
+  const long long units = (long long)a.mtiles * a.ntiles;
+  if (units > 0x3fffffffLL) return kErrShape;
+  CUtensorMap wm, xm;
+  if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, 128)) return e;
+  if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, 128)) return e;
+  auto fn = linear_pair_kernel<T>;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess)
+    return kErrLaunch;
+  const int pairs = device_sm_count() / 2;
+  fn<<<2 * (unsigned)(units < pairs ? units : pairs), kLinThreads, kPairSmem, stream>>>(xm, wm, a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+// Clusters of s CTAs (one an SM) that the current device runs at a time: SMs
+// lie in groups that a cluster does not cross, so 21 clusters of 7 do not fit
+// 148 SMs at once, though 147 CTAs do.
+int linear_clusters(int s) {
+  static std::atomic<int> known[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const bool keep = dev < 64;
+  if (keep && known[dev][s].load()) return known[dev][s].load() - 1;
+  auto fn = linear_kernel<32, 4, true, true, float>;
+  constexpr int smem = LinShape<32, 4>::kSmem;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(s);
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = s;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (keep) known[dev][s].store(n + 1);
+  return n;
+}
+
+// CTAs that share a tile's k-blocks: the most (8 is a portable cluster) whose
+// clusters all run at once, each CTA with two k-blocks or more.
+int linear_splits(long long units, int cols) {
+  const int nkb = (cols + kLinKB - 1) / kLinKB;
+  for (int s = nkb / 2 < 8 ? nkb / 2 : 8; s > 1; --s)
+    if (units * s <= device_sm_count() && units <= linear_clusters(s)) return s;
+  return 1;
+}
+
+template <int BN, int CH, bool SWAP, typename T>
+int linear_single(const LinearArgs& l, cudaStream_t stream) {
+  const long long ma = SWAP ? l.rows : l.tokens, nb = SWAP ? l.tokens : l.rows;
+  const int splits = linear_splits(((ma + kLinM - 1) / kLinM) * ((nb + BN - 1) / BN), l.cols);
+  return splits > 1 ? linear_run<BN, CH, SWAP, true, T>(l, splits, stream)
+                    : linear_run<BN, CH, SWAP, false, T>(l, 1, stream);
 }
 
 template <typename T>
 int linear_pick(const LinearArgs& l, cudaStream_t stream) {
-  if (l.tokens <= 32) return linear_run<32, true, T>(l, stream);
-  if (l.tokens <= 128) return linear_run<64, true, T>(l, stream);
-  return linear_run<256, false, T>(l, stream);
+  if (l.tokens <= 32) return linear_single<32, 4, true, T>(l, stream);
+  if (l.tokens <= 128) return linear_single<64, 4, true, T>(l, stream);
+  const long long pairs = (((long long)l.tokens + 255) / 256) * (((long long)l.rows + 255) / 256);
+  if (2 * pairs >= device_sm_count()) return linear_pair<T>(l, stream);
+  return linear_single<256, 1, false, T>(l, stream);
 }
 
 }  // namespace

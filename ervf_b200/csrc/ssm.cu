@@ -28,164 +28,175 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V consecutive elements as f32.  V is 1 or fills 16 bytes.
+// V consecutive elements as they lie in memory, V = 1 or V elements one load's
+// width (8 or 16 bytes) apart.
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = to_f32(*p);
-  } else {
-    static_assert(V * sizeof(T) == 16, "16-byte vectors");
-    uint4 q = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_f32(e[i]);
+struct Raw {
+  static constexpr int kBytes = V * (int)sizeof(T), kWords = kBytes < 4 ? 1 : kBytes / 4;
+  static_assert(V == 1 || kBytes == 8 || kBytes == 16, "one load");
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (kBytes == 8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      w[0] = q.x; w[1] = q.y;
+    } else {
+      const uint4 q = *reinterpret_cast<const uint4*>(p);
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    }
   }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    *p = from_f32<T>(v[0]);
-  } else {
-    uint4 q;
-    T* e = reinterpret_cast<T*>(&q);
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = q;
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-}
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  }
+  __device__ __forceinline__ void set(const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(v[i]);
+    } else if constexpr (V == 1) {
+      w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(v[i + 1]), "f"(v[i]));
+    }
+  }
+};
 
 // ------------------------------------------------------------- convolution
 
 // y_t = act(bias + sum_j w[j] x[t - width + 1 + j]) for each channel.  A
 // thread owns V channels of one tile of a sequence, keeps the window in
 // registers and four tokens' loads in flight ahead of the four it works on.
-// Bound by HBM: every input is read once (and `width - 1` rows again per
-// tile, from L2), every output written once.  The thread of a sequence's
-// first tile is the only one that touches the carried state: it reads the old
-// inputs, and writes the sequence's last `width - 1` ones.
-constexpr int kConvTile = 32, kConvThreads = 128, kConvAhead = 4;
-
-// V elements as they lie in memory.
-template <typename T, int V>
-struct Raw {
-  static constexpr int kWords = V == 1 ? 1 : 4;
-  uint32_t w[kWords];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (V == 1) {
-      if constexpr (sizeof(T) == 2) w[0] = *reinterpret_cast<const uint16_t*>(p);
-      else w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
-    }
-  }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-    else return __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
-  }
-};
+// Bound by HBM and, near it, by the two special-function operations of each
+// silu: every input is read once (and `width - 1` rows again per tile, from
+// L2), every output written once.  The thread of a sequence's first tile is
+// the only one that touches the carried state: it reads the old inputs, and
+// writes the sequence's last `width - 1` ones.
+constexpr int kConvThreads = 128, kConvAhead = 4;
 
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(kConvThreads, 4) conv_prompt_kernel(ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, 6) conv_prompt_kernel(ConvArgs a) {
   const int ch = (blockIdx.y * kConvThreads + threadIdx.x) * V;
   int seq, nth, total;
-  if (!find_tile(a.pk, blockIdx.x, kConvTile, 1, seq, nth, total)) return;
+  if (!find_tile(a.pk, blockIdx.x, a.tile, 1, seq, nth, total)) return;
   if (ch >= a.channels) return;
   int begin, len;
   seq_range(a.pk, seq, begin, len);
-  const T* x = static_cast<const T*>(a.x) + (size_t)begin * a.x_stride + ch;
-  T* out = static_cast<T*>(a.out) + (size_t)begin * a.out_stride + ch;
+  const int t0 = nth * a.tile, t1 = min(t0 + a.tile, len);
+  const T* x = static_cast<const T*>(a.x) + (size_t)(begin + t0) * a.x_stride + ch;
+  T* out = static_cast<T*>(a.out) + (size_t)(begin + t0) * a.out_stride + ch;
+  int left = t1 - t0;
+  Raw<T, V> next[kConvAhead];
+  auto ahead = [&](const T* p, int n) {
+#pragma unroll
+    for (int u = 0; u < kConvAhead; ++u)
+      if (u < n) next[u].load(p + (size_t)u * a.x_stride);
+  };
+  ahead(x, left);
+  Raw<T, V> old[W - 1];  // the W - 1 inputs before the tile, oldest first
   const int slot = nth == 0 && a.state ? seq_slot(a.pk, seq) : -1;
   T* state = slot < 0 ? nullptr : static_cast<T*>(a.state) + (size_t)slot * (W - 1) * a.channels + ch;
-  const int t0 = nth * kConvTile, t1 = min(t0 + kConvTile, len);
-  Raw<T, V> next[kConvAhead];
-#pragma unroll
-  for (int u = 0; u < kConvAhead; ++u)
-    if (t0 + u < t1) next[u].load(x + (size_t)(t0 + u) * a.x_stride);
-  float win[W - 1][V];  // the W - 1 inputs before the next one, oldest first
+  const bool carried = state && a.pk.has && a.pk.has[seq];
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    const int t = t0 - (W - 1) + j;
-    if (t >= 0) {
-      load_vec<T, V>(x + (size_t)t * a.x_stride, win[j]);
-    } else if (state && a.pk.has && a.pk.has[seq]) {
-      load_vec<T, V>(state + (size_t)j * a.channels, win[j]);
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) win[j][v] = 0.0f;
-    }
+    const int back = W - 1 - j;
+    if (t0 >= back) old[j].load(x - (size_t)back * a.x_stride);
+    else if (carried) old[j].load(state + (size_t)j * a.channels);
+    else old[j].clear();
   }
-  float w[V][W], bias[V];
+  if (state) {
+    // last W - 1 inputs of [carried state, sequence]
+    Raw<T, V> last[W - 1];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      const int t = len - (W - 1) + j;
+      if (t >= 0) {
+        last[j].load(x + (size_t)t * a.x_stride);
+      } else {
+        last[j].clear();
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k)
+          if (t + (W - 1) == k) last[j] = old[k];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) last[j].store(state + (size_t)j * a.channels);
+  }
+  float w[V][W], bias[V], win[W - 1][V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     bias[v] = a.bias ? a.bias[ch + v] : 0.0f;
 #pragma unroll
     for (int j = 0; j < W; ++j) w[v][j] = a.w[(size_t)(ch + v) * W + j];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) win[j][v] = old[j].get(v);
   }
-  if (state) {
-    // last W - 1 inputs of [carried state, sequence]
-    float last[W - 1][V];
+  auto token = [&](const Raw<T, V>& c, T* o) {
+    float y[V];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) {
-      const int t = len - (W - 1) + j;
-      if (t >= 0) {
-        load_vec<T, V>(x + (size_t)t * a.x_stride, last[j]);
-      } else {
-        // win holds the carried inputs at positions -(W - 1) .. -1
+    for (int v = 0; v < V; ++v) {
+      const float e = c.get(v);
+      float sum = bias[v];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float e = 0.0f;
+      for (int j = 0; j < W - 1; ++j) sum = fmaf(w[v][j], win[j][v], sum);
+      sum = fmaf(w[v][W - 1], e, sum);
+      y[v] = a.silu ? silu(sum) : sum;
 #pragma unroll
-          for (int k = 0; k < W - 1; ++k)
-            if (t + (W - 1) == k) e = win[k][v];
-          last[j][v] = e;
-        }
-      }
+      for (int j = 0; j + 1 < W - 1; ++j) win[j][v] = win[j + 1][v];
+      win[W - 2][v] = e;
     }
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_vec<T, V>(state + (size_t)j * a.channels, last[j]);
-  }
-  for (int t = t0; t < t1; t += kConvAhead) {
+    Raw<T, V> q;
+    q.set(y);
+    q.store(o);
+  };
+  while (left > 0) {
     Raw<T, V> cur[kConvAhead];
 #pragma unroll
     for (int u = 0; u < kConvAhead; ++u) cur[u] = next[u];
+    x += (size_t)kConvAhead * a.x_stride;
+    ahead(x, left - kConvAhead);
+    if (left >= kConvAhead) {
 #pragma unroll
-    for (int u = 0; u < kConvAhead; ++u)
-      if (t + kConvAhead + u < t1) next[u].load(x + (size_t)(t + kConvAhead + u) * a.x_stride);
+      for (int u = 0; u < kConvAhead; ++u) token(cur[u], out + (size_t)u * a.out_stride);
+    } else {
 #pragma unroll
-    for (int u = 0; u < kConvAhead; ++u) {
-      if (t + u >= t1) break;
-      float y[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float c = cur[u].get(v);
-        float sum = bias[v];
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) sum = fmaf(w[v][j], win[j][v], sum);
-        sum = fmaf(w[v][W - 1], c, sum);
-        y[v] = a.silu ? silu(sum) : sum;
-#pragma unroll
-        for (int j = 0; j + 1 < W - 1; ++j) win[j][v] = win[j + 1][v];
-        win[W - 2][v] = c;
-      }
-      store_vec<T, V>(out + (size_t)(t + u) * a.out_stride, y);
+      for (int u = 0; u < kConvAhead - 1; ++u)
+        if (u < left) token(cur[u], out + (size_t)u * a.out_stride);
     }
+    out += (size_t)kConvAhead * a.out_stride;
+    left -= kConvAhead;
   }
 }
 
 template <typename T, int V>
-int launch_conv(const ConvArgs& a, cudaStream_t stream) {
-  const dim3 grid((unsigned)(a.pk.tokens / kConvTile + a.pk.seqs),
-                  (a.channels + kConvThreads * V - 1) / (kConvThreads * V));
+int launch_conv(ConvArgs a, cudaStream_t stream) {
+  // 64 tokens a tile spread the weights' loads further; 32 where that would
+  // leave the SMs short of CTAs
+  const long long cols = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
+  a.tile = (a.pk.tokens / 64 + a.pk.seqs) * cols >= 12LL * device_sm_count() ? 64 : 32;
+  const dim3 grid((unsigned)(a.pk.tokens / a.tile + a.pk.seqs), (unsigned)cols);
   if (a.width == 2) conv_prompt_kernel<T, 2, V><<<grid, kConvThreads, 0, stream>>>(a);
   else if (a.width == 3) conv_prompt_kernel<T, 3, V><<<grid, kConvThreads, 0, stream>>>(a);
   else conv_prompt_kernel<T, 4, V><<<grid, kConvThreads, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
-// 16-byte vectors of V elements fit a row-strided array.
-bool vec_ok(const void* p, long long stride, size_t elem) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((unsigned long long)stride * elem & 15) == 0;
+// Vectors of `bytes` fit a row-strided array.
+bool vec_ok(const void* p, long long stride, size_t elem, unsigned bytes = 16) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && ((unsigned long long)stride * elem & (bytes - 1)) == 0;
 }
 
 // --------------------------------------------------- scan, token by token
@@ -295,141 +306,178 @@ int launch_scan_seq(const ScanArgs& a, cudaStream_t stream) {
 //  0. the first rows of the first head's state start on their way;
 //  1. every CTA convolves its heads' x channels and, for itself, the group's
 //     B and C channels (2 d_state of them: recomputing is cheaper than
-//     sending them on);
-//  2. after a cluster barrier (every CTA has read the carried B / C inputs)
-//     CTA 0 shifts those inputs by one token;
-//  3. the states' update and y: L lanes share a row of d_state, a warp works
-//     on 8 rows a lane at a time (128 bytes in flight each);
-//  4. the CTAs' sums of squares meet in shared memory of each (added in rank
-//     order), then the norm and the output.
+//     sending them on), and arrives at the cluster's barrier;
+//  2. the states' update and y: L lanes share a row of d_state, a lane works
+//     on kRows rows while the next ones are on their way;
+//  3. behind the barrier (every CTA has read the carried B / C inputs) CTA 0
+//     stores those inputs moved on by one token, and every CTA its sum of
+//     squares into each other's shared memory;
+//  4. behind a second one the sums are added in rank order: norm and output.
 constexpr int kTokThreads = 256;
 
+// What a channel's convolution reads: oldest input first, the new one last.
 template <typename T>
-__device__ __forceinline__ float conv_one(const TokenArgs& a, const T* xin, const T* cs, int ch) {
-  float s = a.conv_bias ? a.conv_bias[ch] : 0.0f;
-  const float* w = a.conv_w + (size_t)ch * a.width;
-  for (int j = 0; j < a.width - 1; ++j)
-    s = fmaf(w[j], cs ? to_f32(cs[(size_t)j * (a.heads * a.head_dim + 2 * a.groups * a.d_state) + ch]) : 0.0f, s);
-  return silu(fmaf(w[a.width - 1], to_f32(xin[ch]), s));
-}
-
-template <typename T>
-__device__ __forceinline__ void conv_shift(const TokenArgs& a, const T* xin, T* cs, int ch) {
-  const size_t pitch = (size_t)a.heads * a.head_dim + 2 * (size_t)a.groups * a.d_state;
-  for (int j = 0; j + 1 < a.width - 1; ++j) cs[j * pitch + ch] = cs[(j + 1) * pitch + ch];
-  cs[(size_t)(a.width - 2) * pitch + ch] = xin[ch];
-}
+struct Taps {
+  T v[kMaxConvWidth];
+  float w[kMaxConvWidth], bias;
+  // all loads before any use; fewer taps than the most leave the first ones zero
+  __device__ __forceinline__ void load(const TokenArgs& a, const T* xin, const T* cs, size_t channels, int ch) {
+    const int gap = kMaxConvWidth - a.width;
+#pragma unroll
+    for (int j = 0; j < kMaxConvWidth; ++j) {
+      w[j] = j >= gap ? a.conv_w[(size_t)ch * a.width + j - gap] : 0.0f;
+      if (j == kMaxConvWidth - 1) v[j] = xin[ch];
+      else v[j] = j >= gap && cs ? cs[(size_t)(j - gap) * channels + ch] : from_f32<T>(0.0f);
+    }
+    bias = a.conv_bias ? a.conv_bias[ch] : 0.0f;
+  }
+  __device__ __forceinline__ float value() const {
+    float s = bias;
+#pragma unroll
+    for (int j = 0; j < kMaxConvWidth; ++j) s = fmaf(w[j], to_f32(v[j]), s);
+    return silu(s);
+  }
+};
 
 // L lanes of four columns each share a row, NV times over.
 template <typename T, int L, int NV>
-__global__ void __launch_bounds__(kTokThreads, 3) ssm_token_kernel(TokenArgs a) {
-  constexpr int kRows = 8 / NV;                              // rows of a lane at a time
+__global__ void __launch_bounds__(kTokThreads, 4) ssm_token_kernel(TokenArgs a) {
+  constexpr int kRows = 4 / NV;                                   // rows of a lane at a time
   constexpr int kStep = kTokThreads / L, kBatch = kRows * kStep;  // rows of the CTA
+  constexpr int kWarps = kTokThreads / 32, kOld = kMaxConvWidth - 1;
   extern __shared__ __align__(16) float sm[];
   cg::cluster_group cl = cg::this_cluster();
   const int c = (int)cl.num_blocks(), r = (int)cl.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int unit = blockIdx.x / c, seq = unit / a.groups, grp = unit - seq * a.groups;
   const int hpg = a.heads / a.groups, P = a.head_dim, N = a.d_state;
-  const int mine = (hpg - r + c - 1) / c;  // heads of this CTA: r, r + c, ...
-  float* sBC = sm;                         // B then C of the group
-  float* sy = sBC + 2 * N;                 // [mine][P]: x, then the gated output
-  float* red = sy + ((hpg + c - 1) / c) * P;  // per-warp sums, then this CTA's sum
+  const int mine = (hpg - r + c - 1) / c, most = (hpg + c - 1) / c;  // heads of this CTA: r, r + c, ...
+  float* sBC = sm;                  // B then C of the group
+  float* sy = sBC + 2 * N;          // [mine][P]: x, then the gated output
+  float* sz = sy + most * P;        // [mine][P]: silu(z)
+  float* sh = sz + most * P;        // [mine]: d, exp(d A), D
+  float* red = sh + 3 * most;       // per-warp sums, then the ranks'
+  T* old = reinterpret_cast<T*>(red + kWarps + 16);  // rank 0: the B / C inputs to carry on
   const int s0 = a.slots ? a.slots[seq] : seq;
   const int slot = s0 >= 0 && s0 < a.n_slots ? s0 : -1;
-  const T* xin = static_cast<const T*>(a.xbc) + (size_t)seq * a.xbc_stride;
   const size_t channels = (size_t)a.heads * P + 2 * (size_t)a.groups * N;
+  const T* xin = static_cast<const T*>(a.xbc) + (size_t)seq * a.xbc_stride;
+  T* cs = slot < 0 ? nullptr : static_cast<T*>(a.conv_state) + (size_t)slot * (a.width - 1) * channels;
   const int sub = tid / L, n0 = (tid % L) * 4;
-  float4 v[kRows][NV];
-  // rows p0 + sub, p0 + sub + kStep, ... of a head's state
-  auto load = [&](const float* st, int p0) {
+  const int batches = (P + kBatch - 1) / kBatch, rounds = mine * batches;
+  float4 next[kRows][NV];
+  auto state_of = [&](int k) {
+    return a.state + ((size_t)slot * a.heads + grp * hpg + r + k * c) * P * N;
+  };
+  // rows p0 + sub, p0 + sub + kStep, ... of the head's state of round i
+  auto load = [&](int i) {
+    const int k = i / batches, p0 = (i - k * batches) * kBatch;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int p = p0 + i * kStep + sub, n = n0 + k * 4 * L;
-        v[i][k] = st && p < P && n < N ? *reinterpret_cast<const float4*>(st + (size_t)p * N + n)
-                                       : make_float4(0, 0, 0, 0);
+      for (int j = 0; j < NV; ++j) {
+        const int p = p0 + i * kStep + sub, n = n0 + j * 4 * L;
+        next[i][j] = slot >= 0 && p < P && n < N ? *reinterpret_cast<const float4*>(state_of(k) + (size_t)p * N + n)
+                                                 : make_float4(0, 0, 0, 0);
       }
   };
-  auto state_of = [&](int k) {
-    return slot < 0 ? nullptr : a.state + ((size_t)slot * a.heads + grp * hpg + r + k * c) * P * N;
-  };
-  load(state_of(0), 0);
-  T* cs = slot < 0 ? nullptr : static_cast<T*>(a.conv_state) + (size_t)slot * (a.width - 1) * channels;
-  for (int i = tid; i < 2 * N; i += kTokThreads) {
-    const int ch = a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N);
-    sBC[i] = conv_one(a, xin, cs, ch);
+  load(0);
+  if (tid >= kTokThreads - 32)
+    for (int k = lane; k < mine; k += 32) {
+      const int head = grp * hpg + r + k * c;
+      const float d = softplus(to_f32(static_cast<const T*>(a.dt)[(size_t)seq * a.dt_stride + head]) +
+                               (a.dt_bias ? a.dt_bias[head] : 0.0f));
+      sh[3 * k] = d;
+      sh[3 * k + 1] = expf(d * a.A[head]);
+      sh[3 * k + 2] = a.D ? a.D[head] : 0.0f;
+    }
+  for (int i = tid; i < 2 * N + mine * P; i += kTokThreads) {
+    Taps<T> t;
+    if (i < 2 * N) {
+      const int ch = a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N);
+      t.load(a, xin, cs, channels, ch);
+      sBC[i] = t.value();
+      if (r == 0)
+#pragma unroll
+        for (int j = 0; j < kOld; ++j) old[j * 2 * N + i] = t.v[j + 1];
+    } else {
+      const int e = i - 2 * N, k = e / P, ch = (grp * hpg + r + k * c) * P + e - k * P;
+      t.load(a, xin, cs, channels, ch);
+      const float z = a.z ? to_f32(static_cast<const T*>(a.z)[(size_t)seq * a.z_stride + ch]) : 0.0f;
+      sy[e] = t.value();
+      sz[e] = a.z ? silu(z) : 1.0f;
+      if (cs)
+#pragma unroll
+        for (int j = 0; j < kOld; ++j)
+          if (j >= kMaxConvWidth - a.width) cs[(size_t)(j - kMaxConvWidth + a.width) * channels + ch] = t.v[j + 1];
+    }
   }
-  for (int i = tid; i < mine * P; i += kTokThreads) {
-    const int k = i / P, ch = (grp * hpg + r + k * c) * P + i - k * P;
-    sy[i] = conv_one(a, xin, cs, ch);
-    if (cs) conv_shift(a, xin, cs, ch);
-  }
-  cl.sync();  // B / C inputs read by every CTA; also this CTA's __syncthreads
-  if (r == 0 && cs)
-    for (int i = tid; i < 2 * N; i += kTokThreads)
-      conv_shift(a, xin, cs, a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N));
+  cl.barrier_arrive();
+  __syncthreads();
   float ss = 0.0f;
-  for (int k = 0; k < mine; ++k) {
-    const int head = grp * hpg + r + k * c;
-    const float d = softplus(to_f32(static_cast<const T*>(a.dt)[(size_t)seq * a.dt_stride + head]) +
-                             (a.dt_bias ? a.dt_bias[head] : 0.0f));
-    const float da = expf(d * a.A[head]), D = a.D ? a.D[head] : 0.0f;
-    float* st = state_of(k);
-    for (int p0 = 0; p0 < P; p0 += kBatch) {
-      if (k + p0 > 0) load(st, p0);
+  for (int i = 0; i < rounds; ++i) {
+    const int k = i / batches, p0 = (i - k * batches) * kBatch;
+    float4 v[kRows][NV];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const int p = p0 + i * kStep + sub;
-        const float x = p < P ? sy[k * P + p] : 0.0f, dx = d * x;
-        float y = 0.0f;
+    for (int q = 0; q < kRows; ++q)
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int n = n0 + j * 4 * L;
-          if (n < N) {
-            const float4 b = *reinterpret_cast<const float4*>(sBC + n);
-            const float4 cc = *reinterpret_cast<const float4*>(sBC + N + n);
-            float4 q = v[i][j];
-            q.x = fmaf(dx, b.x, da * q.x);
-            q.y = fmaf(dx, b.y, da * q.y);
-            q.z = fmaf(dx, b.z, da * q.z);
-            q.w = fmaf(dx, b.w, da * q.w);
-            if (st && p < P) *reinterpret_cast<float4*>(st + (size_t)p * N + n) = q;
-            y += (q.x * cc.x + q.y * cc.y) + (q.z * cc.z + q.w * cc.w);
-          }
+      for (int j = 0; j < NV; ++j) v[q][j] = next[q][j];
+    if (i + 1 < rounds) load(i + 1);
+    const float d = sh[3 * k], da = sh[3 * k + 1], D = sh[3 * k + 2];
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      const int p = p0 + q * kStep + sub;
+      const float x = p < P ? sy[k * P + p] : 0.0f, dx = d * x;
+      float y = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int n = n0 + j * 4 * L;
+        if (n < N) {
+          const float4 b = *reinterpret_cast<const float4*>(sBC + n);
+          const float4 cc = *reinterpret_cast<const float4*>(sBC + N + n);
+          float4 e = v[q][j];
+          e.x = fmaf(dx, b.x, da * e.x);
+          e.y = fmaf(dx, b.y, da * e.y);
+          e.z = fmaf(dx, b.z, da * e.z);
+          e.w = fmaf(dx, b.w, da * e.w);
+          if (slot >= 0 && p < P) *reinterpret_cast<float4*>(state_of(k) + (size_t)p * N + n) = e;
+          y += (e.x * cc.x + e.y * cc.y) + (e.z * cc.z + e.w * cc.w);
         }
+      }
 #pragma unroll
-        for (int o = L / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-        if (p < P) {
-          y = fmaf(D, x, y);
-          if (a.z) y *= silu(to_f32(static_cast<const T*>(a.z)[(size_t)seq * a.z_stride + head * P + p]));
-          if (n0 == 0) {
-            ss = fmaf(y, y, ss);
-            sy[k * P + p] = y;  // its x was read by this row's lanes, together
-          }
-        }
-        __syncwarp();
+      for (int o = L / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (n0 == 0 && p < P) {
+        y = fmaf(D, x, y) * sz[k * P + p];
+        ss = fmaf(y, y, ss);
+        sy[k * P + p] = y;  // its x was read by this row's lanes, together
       }
     }
+    __syncwarp();
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (lane == 0) red[warp] = ss;
+  __syncthreads();
+  cl.barrier_wait();
+  if (r == 0 && cs)
+    for (int i = tid; i < 2 * N; i += kTokThreads) {
+      const int ch = a.heads * P + (i < N ? grp * N + i : (a.groups + grp) * N + i - N);
+#pragma unroll
+      for (int j = 0; j < kOld; ++j)
+        if (j >= kMaxConvWidth - a.width)
+          cs[(size_t)(j - kMaxConvWidth + a.width) * channels + ch] = old[j * 2 * N + i];
+    }
   float scale = 1.0f;
   if (a.norm_w) {
-    if (lane == 0) red[warp] = ss;
-    __syncthreads();
-    if (tid == 0) {
+    if (tid < c) {
       float t = 0.0f;
-      for (int i = 0; i < kTokThreads / 32; ++i) t += red[i];
-      red[kTokThreads / 32] = t;
+      for (int i = 0; i < kWarps; ++i) t += red[i];
+      *cl.map_shared_rank(red + kWarps + r, tid) = t;
     }
     cl.sync();
     float t = 0.0f;
-    for (int i = 0; i < c; ++i) t += *cl.map_shared_rank(red + kTokThreads / 32, i);
+    for (int i = 0; i < c; ++i) t += red[kWarps + i];
     scale = rsqrtf(t / (float)(hpg * P) + a.eps);
-  } else {
-    __syncthreads();
   }
   T* out = static_cast<T*>(a.out) + (size_t)seq * a.out_stride;
   for (int i = tid; i < mine * P; i += kTokThreads) {
@@ -437,7 +485,6 @@ __global__ void __launch_bounds__(kTokThreads, 3) ssm_token_kernel(TokenArgs a) 
     const float v = sy[i] * scale;
     out[ch] = from_f32<T>(a.norm_w ? v * a.norm_w[ch] : v);
   }
-  if (a.norm_w) cl.sync();  // the others' sums are read before a CTA leaves
 }
 
 template <typename T>
@@ -456,7 +503,7 @@ const void* token_kernel(int d_state) {
 constexpr int kNormThreads = 128;
 
 template <typename T, int NV>
-__global__ void __launch_bounds__(kNormThreads) gated_norm_warp_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, NV <= 2 ? 8 : 4) gated_norm_warp_kernel(NormArgs a) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, grp = blockIdx.y;
   const size_t off = (size_t)grp * a.group_size;
@@ -503,7 +550,8 @@ __global__ void __launch_bounds__(kNormThreads) gated_norm_warp_kernel(NormArgs 
       if (i < a.group_size) {
 #pragma unroll
         for (int j = 0; j < V; ++j) g[k][j] *= scale * w[k][j];
-        store_vec<T, V>(out + (size_t)t * a.out_stride + i, g[k]);
+        ry[k].set(g[k]);
+        ry[k].store(out + (size_t)t * a.out_stride + i);
       }
     }
   }
@@ -547,7 +595,7 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
   if (a.group_size % V == 0 && nv <= 4 && a.groups <= 65535 && vec_ok(a.y, a.y_stride, sizeof(T)) &&
       vec_ok(a.z, a.z ? a.z_stride : 0, sizeof(T)) && vec_ok(a.out, a.out_stride, sizeof(T))) {
     const long long rows = ((long long)a.tokens + kNormThreads / 32 - 1) / (kNormThreads / 32);
-    const long long most = (8LL * device_sm_count() + a.groups - 1) / a.groups;  // 32 warps a SM, walking
+    const long long most = ((nv <= 2 ? 8LL : 4LL) * device_sm_count() + a.groups - 1) / a.groups;  // one wave, walking
     const dim3 grid((unsigned)(rows < most ? rows : most), a.groups);
     if (nv == 1) gated_norm_warp_kernel<T, 1><<<grid, kNormThreads, 0, stream>>>(a);
     else if (nv == 2) gated_norm_warp_kernel<T, 2><<<grid, kNormThreads, 0, stream>>>(a);
@@ -562,12 +610,11 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_conv1d_prompt(const ConvArgs& a, cudaStream_t stream) {
-  const size_t e = a.type == kTypeBF16 ? 2 : 4;
-  const int v = (int)(16 / e);
-  const bool vec = a.channels % v == 0 && vec_ok(a.x, a.x_stride, e) && vec_ok(a.out, a.out_stride, e) &&
-                   vec_ok(a.state, a.channels, e);
+  const unsigned e = a.type == kTypeBF16 ? 2 : 4;
+  const bool vec = a.channels % 4 == 0 && vec_ok(a.x, a.x_stride, e, 4 * e) && vec_ok(a.out, a.out_stride, e, 4 * e) &&
+                   vec_ok(a.state, a.channels, e, 4 * e);
   if (a.type == kTypeBF16)
-    return vec ? launch_conv<__nv_bfloat16, 8>(a, stream) : launch_conv<__nv_bfloat16, 1>(a, stream);
+    return vec ? launch_conv<__nv_bfloat16, 4>(a, stream) : launch_conv<__nv_bfloat16, 1>(a, stream);
   return vec ? launch_conv<float, 4>(a, stream) : launch_conv<float, 1>(a, stream);
 }
 
@@ -576,8 +623,16 @@ int launch_scan_tokens(const ScanArgs& a, cudaStream_t stream) {
 }
 
 int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
-  const int hpg = a.heads / a.groups, c = hpg < 8 ? hpg : 8;
-  const size_t smem = (2 * (size_t)a.d_state + (size_t)((hpg + c - 1) / c) * a.head_dim + kTokThreads / 32 + 1) * 4;
+  const int hpg = a.heads / a.groups;
+  // as many CTAs a group as its heads, but no more than three waves of them: a
+  // batch of 96 with eight groups takes 117 us with eight CTAs a group, 93 with
+  // four, 86 with two and 97 with one (each convolves B and C for itself); one
+  // sequence's latency is least with eight
+  int c = hpg < 8 ? hpg : 8;
+  while (c > 1 && (long long)a.seqs * a.groups * c > 12LL * device_sm_count()) c = (c + 1) / 2;
+  const size_t most = (hpg + c - 1) / c, elem = a.type == kTypeBF16 ? 2 : 4;
+  const size_t smem = (2 * (size_t)a.d_state + 2 * most * a.head_dim + 3 * most + kTokThreads / 32 + 16) * 4 +
+                      (kMaxConvWidth - 1) * 2 * a.d_state * elem;
   const void* fn = a.type == kTypeBF16 ? token_kernel<__nv_bfloat16>(a.d_state) : token_kernel<float>(a.d_state);
   if (smem > 48 * 1024) return kErrShape;
   cudaLaunchConfig_t cfg{};

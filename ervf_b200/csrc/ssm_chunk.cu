@@ -127,12 +127,6 @@ struct ChunkSmem {
 };
 static_assert(ChunkSmem<128, true>::kBytes <= 232448 && ChunkSmem<128, false>::kBytes <= 232448, "shared memory");
 
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
