@@ -12,8 +12,10 @@
 //   warp 0      producer: TMA of both operands' tiles into a ring of stages
 //   warp 1      one lane issues the tcgen05.mma of each stage into one of two
 //               accumulator buffers in tensor memory
-//   warps 2..5  epilogue: tcgen05.ld of a finished buffer, bias, activation,
-//               residual, store -- while the next tile's MMAs run
+//   warps 2..9  epilogue: tcgen05.ld of a finished buffer (two warps a quarter
+//               of its lanes, half the columns each), bias, activation,
+//               residual, store -- while the next tile's MMAs run; bias and
+//               residual are loaded one step ahead
 // Three forms of it:
 //   few tokens (rows = features): bound by reading W from HBM.  Each of a
 //     k-block's four MMAs has an accumulator of its own, added in the epilogue:
@@ -41,7 +43,7 @@ namespace ervf {
 namespace {
 
 constexpr int kLinM = 128, kLinKB = 64;
-constexpr int kLinThreads = 6 * 32;
+constexpr int kLinEpi = 8, kLinThreads = (2 + kLinEpi) * 32;
 constexpr int kLinATile = kLinM * kLinKB * 2;
 
 template <int BN, int CH>
@@ -127,59 +129,68 @@ __device__ __forceinline__ void lin_put(T* p, float v) {
   else *p = v;
 }
 
-// N consecutive features r.. of token t.
-template <typename T, int N>
-__device__ __forceinline__ void lin_row(const LinTile& a, size_t t, int r, const float (&acc)[N]) {
-  T* o = static_cast<T*>(a.out) + t * a.out_stride + r;
-  const T* q = a.resid ? static_cast<const T*>(a.resid) + t * a.resid_stride + r : nullptr;
-  constexpr int V = 16 / sizeof(T);
-  const bool whole = r + N <= a.rows && ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(q)) & 15) == 0 &&
-                     (!a.bias || (reinterpret_cast<uintptr_t>(a.bias + r) & 15) == 0);
-  if (whole) {
+// What 16 consecutive features r.. of token t need beside their sums.
+template <typename T>
+struct LinRow {
+  static constexpr int V = 16 / sizeof(T), kVecs = 16 / V;
+  bool whole;  // 16 features, all aligned
+  float4 bias[4];
+  uint4 resid[kVecs];
+  __device__ __forceinline__ void load(const LinTile& a, int t, int r) {
+    whole = t < a.tokens && r + 16 <= a.rows;
+    if (!whole) return;
+    const T* o = static_cast<const T*>(a.out) + (size_t)t * a.out_stride + r;
+    const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + r : nullptr;
+    whole = ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(q) |
+              (a.bias ? reinterpret_cast<uintptr_t>(a.bias + r) : 0)) & 15) == 0;
+    if (!whole) return;
 #pragma unroll
-    for (int i = 0; i < N; i += V) {
-      uint4 rq = q ? *reinterpret_cast<const uint4*>(q + i) : make_uint4(0, 0, 0, 0), oq;
-      const T* re = reinterpret_cast<const T*>(&rq);
-      T* oe = reinterpret_cast<T*>(&oq);
+    for (int i = 0; i < 4; ++i)
+      bias[i] = a.bias ? *reinterpret_cast<const float4*>(a.bias + r + 4 * i) : make_float4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const float4 b = a.bias ? *reinterpret_cast<const float4*>(a.bias + r + i + j) : make_float4(0, 0, 0, 0);
-        const float bb[4] = {b.x, b.y, b.z, b.w};
+    for (int i = 0; i < kVecs; ++i)
+      resid[i] = q ? *reinterpret_cast<const uint4*>(q + i * V) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void store(const LinTile& a, int t, int r, const float (&acc)[16]) const {
+    if (t >= a.tokens || r >= a.rows) return;
+    T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + r;
+    if (whole) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float v = lin_act(acc[i + j + k] + bb[k], a.act);
-          lin_put(oe + j + k, q ? v + lin_get(re + j + k) : v);
+      for (int i = 0; i < kVecs; ++i) {
+        const T* re = reinterpret_cast<const T*>(&resid[i]);
+        uint4 oq;
+        T* oe = reinterpret_cast<T*>(&oq);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int k = i * V + j;
+          const float4 b = bias[k / 4];
+          const float bb[4] = {b.x, b.y, b.z, b.w};
+          const float v = lin_act(acc[k] + bb[k % 4], a.act);
+          lin_put(oe + j, a.resid ? v + lin_get(re + j) : v);
         }
+        *reinterpret_cast<uint4*>(o + i * V) = oq;
       }
-      *reinterpret_cast<uint4*>(o + i) = oq;
+      return;
     }
-    return;
-  }
+    const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + r : nullptr;
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+      if (r + i < a.rows) {
+        float v = acc[0];
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (r + i < a.rows) {
-      const float v = lin_act(acc[i] + (a.bias ? a.bias[r + i] : 0.0f), a.act);
-      lin_put(o + i, q ? v + lin_get(q + i) : v);
-    }
-}
+        for (int k = 1; k < 16; ++k) v = i == k ? acc[k] : v;
+        v = lin_act(v + (a.bias ? a.bias[r + i] : 0.0f), a.act);
+        lin_put(o + i, q ? v + lin_get(q + i) : v);
+      }
+  }
+};
 
-// 16 columns c.. of a tile from row lane `m`: tokens (SWAP) or features.
-template <bool SWAP, typename T>
-__device__ __forceinline__ void lin_store(const LinTile& a, int m, int n, const float (&f)[16]) {
-  if constexpr (SWAP) {
-    if (m < a.rows) {
-      const float b = a.bias ? a.bias[m] : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n + i < a.tokens) {
-          float o = lin_act(f[i] + b, a.act);
-          if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)(n + i) * a.resid_stride + m);
-          lin_put(static_cast<T*>(a.out) + (size_t)(n + i) * a.out_stride + m, o);
-        }
-    }
-  } else {
-    if (m < a.tokens && n < a.rows) lin_row<T, 16>(a, m, n, f);
-  }
+// One sum of feature m of token t.
+template <typename T>
+__device__ __forceinline__ void lin_one(const LinTile& a, int t, int m, float bias, float f) {
+  float o = lin_act(f + bias, a.act);
+  if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + m);
+  lin_put(static_cast<T*>(a.out) + (size_t)t * a.out_stride + m, o);
 }
 
 __device__ __forceinline__ float lin_remote(const float* p, int rank) {
@@ -219,7 +230,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&dfull[i], 1);
-      mbar_init(&dempty[i], 4);
+      mbar_init(&dempty[i], kLinEpi);
     }
     mbar_init(mma_done, 1);
     *dead = 0;
@@ -306,14 +317,25 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         for (int i = 0; i < 16; ++i) f[i] = h ? f[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
       }
     };
+    constexpr int kCols = BN >= 32 ? BN / 2 : BN;  // columns of a warp
+    const int c0 = (warp - 2) / 4 * kCols;
     int nu = 0;
     for (int u = u0; u < units && !*dead; u += step, ++nu) {
       const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
+      const int m = mt * kLinM + 32 * q + lane;
+      LinRow<T> pre;
+      float bias = 0.0f;
+      if constexpr (!SPLIT) {
+        if constexpr (SWAP) bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
+        else pre.load(a, m, nt * BN + c0);
+      }
       const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
       if (!__all_sync(0xffffffffu, w_ok)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 16) {
+      for (int c = c0; c < c0 + kCols; c += 16) {
+        LinRow<T> ahead;
+        if constexpr (!SPLIT && !SWAP) ahead.load(a, m, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
         float f[16];
         sums(d, c, f);
         if constexpr (SPLIT) {
@@ -321,9 +343,15 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           float* part = reinterpret_cast<float*>(ring) + (size_t)c * kLinM + 32 * q + lane;
 #pragma unroll
           for (int i = 0; i < 16; ++i) part[i * kLinM] = f[i];
+        } else if constexpr (SWAP) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (m < a.rows && nt * BN + c + i < a.tokens) lin_one<T>(a, nt * BN + c + i, m, bias, f[i]);
         } else {
-          lin_store<SWAP, T>(a, mt * kLinM + 32 * q + lane, nt * BN + c, f);
+          pre.store(a, m, nt * BN + c, f);
+          pre = ahead;
         }
+        __syncwarp();
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -334,31 +362,38 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     __syncwarp();
     cluster_sync();
     if (warp >= 2) {
-      // this rank's share of the tile: every splits'th column (of tokens) or 16 of them (of features)
+      // this rank's share of the tile, dealt to its warps: columns (of
+      // tokens), or 16 of them (of features)
       const int q = warp & 3, mt = u0 % a.mtiles, nt = u0 / a.mtiles, m = mt * kLinM + 32 * q + lane;
+      const int who = rank + a.splits * ((warp - 2) / 4), all = a.splits * (kLinEpi / 4);
       const float* part = reinterpret_cast<const float*>(ring) + 32 * q + lane;
       if constexpr (SWAP) {
         const int cols = min(BN, a.tokens - nt * BN);
-        for (int c = rank; c < cols; c += a.splits) {
-          float f = 0.0f;
-          for (int r = 0; r < a.splits; ++r) f += lin_remote(part + (size_t)c * kLinM, r);
-          if (m < a.rows) {
-            const size_t t = (size_t)(nt * BN + c);
-            float o = lin_act(f + (a.bias ? a.bias[m] : 0.0f), a.act);
-            if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + t * a.resid_stride + m);
-            lin_put(static_cast<T*>(a.out) + t * a.out_stride + m, o);
-          }
+        const float bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
+        for (int c = who; c < cols; c += all) {
+          float v[8], f = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) v[r] = r < a.splits ? lin_remote(part + (size_t)c * kLinM, r) : 0.0f;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) f += v[r];  // in rank order
+          if (m < a.rows) lin_one<T>(a, nt * BN + c, m, bias, f);
         }
       } else {
-        for (int c = 16 * rank; c < BN; c += 16 * a.splits) {
+        for (int c = 16 * who; c < BN; c += 16 * all) {
+          LinRow<T> pre;
+          pre.load(a, m, nt * BN + c);
           float f[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] = 0.0f;
+#pragma unroll 2
           for (int r = 0; r < a.splits; ++r) {
+            float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] += lin_remote(part + (size_t)(c + i) * kLinM, r);
+            for (int i = 0; i < 16; ++i) v[i] = lin_remote(part + (size_t)(c + i) * kLinM, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] += v[i];
           }
-          lin_store<SWAP, T>(a, m, nt * BN + c, f);
+          pre.store(a, m, nt * BN + c, f);
         }
       }
     }
@@ -373,11 +408,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
 // ------------------------------------------------------- a pair of CTAs
 
-// One 256 x 256 tile by two CTAs: each loads its 128 rows of x and 128 of the
-// tile's 256 rows of W; the even one issues the MMAs of both.
-constexpr int kPairTile = 128 * kLinKB * 2;    // one operand's part in one CTA
-constexpr int kPairStage = 2 * kPairTile, kPairStages = 6;
-constexpr int kPairSmem = 2048 + kPairStages * kPairStage;
+// One 256 x BN tile by two CTAs: each loads its 128 rows of x and half of the
+// tile's BN rows of W; the even one issues the MMAs of both.
+constexpr int kPairTile = 128 * kLinKB * 2;  // x's part in one CTA
+template <int BN>
+struct PairShape {
+  static constexpr int kStage = kPairTile + BN / 2 * kLinKB * 2, kStages = BN == 256 ? 6 : 8;
+  static constexpr int kSmem = 2048 + kStages * kStage;
+};
 
 __device__ __forceinline__ uint32_t lead_addr(const void* p) {
   uint32_t at;
@@ -397,9 +435,10 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
       ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
-template <typename T>
+template <int BN, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, LinTile a) {
+  constexpr int kPairStages = PairShape<BN>::kStages, kPairStage = PairShape<BN>::kStage;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);  // counted at the even CTA
@@ -411,7 +450,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
   volatile int* dead = reinterpret_cast<volatile int*>(smem + 516);
   uint8_t* ring = smem + 1024;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1;
-  constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (32u << 17) | (16u << 24);  // N 256, M 256
+  constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
+                             (16u << 24);  // M 256
 
   if (tid == 0) {
     for (int i = 0; i < kPairStages; ++i) {
@@ -420,7 +460,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&dfull[i], 1);
-      mbar_init(&dempty[i], 8);
+      mbar_init(&dempty[i], 2 * kLinEpi);
     }
     mbar_init(mma_done, 1);
     *dead = 0;
@@ -428,7 +468,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-                 ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+                 ::"r"(smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -450,7 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
           const uint32_t bar = lead_addr(&full[s]);
           uint8_t* st = ring + s * kPairStage;
           pair_tma(st, &x_map, kb * kLinKB, (2 * mt + rank) * 128, bar);
-          pair_tma(st + kPairTile, &w_map, kb * kLinKB, (2 * nt + rank) * 128, bar);
+          pair_tma(st + kPairTile, &w_map, kb * kLinKB, nt * BN + rank * (BN / 2), bar);
         }
       }
       // leave no tensor copy in flight: each stage's release follows its arrival
@@ -484,7 +524,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
             asm volatile(
                 "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                 " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
-                ::"r"(tmem + (uint32_t)(d * 256)), "l"(lin_desc(st + 32 * j)),
+                ::"r"(tmem + (uint32_t)(d * BN)), "l"(lin_desc(st + 32 * j)),
                   "l"(lin_desc(st + kPairTile + 32 * j)), "r"(idesc), "r"((uint32_t)(kb | j)) : "memory");
           }
           pair_commit(&empty[s]);
@@ -499,22 +539,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
     }
   } else {
     const int q = warp & 3;  // tensor-memory lanes 32 q ..
+    const int c0 = (warp - 2) / 4 * (BN / 2);
     int nu = 0;
     for (int u = u0; u < units && !*dead; u += step, ++nu) {
       const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
+      const int m = (2 * mt + rank) * 128 + 32 * q + lane;
+      LinRow<T> pre;
+      pre.load(a, m, nt * BN + c0);
       const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
       if (!__all_sync(0xffffffffu, w_ok)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int m = (2 * mt + rank) * 128 + 32 * q + lane;
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 16) {
+      for (int c = c0; c < c0 + BN / 2; c += 16) {
+        LinRow<T> ahead;
+        ahead.load(a, m, c + 16 < c0 + BN / 2 ? nt * BN + c + 16 : a.rows);
         uint32_t v[16];
-        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * 256 + c), v);
+        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-        lin_store<false, T>(a, m, nt * 256 + c, f);
+        pre.store(a, m, nt * BN + c, f);
+        pre = ahead;
+        __syncwarp();
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -527,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
   __syncwarp();
   cluster_sync();  // nothing of the other CTA reads or signals here any more
   if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
 }
 
 // ------------------------------------------------------------------- host
@@ -595,18 +642,19 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, fn, SWAP ? wm : xm, SWAP ? xm : wm, a) == cudaSuccess ? kOk : kErrLaunch;
 }
 
-template <typename T>
+template <int BN, typename T>
 int linear_pair(const LinearArgs& l, cudaStream_t stream) {
+  constexpr int kPairSmem = PairShape<BN>::kSmem;
   LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, 1};
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   a.mtiles = (l.tokens + 255) / 256;
-  a.ntiles = (l.rows + 255) / 256;
+  a.ntiles = (l.rows + BN - 1) / BN;
   const long long units = (long long)a.mtiles * a.ntiles;
   if (units > 0x3fffffffLL) return kErrShape;
   CUtensorMap wm, xm;
-  if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, 128)) return e;
+  if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, BN / 2)) return e;
   if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, 128)) return e;
-  auto fn = linear_pair_kernel<T>;
+  auto fn = linear_pair_kernel<BN, T>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess)
     return kErrLaunch;
   const int pairs = device_sm_count() / 2;
@@ -666,8 +714,9 @@ template <typename T>
 int linear_pick(const LinearArgs& l, cudaStream_t stream) {
   if (l.tokens <= 32) return linear_single<32, 4, true, T>(l, stream);
   if (l.tokens <= 128) return linear_single<64, 4, true, T>(l, stream);
-  const long long pairs = (((long long)l.tokens + 255) / 256) * (((long long)l.rows + 255) / 256);
-  if (2 * pairs >= device_sm_count()) return linear_pair<T>(l, stream);
+  const long long mt = ((long long)l.tokens + 255) / 256, sms = device_sm_count();
+  if (4 * mt * ((l.rows + 255LL) / 256) >= 3 * sms) return linear_pair<256, T>(l, stream);
+  if (4 * mt * ((l.rows + 127LL) / 128) >= sms) return linear_pair<128, T>(l, stream);
   return linear_single<256, 1, false, T>(l, stream);
 }
 

@@ -44,7 +44,7 @@ def k(cuda):
     (1, 8, 1), (7, 16, 3), (128, 64, 1), (129, 72, 33), (300, 1000, 17), (256, 4104, 2),
     (1000, 264, 128), (257, 520, 129), (513, 136, 300), (2688, 4096, 1), (2688, 1856, 8),
     (640, 328, 257), (1111, 88, 511), (20000, 64, 5), (96, 8192, 64),
-    (2500, 200, 2001), (5000, 72, 1030), (300, 1032, 9000)])
+    (2500, 200, 2001), (5000, 72, 1030), (300, 1032, 9000), (2700, 136, 3333)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_linear(k, cuda, rows, cols, tokens, dtype):
     W, x, b, r = make(rows, cols, tokens, dtype, True, True)
