@@ -9,7 +9,8 @@
 // One CTA per SM walks a list of (head pair, sequence, chunk) steps and carries
 // the two heads' state in registers; C B^T is shared by the pair.  The list
 // is cut into equal pieces, one per CTA, wherever the cuts fall:
-//   pass 0  softplus, running sums and weights of every (head, chunk)
+//   pass 0  softplus, running sums and weights of every (head, chunk); each
+//           CTA's piece
 //   pass 1  (WHOLE = false) a CTA whose piece ends inside a sequence computes
 //           the state that its own part of that sequence adds, and its decay;
 //   pass 2  joins these along each sequence, in order;
@@ -25,20 +26,22 @@
 //
 // Warps (a warpgroup's register share in brackets), and what bounds them at
 // 128 state columns (clocks per step of two heads, measured tcgen05 rates):
-//   0..7   P [80]: C B^T from tensor memory, weighted, back to tensor memory
-//          as an A operand; S C to exp(c_t) S C + D x in tensor memory
-//   8..15  states [96]: the f32 state, 64 registers a thread; split for S C
-//   16..23 W [56]: x scaled to the chunk's end and split into three, 32 tokens
-//          at a time, as the B operand of the state's new terms; then y, tensor
-//          memory -> bf16 -> rows, while the next x tile is on its way
-//   24     TMA of the B, C and x tiles and of the steps
-//   25     MMAs of y: C B^T 8 x 65, S C 16 x 69, P x 16 x 68
-//   26     MMAs of the state's new terms: 24 x 69; with 25's, 4370 clocks
+//   0..7   P and y [80]: C B^T from tensor memory, weighted, back to tensor
+//          memory as an A operand, both heads; their products with x take the
+//          columns of C B^T; then exp(c_t) S C + P x + D x -> bf16
+//   8..15  states [96]: the f32 state, 64 registers a thread, split for S C
+//   16..23 W [48]: x scaled to the chunk's end and split into three, 32 tokens
+//          at a time, as the B operand of the state's new terms
+//   24     TMA of the steps and of the B and C tiles
+//   25     MMAs C B^T 8 x 65 and P x 16 x 68; TMA of the x tiles
+//   26     MMAs of the state's new terms 24 x 69 and S C 16 x 69
 //   27     clears rows behind a sequence's end, so that a neighbour's NaN meets
 //          no zero weight
-// Both operands of a 128-column MMA in shared memory take its whole bandwidth
-// (128 bytes a clock); with W, the split state and the tiles a step moves 800 KB
-// there, 6250 clocks.
+// The MMAs take 4370 clocks.  Both operands of a 128-column MMA in shared
+// memory take its whole bandwidth (128 bytes a clock); with W, the split state
+// and the tiles a step moves 740 KB there, 5800 clocks.  The loops are kept short
+// (short waits, little unrolling): seven roles' code does not fit the
+// instruction cache otherwise.
 // In pass 1 warps 0..7 do W's work too.
 // Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
 // dead, and every role leaves; copies and MMAs are drained first.
@@ -54,11 +57,11 @@ namespace {
 
 constexpr int kQ = 128, kP = 64;          // tokens per chunk, head_dim
 constexpr int kPanel = kQ * 128;          // 128 rows of 64 bf16, 128-byte swizzle
-constexpr int kWRows = 32, kWPanel = kWRows * 128;  // tokens of a W buffer, one part of one head of it
+constexpr int kWRows = 32, kPieces = kQ / kWRows, kWPanel = kWRows * 128;  // tokens of a W buffer, one part of one head of it
 constexpr int kChWarps = 28, kChThreads = kChWarps * 32;
 // registers a thread at launch, and each warpgroup's after its split: the
 // shares must not exceed what the block was launched with
-constexpr int kRegs = 72, kRegP = 80, kRegS = 96, kRegW = 56, kRegMisc = 40;
+constexpr int kRegs = 72, kRegP = 80, kRegS = 96, kRegW = 48, kRegMisc = 56;
 static_assert(2 * kRegP + 2 * kRegS + 2 * kRegW + kRegMisc <= 7 * kRegs, "register shares");
 constexpr int kMaxCtas = 148;
 // tensor-memory columns
@@ -78,6 +81,13 @@ struct alignas(16) Steps {
 };
 static_assert(sizeof(Steps) % 16 == 0, "bulk copies");
 
+// A CTA's piece of the list: its first step (pair, sequence, chunk), the place
+// of that chunk among all sequences', the number of steps, and the piece before
+// (pieces may be empty).
+struct alignas(16) Plan {
+  int pair, seq, chunk, nth, count, before, total, pad;
+};
+
 struct ChunkArgs {
   Packing pk;
   const __nv_bfloat16* dt;
@@ -91,13 +101,15 @@ struct ChunkArgs {
   float* local;                // [ctas][2][kP][n]: pass 1's states, joined in place by pass 2
   float* init;                 // [ctas][2][kP][n]: carried states of sequences that are cut
   float* decay;                // [ctas][2]
+  Plan* plan;                  // [pass 1, pass 3][ctas]
   int* meta;                   // [ctas]: 0 no cut, else pair * 4 + (1 from a sequence's start, 2 continued)
 };
 
-// kStages tiles of B and x: pass 1 has the room of C, S and y.  Two teams scale
+// kStages tiles of B and x: pass 1 has the room of C and S.  Two teams scale
 // x, each into a W buffer of its own (a team may run a step ahead of the
 // other: buffers taken in turns would need more than a parity to tell their
-// rounds apart).
+// rounds apart).  Pieces of 16 tokens and two buffers a team were slower: the
+// issuing thread's waits cost more than the overlap gave.
 template <bool WHOLE>
 struct Depth {
   static constexpr int kStages = WHOLE ? 1 : 2, kWBufs = 2, kTeam = WHOLE ? 128 : 256;
@@ -107,7 +119,7 @@ struct Barriers {
   uint64_t raw_b[2], raw_c, raw_x[2];  // TMA bytes landed
   uint64_t rdy_b[2], rdy_x[2];         // and rows behind the end cleared
   uint64_t sc_full[2], sc_free[2];
-  uint64_t cb_full, cb_free, cs_done, p_full[2], px_done[2], y_free;
+  uint64_t cb_full, cs_done, p_full, px_done, y_free;
   uint64_t w_full[2], w_free[2], ds_done, ds_free, b_free[2], s_full, x_read[2], mma_done;
 };
 
@@ -120,7 +132,7 @@ struct ChunkSmem {
   static constexpr int kC = kW + Dp::kWBufs * 6 * kWPanel;
   static constexpr int kS = kC + (WHOLE ? kTile : 0);       // [hi, lo][head][N rows]
   static constexpr int kSPanel = N * 128;
-  static constexpr int kY = kS + (WHOLE ? 4 * kSPanel : 0); // 8 warps x 1 KB
+  static constexpr int kY = kS + (WHOLE ? 4 * kSPanel : 0);   // 8 warps x 1 KB
   static constexpr int kSteps = kY + (WHOLE ? 8 * 1024 : 0);  // [2 buffers][2 heads]
   static constexpr int kBar = kSteps + 4 * (int)sizeof(Steps);
   static constexpr int kBytes = 1024 + kBar + 512;
@@ -152,35 +164,26 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uin
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
       ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)acc) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, 1, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      ::"r"(d), "r"(a), "l"(db), "r"(idesc) : "memory");
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"((uint32_t)acc) : "memory");
 }
 __device__ __forceinline__ void ch_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tm_ld32(uint32_t t, uint32_t (&v)[32]) {
+// 16 columns each of two places.
+__device__ __forceinline__ void tm_ld16x2(uint32_t t, uint32_t t2, uint32_t (&v)[16], uint32_t (&w)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(t));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tm_st32(uint32_t t, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
-        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
-        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+        "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]),
+        "=r"(w[8]), "=r"(w[9]), "=r"(w[10]), "=r"(w[11]), "=r"(w[12]), "=r"(w[13]), "=r"(w[14]), "=r"(w[15])
+      : "r"(t), "r"(t2) : "memory");
 }
 __device__ __forceinline__ void tm_ld16(uint32_t t, uint32_t (&v)[16]) {
   asm volatile(
@@ -189,13 +192,6 @@ __device__ __forceinline__ void tm_ld16(uint32_t t, uint32_t (&v)[16]) {
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(t));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tm_st16(uint32_t t, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
 }
 __device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -218,25 +214,25 @@ __device__ __forceinline__ void ch_prefetch(const CUtensorMap* map, int x, int y
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 
-__device__ __noinline__ void ch_timeout(volatile int* dead) {
-  atomicExch(&g_device_error, kErrTimeout);
-  *dead = 1;
-}
-
-// Bounded wait of one thread: kChTries tries, each of which the hardware may
-// suspend for up to 20 us; gives up too when another role died.  Small on
-// purpose: with some forty waits in line, a clock to watch in each made the
-// kernel 97 KB long, and its warps waited for instructions.
-constexpr int kChTries = 100000;
-
+// Bounded wait of one thread: 100,000 tries, each of which the hardware may
+// suspend for up to 20 us; gives up too when another role died.  A wait that
+// runs out marks the CTA dead (2; its last act tells the host).  Short on
+// purpose: the kernel waits in some forty places, and its warps, each in a loop
+// of its own, wait for instructions as soon as those loops outgrow the cache.
 __device__ __forceinline__ bool ch_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-#pragma unroll 1
-  for (int i = 0; i < kChTries; ++i) {
-    if (mbar_try_wait_sleep(bar, parity, 20000)) return true;
-    if (*dead) return false;
-  }
-  ch_timeout(dead);
-  return false;
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n, d;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n mov.u32 n, 100000;\n"
+      "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n @p bra DONE;\n"
+      " ld.volatile.shared.u32 d, [%3];\n setp.ne.u32 q, d, 0;\n @q bra DONE;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra AGAIN;\n"
+      " st.volatile.shared.u32 [%3], 2;\n"
+      "DONE:\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(dead))), "r"(20000u)
+      : "memory");
+  return ok != 0;
 }
 // The same for a whole warp: one decision.
 __device__ __forceinline__ bool ch_wait_w(uint64_t* bar, uint32_t parity, volatile int* dead) {
@@ -279,7 +275,10 @@ struct Walk {
 // Heads of a pair; an odd group's last pair has its head twice.
 struct Heads {
   int grp, h[2];
-  __device__ Heads(const ChunkArgs& a, int pair) {
+  int of = -1;  // the pair they are of
+  __device__ void at(const ChunkArgs& a, int pair) {
+    if (pair == of) return;
+    of = pair;
     grp = pair / a.ppg;
     const int k = (pair - grp * a.ppg) * 2;
     h[0] = grp * a.hpg + k;
@@ -297,39 +296,40 @@ __device__ __forceinline__ void split2(float e, float o, uint32_t& hi, uint32_t&
 }
 
 // W: a team scales x of step `it` to the chunk's end and splits it into three,
-// kWRows tokens of both heads at a time: every second such quarter of the chunk.
+// kWRows tokens of both heads at a time: every second such piece of the chunk.
 template <int N, bool WHOLE>
 __device__ __forceinline__ bool scale_x(uint8_t* smem, Barriers& br, int team, int it, volatile int* dead) {
   using Sm = ChunkSmem<N, WHOLE>;
   constexpr int STG = Depth<WHOLE>::kStages, NT = Depth<WHOLE>::kTeam;
   const Steps* st = reinterpret_cast<const Steps*>(smem + Sm::kSteps) + 2 * (it & 1);
-  const int stg = it % STG, wt = threadIdx.x & (NT - 1);
+  const int stg = it % STG, wt = threadIdx.x & (NT - 1), ch = wt & 7;
   if (!ch_wait_w(&br.sc_full[it & 1], (it >> 1) & 1, dead)) return false;
   if (!ch_wait_w(&br.rdy_x[stg], (it / STG) & 1, dead)) return false;
   const uint8_t* xt = smem + Sm::kX + stg * 2 * kPanel;
+  uint8_t* wb = smem + Sm::kW + team * 6 * kWPanel;
 #pragma unroll 1
-  for (int qt = team; qt < kQ / kWRows; qt += 2) {
+  for (int i = 0; i < kPieces / 2; ++i) {
+    const int row0 = kWRows * (2 * i + team);
     // the buffer's rounds 2 it, 2 it + 1
-    if (!ch_wait_w(&br.w_free[team], (qt >> 1) ^ 1, dead)) return false;
-    uint8_t* wb = smem + Sm::kW + team * 6 * kWPanel;
+    if (!ch_wait_w(&br.w_free[team], i ^ 1, dead)) return false;
 #pragma unroll 2
-    for (int i = 0; i < 2 * kWRows * 8 / NT; ++i) {
-      const int id = i * NT + wt, h = id >> 8, r = (id >> 3) & 31, ch = id & 7;
-      const int row = kWRows * qt + r;
-      const float w = st[h].w[row];
-      const uint32_t off = (uint32_t)((ch ^ (r & 7)) << 4);
-      const uint4 xv = *reinterpret_cast<const uint4*>(xt + h * kPanel + row * 128 + off);
+    for (int k = 0; k < 512 / NT; ++k) {
+      const int h = (k * NT + wt) >> 8, r = ((k * NT + wt) >> 3) & 31;
+      const uint32_t off = (uint32_t)(r * 128 + ((ch ^ (r & 7)) << 4));
+      const float w = st[h].w[row0 + r];
+      const uint4 xv = *reinterpret_cast<const uint4*>(xt + h * kPanel + row0 * 128 + off);
       const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
       uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float e = lo_f(xs[j]) * w, o = hi_f(xs[j]) * w;
-        p0[j] = pack2(e, o);
-        e -= lo_f(p0[j]);
-        o -= hi_f(p0[j]);
-        split2(e, o, p1[j], p2[j]);
+        float2 e = mul2(make_float2(lo_f(xs[j]), hi_f(xs[j])), make_float2(w, w));
+        p0[j] = pack2(e.x, e.y);
+        e = add2(e, make_float2(-lo_f(p0[j]), -hi_f(p0[j])));
+        p1[j] = pack2(e.x, e.y);
+        e = add2(e, make_float2(-lo_f(p1[j]), -hi_f(p1[j])));
+        p2[j] = pack2(e.x, e.y);
       }
-      uint8_t* dst = wb + h * kWPanel + r * 128 + off;
+      uint8_t* dst = wb + h * kWPanel + off;
       *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
       *reinterpret_cast<uint4*>(dst + 2 * kWPanel) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
       *reinterpret_cast<uint4*>(dst + 4 * kWPanel) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
@@ -359,48 +359,16 @@ __global__ void __launch_bounds__(kChThreads, 1)
   static_assert(sizeof(Barriers) <= 400, "barrier block");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Sm::kBar + 400);
   volatile int* dead = reinterpret_cast<volatile int*>(smem + Sm::kBar + 404);
-  int* first = reinterpret_cast<int*>(smem + Sm::kBar + 408);  // pair, seq, chunk, steps, piece before, chunks, chunk of all
+  Plan* first = reinterpret_cast<Plan*>(smem + Sm::kBar + 416);
   Steps* steps = reinterpret_cast<Steps*>(smem + Sm::kSteps);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int cta = blockIdx.x, ctas = gridDim.x;
+  const int cta = blockIdx.x;
 
   if (warp == 0) {
-    // this CTA's piece of the list
-    int seq = 0, nth = 0, total = 0;
-    find_tile(a.pk, -1, kQ, 0, seq, nth, total);
-    const long long all = (long long)total * a.pairs;
-    const long long f0 = cut(all, cta, ctas), f1 = cut(all, cta + 1, ctas);
-    int n = (int)(f1 - f0), pair = 0, before = cta - 1;
-    if (n > 0)  // the piece before this one: pieces may be empty
-      while (before > 0 && cut(all, before, ctas) == f0) --before;
-    if (n > 0) {
-      int t;
-      if (WHOLE) {
-        pair = (int)(f0 / total);
-        find_tile(a.pk, (int)(f0 - (long long)pair * total), kQ, 0, seq, nth, t);
-      } else {
-        // its part of the sequence that its piece ends in, if that goes on
-        pair = (int)((f1 - 1) / total);
-        find_tile(a.pk, (int)(f1 - 1 - (long long)pair * total), kQ, 0, seq, nth, t);
-        int b, len;
-        seq_range(a.pk, seq, b, len);
-        if (nth == chunks_of(len) - 1) {
-          n = 0;
-        } else {
-          n = (int)min((long long)(nth + 1), f1 - f0);
-          nth = nth + 1 - n;
-        }
-      }
-    }
     if (lane == 0) {
-      first[0] = pair;
-      first[1] = seq;
-      first[2] = nth;
-      first[3] = n;
-      first[4] = before;
-      first[5] = total;
-      first[6] = (int)((WHOLE ? f0 : f1 - n) % max(total, 1));
-      if (!WHOLE) a.meta[cta] = n == 0 ? 0 : (pair << 2) + (nth == 0 ? 1 : 2);
+      const int4* pl = reinterpret_cast<const int4*>(a.plan + (WHOLE ? kMaxCtas : 0) + cta);
+      reinterpret_cast<int4*>(first)[0] = pl[0];
+      reinterpret_cast<int4*>(first)[1] = pl[1];
       // warps that scale x, and that read the steps
       const int scalers = WHOLE ? 8 : 16, cons = 8 + scalers + (WHOLE ? 8 : 0);
       for (int i = 0; i < 2; ++i) {
@@ -410,10 +378,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
         mbar_init(&br.rdy_x[i], 1);
         mbar_init(&br.sc_full[i], 1);
         mbar_init(&br.sc_free[i], cons);
-        mbar_init(&br.px_done[i], 1);
         mbar_init(&br.b_free[i], 1);
-        mbar_init(&br.x_read[i], scalers);
-        mbar_init(&br.p_full[i], 8);
+        mbar_init(&br.x_read[i], 16);  // scalers, and whole: y's readers
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&br.w_full[i], Depth<WHOLE>::kTeam / 32);
@@ -421,8 +387,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
       }
       mbar_init(&br.raw_c, 1);
       mbar_init(&br.cb_full, 1);
-      mbar_init(&br.cb_free, 8);
       mbar_init(&br.cs_done, 1);
+      mbar_init(&br.p_full, 8);
+      mbar_init(&br.px_done, 1);
       mbar_init(&br.y_free, 8);
       mbar_init(&br.ds_done, 1);
       mbar_init(&br.ds_free, 8);
@@ -441,9 +408,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
   __syncthreads();
   tc_after();
   const uint32_t tmem = *tmem_slot;
-  const int count = first[3];
+  const int count = first->count;
   Walk wk;
-  if (count > 0) wk.at(a.pk, first[0], first[1], first[2]);
+  if (count > 0) wk.at(a.pk, first->pair, first->seq, first->chunk);
   const int q = warp & 3;  // tensor-memory lanes 32 q ..
   const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
 
@@ -458,6 +425,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
         if (!scale_x<N, WHOLE>(smem, br, 0, it, dead)) break;
     } else if (count > 0) {
       const int side = warp >> 2, t = 32 * q + lane;
+      Heads hd;
       if (side == 1) {
         // columns behind the diagonal block stay zero
         const uint32_t z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -471,83 +439,104 @@ __global__ void __launch_bounds__(kChThreads, 1)
         const uint32_t ph = it & 1;
         if (!ch_wait_w(&br.sc_full[ph], (it >> 1) & 1, dead)) break;
         if (!ch_wait_w(&br.cb_full, ph, dead)) break;
-        bool ok = true;
+        tc_after();
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           const Steps& st = steps[2 * ph + h];
           const float lp = st.lp[t], b1 = st.blk[1], b2 = st.blk[2];
-          // this head's P buffer is free: its last product is done
-          if (!ch_wait_w(&br.px_done[h], ph ^ 1, dead)) {
-            ok = false;
-            break;
-          }
-          tc_after();
 #pragma unroll 1
           for (int j = q - side; j >= 0; j -= (q == 2 && side == 1) ? 1 : 2) {
             if (q == 2 && j == 0 && side == 0) break;
-            uint32_t v[32];
-            tm_ld32(lanes + kTmCB + 32 * j, v);
-            uint32_t o[16];
-            if (j == q) {
+            // from the end of block j to t: whole blocks between, then t's own part
+            const float u = ex2(lp + (j + 1 < q ? (j == 0 ? b1 : b2) : 0.0f) + (j + 2 < q ? b2 : 0.0f));
+#pragma unroll 1
+            for (int c = 0; c < 32; c += 16) {
+              uint32_t v[16], o[8];
+              tm_ld16(lanes + kTmCB + 32 * j + c, v);
+              if (j == q) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 ls = *reinterpret_cast<const float4*>(&st.lp[32 * j + i]);
-                const float4 ds = *reinterpret_cast<const float4*>(&st.d[32 * j + i]);
-                const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {ds.x, ds.y, ds.z, ds.w};
-                float p[4];
+                for (int i = 0; i < 16; i += 4) {
+                  const float4 ls = *reinterpret_cast<const float4*>(&st.lp[32 * j + c + i]);
+                  const float4 ds = *reinterpret_cast<const float4*>(&st.d[32 * j + c + i]);
+                  const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {ds.x, ds.y, ds.z, ds.w};
+                  float p[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  p[k] = __uint_as_float(v[i + k]) * (dv[k] * ex2(lp - lv[k]));
-                  if (i + k > lane) p[k] = 0.0f;
+                  for (int k = 0; k < 4; ++k) {
+                    p[k] = __uint_as_float(v[i + k]) * (dv[k] * ex2(lp - lv[k]));
+                    if (c + i + k > lane) p[k] = 0.0f;
+                  }
+                  o[i / 2] = pack2(p[0], p[1]);
+                  o[i / 2 + 1] = pack2(p[2], p[3]);
                 }
-                o[i / 2] = pack2(p[0], p[1]);
-                o[i / 2 + 1] = pack2(p[2], p[3]);
-              }
-            } else {
-              // from the end of block j to t: whole blocks between, then t's own part
-              const float u = ex2(lp + (j + 1 < q ? (j == 0 ? b1 : b2) : 0.0f) + (j + 2 < q ? b2 : 0.0f));
+              } else {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(&st.v[32 * j + i]);
-                o[i / 2] = pack2(__uint_as_float(v[i]) * (u * w.x), __uint_as_float(v[i + 1]) * (u * w.y));
-                o[i / 2 + 1] = pack2(__uint_as_float(v[i + 2]) * (u * w.z), __uint_as_float(v[i + 3]) * (u * w.w));
+                for (int i = 0; i < 16; i += 4) {
+                  const float4 w = *reinterpret_cast<const float4*>(&st.v[32 * j + c + i]);
+                  const float2 e = mul2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
+                                        mul2(make_float2(w.x, w.y), make_float2(u, u)));
+                  const float2 f = mul2(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])),
+                                        mul2(make_float2(w.z, w.w), make_float2(u, u)));
+                  o[i / 2] = pack2(e.x, e.y);
+                  o[i / 2 + 1] = pack2(f.x, f.y);
+                }
               }
+              tm_st8(lanes + kTmP + 64 * h + 16 * j + c / 2, o);
             }
-            tm_st16(lanes + kTmP + 64 * h + 16 * j, o);
           }
-          if (h == 1) {
-            tc_before();
-            ch_arrive_w(&br.cb_free);
-          }
-          // half of this head's row: S C times exp(c_t), plus D x
-          if (h == 0) ok = ch_wait_w(&br.cs_done, ph, dead) && ch_wait_w(&br.rdy_x[0], ph, dead);
-          if (!ok) break;
-          tc_after();
-          {
-            const float e = ex2(lp + (q > 0 ? st.blk[0] : 0.0f) + (q > 1 ? b1 : 0.0f) + (q > 2 ? b2 : 0.0f));
-            const float D = st.D;
-            uint32_t v[32];
-            tm_ld32(lanes + kTmY + 64 * h + 32 * side, v);
+        }
+        tm_wait_st();
+        tc_before();
+        ch_arrive_w(&br.p_full);
+        // y: exp(c_t) S C + P x + D x, half of each head's columns
+        if (!ch_wait_w(&br.cs_done, ph, dead)) break;
+        if (!ch_wait_w(&br.px_done, ph, dead)) break;
+        tc_after();
+        hd.at(a, wk.pair);
+        const int left = wk.valid() - 32 * q;  // rows of this warp inside the sequence
+        __nv_bfloat16* rows = a.y + (size_t)(wk.row0() + 32 * q) * a.y_stride + 32 * side;
+        uint8_t* stage = smem + Sm::kY + warp * 1024;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const Steps& st = steps[2 * ph + h];
+          const float D = st.D, e = ex2(st.lp[t] + (q > 0 ? st.blk[0] : 0.0f) + (q > 1 ? st.blk[1] : 0.0f) +
+                                        (q > 2 ? st.blk[2] : 0.0f));
+          __nv_bfloat16* y = rows + (size_t)(h ? hd.h[1] : hd.h[0]) * kP;
+          const bool put = h == 0 || hd.h[1] != hd.h[0];
+          const uint8_t* xr = smem + Sm::kX + h * kPanel + t * 128;
+#pragma unroll 1
+          for (int c = 0; c < 4; c += 2) {
+            uint32_t u[16], v[16];
+            tm_ld16x2(lanes + kTmY + 64 * h + 32 * side + 8 * c, lanes + kTmCB + 64 * h + 32 * side + 8 * c, u, v);
+            // 32 rows of 32 bytes through shared memory: two lanes store one row's
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint4 xv = *reinterpret_cast<const uint4*>(smem + Sm::kX + h * kPanel + t * 128 +
-                                                               (((4 * side + c) ^ (t & 7)) << 4));
+            for (int k = 0; k < 2; ++k) {
+              const uint4 xv = *reinterpret_cast<const uint4*>(xr + (((4 * side + c + k) ^ (t & 7)) << 4));
               const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
+              uint32_t o[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                v[8 * c + 2 * i] = __float_as_uint(fmaf(D, lo_f(xs[i]), __uint_as_float(v[8 * c + 2 * i]) * e));
-                v[8 * c + 2 * i + 1] =
-                    __float_as_uint(fmaf(D, hi_f(xs[i]), __uint_as_float(v[8 * c + 2 * i + 1]) * e));
+                const int m = 8 * k + 2 * i;
+                o[i] = pack2(fmaf(D, lo_f(xs[i]), fmaf(e, __uint_as_float(u[m]), __uint_as_float(v[m]))),
+                             fmaf(D, hi_f(xs[i]), fmaf(e, __uint_as_float(u[m + 1]), __uint_as_float(v[m + 1]))));
               }
+              *reinterpret_cast<uint4*>(stage + lane * 32 + ((k ^ ((lane >> 2) & 1)) << 4)) =
+                  make_uint4(o[0], o[1], o[2], o[3]);
             }
-            tm_st32(lanes + kTmY + 64 * h + 32 * side, v);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int r = 16 * k + (lane >> 1), i = lane & 1;
+              const uint4 val = *reinterpret_cast<const uint4*>(stage + r * 32 + ((i ^ ((r >> 2) & 1)) << 4));
+              if (put && r < left) *reinterpret_cast<uint4*>(y + (size_t)r * a.y_stride + 8 * (c + i)) = val;
+            }
+            __syncwarp();
           }
-          tm_wait_st();
-          tc_before();
-          ch_arrive_w(&br.p_full[h]);
         }
-        if (!ok) break;
+        tc_before();
+        ch_arrive_w(&br.y_free);
+        ch_arrive_w(&br.x_read[0]);
         ch_arrive_w(&br.sc_free[ph]);
+        if (it + 1 < count) wk.next(a.pk);
       }
     }
   } else if (warp < 16) {
@@ -557,6 +546,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
     const int n = 32 * q + lane;
     const bool own = n < N;
     float s[2][32];
+    float sum0 = 0.0f, sum1 = 0.0f;  // pass 1: exponent of the whole part
+    Heads hd;
     // offset of this thread's element i of a head's [kP][N] state
     auto at = [&](int i) { return (size_t)(32 * half + i) * N + n; };
     for (int it = 0; it < count; ++it) {
@@ -564,11 +555,11 @@ __global__ void __launch_bounds__(kChThreads, 1)
       if (wk.chunk == 0 || it == 0) {
         // where the state before this chunk comes from
         const int slot = a.state ? seq_slot(a.pk, wk.seq) : -1;
-        const Heads hd(a, wk.pair);
+        hd.at(a, wk.pair);
         const float* src = nullptr;
         bool slots = false;
         if (wk.chunk > 0) {
-          if (WHOLE) src = a.local + (size_t)first[4] * 2 * kP * N;
+          if (WHOLE) src = a.local + (size_t)first->before * 2 * kP * N;
         } else if (slot >= 0 && a.pk.has && a.pk.has[wk.seq]) {
           // a sequence that another CTA finishes may already have its new state in the slot
           if (WHOLE && wk.nch > count - it) src = a.init + (size_t)cta * 2 * kP * N;
@@ -614,6 +605,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
       }
       if (!ch_wait_w(&br.sc_full[ph], (it >> 1) & 1, dead)) break;
       const float d0 = steps[2 * ph].all, d1 = steps[2 * ph + 1].all;
+      if (!WHOLE) {
+        sum0 += steps[2 * ph].sum;
+        sum1 += steps[2 * ph + 1].sum;
+      }
       ch_arrive_w(&br.sc_free[ph]);
       if (!ch_wait_w(&br.ds_done, ph, dead)) break;
       tc_after();
@@ -630,7 +625,6 @@ __global__ void __launch_bounds__(kChThreads, 1)
       ch_arrive_w(&br.ds_free);
       if (WHOLE && wk.chunk == wk.nch - 1) {
         const int slot = a.state ? seq_slot(a.pk, wk.seq) : -1;
-        const Heads hd(a, wk.pair);
         if (slot >= 0 && own)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -642,6 +636,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
       }
       if (it + 1 < count) wk.next(a.pk);
     }
+    if (!WHOLE && count > 0 && tid == 256) {
+      a.decay[2 * cta] = ex2(sum0);
+      a.decay[2 * cta + 1] = ex2(sum1);
+    }
     if (!WHOLE && count > 0 && own) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -651,97 +649,42 @@ __global__ void __launch_bounds__(kChThreads, 1)
       }
     }
   } else if (warp < 24) {
-    // ------------------------------------------------------------ W, then y
+    // ------------------------------------------------------------------ W
     regs_down<kRegW>();
-    const int side = (warp - 16) >> 2;
-    uint8_t* stage = smem + Sm::kY + (warp - 16) * 1024;
-    for (int it = 0; it < count; ++it) {
-      if (!scale_x<N, WHOLE>(smem, br, WHOLE ? side : 1, it, dead)) break;
-      if (!WHOLE) continue;
-      const int left = wk.valid() - 32 * q;  // rows of this warp inside the sequence
-      const Heads hd(a, wk.pair);
-      __nv_bfloat16* rows = a.y + (size_t)(wk.row0() + 32 * q) * a.y_stride + 32 * side;
-      bool ok = true;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        if (!ch_wait_w(&br.px_done[h], it & 1, dead)) {
-          ok = false;
-          break;
-        }
-        tc_after();
-        uint32_t v[32];
-        tm_ld32(lanes + kTmY + 64 * h + 32 * side, v);
-        if (h == 1) {
-          tc_before();
-          ch_arrive_w(&br.y_free);
-          if (hd.h[1] == hd.h[0]) break;
-        }
-        __nv_bfloat16* y = rows + (size_t)(h ? hd.h[1] : hd.h[0]) * kP;
-        uint32_t o[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-        // 16 rows of 64 bytes at a time through shared memory: four lanes store one row's
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          __syncwarp();
-          if ((lane >> 4) == g) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4*>(stage + (lane & 15) * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int r = 8 * k + (lane >> 2), i = lane & 3;
-            const uint4 val = *reinterpret_cast<const uint4*>(stage + r * 64 + ((i ^ ((r >> 1) & 3)) << 4));
-            if (16 * g + r < left) *reinterpret_cast<uint4*>(y + (size_t)(16 * g + r) * a.y_stride + 8 * i) = val;
-          }
-        }
-      }
-      if (!ok) break;
-      if (it + 1 < count) wk.next(a.pk);
-    }
+    const int team = WHOLE ? (warp - 16) >> 2 : 1;
+    for (int it = 0; it < count; ++it)
+      if (!scale_x<N, WHOLE>(smem, br, team, it, dead)) break;
   } else {
     regs_down<kRegMisc>();
     if (warp == 24) {
-      // -------------------------------------------------------------- TMA
+      // --------------------------------------------- TMA of steps, C and B
       if (lane == 0) {
         // the list walks the chunks pair after pair, as the steps lie
-        const Steps* src = a.steps + 2 * ((size_t)first[0] * first[5] + first[6]);
+        const Steps* src = a.steps + 2 * ((size_t)first->pair * first->total + first->nth);
+        Heads hd;
         for (int it = 0; it < count; ++it) {
           const uint32_t ph = it & 1, sph = (it / STG) & 1;
-          const Heads hd(a, wk.pair);
+          hd.at(a, wk.pair);
           const int grp = hd.grp, row = wk.row0(), stg = it % STG;
           if (!ch_wait(&br.sc_free[ph], ((it >> 1) & 1) ^ 1, dead)) break;
           mbar_arrive_expect_tx(&br.sc_full[ph], 2 * sizeof(Steps));
           bulk_g2s(steps + 2 * ph, src, 2 * sizeof(Steps), &br.sc_full[ph]);
           src += 2;
           if (WHOLE) {
+            // C B^T and S C of the last step are done
+            if (!ch_wait(&br.cb_full, ph ^ 1, dead)) break;
             if (!ch_wait(&br.cs_done, ph ^ 1, dead)) break;
             mbar_arrive_expect_tx(&br.raw_c, Sm::kTile);
+#pragma unroll
             for (int i = 0; i < N / 64; ++i)
               ch_tma(smem + Sm::kC + i * kPanel, &c_map, grp * N + 64 * i, row, &br.raw_c);
           }
-          if (WHOLE && !ch_wait(&br.cb_full, ph ^ 1, dead)) break;
           if (!ch_wait(&br.b_free[stg], sph ^ 1, dead)) break;
           mbar_arrive_expect_tx(&br.raw_b[stg], Sm::kTile);
+#pragma unroll
           for (int i = 0; i < N / 64; ++i)
             ch_tma(smem + Sm::kB + stg * Sm::kTile + i * kPanel, &b_map, grp * N + 64 * i, row, &br.raw_b[stg]);
-          if (WHOLE && !ch_wait(&br.px_done[1], ph ^ 1, dead)) break;
-          if (!ch_wait(&br.x_read[stg], sph ^ 1, dead)) break;
-          mbar_arrive_expect_tx(&br.raw_x[stg], 2 * kPanel);
-          for (int h = 0; h < 2; ++h)
-            ch_tma(smem + Sm::kX + (2 * stg + h) * kPanel, &x_map, hd.h[h] * kP, row, &br.raw_x[stg]);
-          if (it + 1 < count) {
-            wk.next(a.pk);
-            const Heads nx(a, wk.pair);
-            for (int i = 0; i < N / 64; ++i) {
-              if (WHOLE) ch_prefetch(&c_map, nx.grp * N + 64 * i, wk.row0());
-              ch_prefetch(&b_map, nx.grp * N + 64 * i, wk.row0());
-            }
-            for (int h = 0; h < 2; ++h) ch_prefetch(&x_map, nx.h[h] * kP, wk.row0());
-          }
+          if (it + 1 < count) wk.next(a.pk);
         }
         // no copy is left in flight: wait for the last ones (a dead CTA's
         // waits return at once, so there a millisecond by the clock)
@@ -751,88 +694,96 @@ __global__ void __launch_bounds__(kChThreads, 1)
           }
         } else {
           for (int it = count > STG ? count - STG : 0; it < count; ++it) {
-            const uint32_t sph = (it / STG) & 1;
             if (WHOLE) ch_wait(&br.raw_c, it & 1, dead);
-            ch_wait(&br.raw_b[it % STG], sph, dead);
-            ch_wait(&br.raw_x[it % STG], sph, dead);
+            ch_wait(&br.raw_b[it % STG], (it / STG) & 1, dead);
+            ch_wait(&br.raw_x[it % STG], (it / STG) & 1, dead);
             ch_wait(&br.sc_full[it & 1], (it >> 1) & 1, dead);
           }
         }
       }
     } else if (warp == 25) {
-      // -------------------------------------------------------- MMAs of y
+      // --------------------------------- TMA of x, MMAs of C B^T and P x
       if (lane == 0) {
         const uint32_t base = smem_u32(smem);
-        constexpr uint32_t id_cb = ch_idesc(128, false, false), id_cs = ch_idesc(128, false, true),
-                           id_px = ch_idesc(64, false, true);
-        for (int it = 0; WHOLE && it < count; ++it) {
+        constexpr uint32_t id_cb = ch_idesc(128, false, false), id_px = ch_idesc(64, false, true);
+        Heads hd;
+        const uint64_t dc = sw_desc(base + Sm::kC, 16), db = sw_desc(base + Sm::kB, 16), dx = sw_desc(base + Sm::kX, 16);
+        for (int it = 0; it < count; ++it) {
           const uint32_t ph = it & 1;
-          if (!ch_wait(&br.rdy_b[0], ph, dead)) break;
-          if (!ch_wait(&br.raw_c, ph, dead)) break;
-          if (!ch_wait(&br.cb_free, ph ^ 1, dead)) break;
-          tc_after();
-#pragma unroll
-          for (int k = 0; k < N / 16; ++k) {
-            const uint32_t o = (k >> 2) * kPanel + (k & 3) * 32;
-            mma_ss(tmem + kTmCB, sw_desc(base + Sm::kC + o, 16), sw_desc(base + Sm::kB + o, 16), id_cb, k > 0);
-          }
-          ch_commit(&br.cb_full);
-          if (!ch_wait(&br.s_full, ph, dead)) break;
-          if (!ch_wait(&br.y_free, ph ^ 1, dead)) break;
-          tc_after();
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int k = 0; k < N / 16; ++k)
-              mma_ss(tmem + kTmY, sw_desc(base + Sm::kC + (k >> 2) * kPanel + (k & 3) * 32, 16),
-                     sw_desc(base + Sm::kS + part * 2 * Sm::kSPanel + k * 2048, Sm::kSPanel), id_cs, part + k > 0);
-          ch_commit(&br.cs_done);
-          if (!ch_wait(&br.rdy_x[0], ph, dead)) break;
-          bool ok = true;
-          for (int h = 0; h < 2; ++h) {
-            if (!ch_wait(&br.p_full[h], ph, dead)) {
-              ok = false;
-              break;
-            }
+          const int stg = it % STG;
+          if (WHOLE) {
+            if (!ch_wait(&br.rdy_b[0], ph, dead)) break;
+            if (!ch_wait(&br.raw_c, ph, dead)) break;
+            if (!ch_wait(&br.y_free, ph ^ 1, dead)) break;  // the columns' last P x is read
             tc_after();
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mma_ts(tmem + kTmY + 64 * h, tmem + kTmP + 64 * h + 8 * k,
-                     sw_desc(base + Sm::kX + h * kPanel + k * 2048, 16), id_px);
-            ch_commit(&br.px_done[h]);
+            for (int k = 0; k < N / 16; ++k) {
+              const int o = ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
+              mma_ss(tmem + kTmCB, dc + o, db + o, id_cb, k > 0);
+            }
+            ch_commit(&br.cb_full);
           }
-          if (!ok) break;
+          // the x tile's last readers, y's among them, are done with it
+          if (!ch_wait(&br.x_read[stg], ((it / STG) & 1) ^ 1, dead)) break;
+          hd.at(a, wk.pair);
+          mbar_arrive_expect_tx(&br.raw_x[stg], 2 * kPanel);
+          ch_tma(smem + Sm::kX + 2 * stg * kPanel, &x_map, hd.h[0] * kP, wk.row0(), &br.raw_x[stg]);
+          ch_tma(smem + Sm::kX + (2 * stg + 1) * kPanel, &x_map, hd.h[1] * kP, wk.row0(), &br.raw_x[stg]);
+          if (it + 1 < count) wk.next(a.pk);
+          if (!WHOLE) continue;
+          if (!ch_wait(&br.rdy_x[0], ph, dead)) break;
+          if (!ch_wait(&br.p_full, ph, dead)) break;  // P written, C B^T read
+          tc_after();
+#pragma unroll 4
+          for (int k = 0; k < 16; ++k)  // eight of each head; x's panels lie behind each other
+            mma_ts(tmem + kTmCB + 64 * (k >> 3), tmem + kTmP + 8 * k, dx + k * (2048 >> 4), id_px, (k & 7) > 0);
+          ch_commit(&br.px_done);
         }
         // every MMA is complete before tensor memory is freed
         ch_commit(&br.mma_done);
         mbar_wait(&br.mma_done, 0, 2000000000LL);
       }
     } else if (warp == 26) {
-      // --------------------------------------- MMAs of the state's new terms
+      // --------------------------- MMAs of the state's new terms and S C
       if (lane == 0) {
         const uint32_t base = smem_u32(smem);
-        constexpr uint32_t id_ds = ch_idesc(128, true, true);
+        const uint64_t dc = sw_desc(base + Sm::kC, 16), ds = sw_desc(base + Sm::kS, Sm::kSPanel);
+        constexpr uint32_t id_ds = ch_idesc(128, true, true), id_cs = ch_idesc(128, false, true);
         for (int it = 0; it < count; ++it) {
+          const uint32_t ph = it & 1;
           const int stg = it % STG;
           if (!ch_wait(&br.rdy_b[stg], (it / STG) & 1, dead)) break;
-          if (!ch_wait(&br.ds_free, (it & 1) ^ 1, dead)) break;
+          if (!ch_wait(&br.ds_free, ph ^ 1, dead)) break;
           bool ok = true;
-          for (int qt = 0; qt < kQ / kWRows; ++qt) {
-            const int buf = qt & 1;
-            if (!ch_wait(&br.w_full[buf], qt >> 1, dead)) {
-              ok = false;
-              break;
+#pragma unroll 1
+          for (int pc = 0; pc < kPieces; ++pc) {
+            if (WHOLE && pc == kPieces / 2) {
+              // S C, half way: the split state is ready by then, and W need not wait for it
+              ok = ch_wait(&br.s_full, ph, dead) && ch_wait(&br.raw_c, ph, dead) &&
+                   ch_wait(&br.y_free, ph ^ 1, dead);
+              if (!ok) break;
+              tc_after();
+#pragma unroll 4
+              for (int i = 0; i < N / 8; ++i) {
+                const int part = i / (N / 16), k = i % (N / 16);
+                mma_ss(tmem + kTmY, dc + (((k >> 2) * kPanel + (k & 3) * 32) >> 4),
+                       ds + ((part * 2 * Sm::kSPanel + k * 2048) >> 4), id_cs, i > 0);
+              }
+              ch_commit(&br.cs_done);
             }
+            const int buf = pc & 1;
+            ok = ch_wait(&br.w_full[buf], pc >> 1, dead);
+            if (!ok) break;
             tc_after();
+            // fewer than 128 state columns: the rows behind them repeat the first (panel stride 0)
+            const uint64_t da = sw_desc(base + Sm::kB + stg * Sm::kTile + kWRows * pc * 128, N == 128 ? kPanel : 0);
+            const uint64_t db = sw_desc(base + Sm::kW + 6 * buf * kWPanel, kWPanel);
 #pragma unroll
             for (int part = 0; part < 3; ++part)
 #pragma unroll
               for (int k = 0; k < kWRows / 16; ++k)
-                // fewer than 128 state columns: the rows behind them repeat the first (panel stride 0)
-                mma_ss(tmem + kTmS,
-                       sw_desc(base + Sm::kB + stg * Sm::kTile + (kWRows * qt + 16 * k) * 128, N == 128 ? kPanel : 0),
-                       sw_desc(base + Sm::kW + (6 * buf + 2 * part) * kWPanel + k * 2048, kWPanel), id_ds,
-                       qt + part + k > 0);
+                mma_ss(tmem + kTmS, da + k * (2048 >> 4), db + (2 * part * kWPanel + k * 2048 >> 4), id_ds,
+                       pc + part + k > 0);
             ch_commit(&br.w_free[buf]);
           }
           if (!ok) break;
@@ -844,16 +795,11 @@ __global__ void __launch_bounds__(kChThreads, 1)
       }
     } else {
       // ------------------------------------------- rows behind an end
-      float sum0 = 0.0f, sum1 = 0.0f;  // pass 1: exponent of the whole part
-      const Steps* src = a.steps + 2 * ((size_t)first[0] * first[5] + first[6]);
       const uint4 zero = make_uint4(0, 0, 0, 0);
+      Heads hd;
       for (int it = 0; it < count; ++it) {
         const uint32_t sph = (it / STG) & 1;
         const int valid = wk.valid(), stg = it % STG;
-        if (!WHOLE) {
-          sum0 += src[2 * it].sum;
-          sum1 += src[2 * it + 1].sum;
-        }
         if (!ch_wait_w(&br.raw_b[stg], sph, dead)) break;
         if (valid < kQ) {
           for (int i = lane; i < (kQ - valid) * 8; i += 32)
@@ -872,13 +818,23 @@ __global__ void __launch_bounds__(kChThreads, 1)
           to_async();
         }
         ch_arrive_w(&br.rdy_x[stg]);
-        if (it + 1 < count) wk.next(a.pk);
+        if (it + 1 < count) {
+          wk.next(a.pk);
+          hd.at(a, wk.pair);
+          if (lane < N / 64) {
+            if (WHOLE) ch_prefetch(&c_map, hd.grp * N + 64 * lane, wk.row0());
+            ch_prefetch(&b_map, hd.grp * N + 64 * lane, wk.row0());
+          } else if (lane < N / 64 + 2) {
+            ch_prefetch(&x_map, (lane == N / 64 ? hd.h[0] : hd.h[1]) * kP, wk.row0());
+          }
+          __syncwarp();
+        }
       }
-      if (!WHOLE && count > 0 && lane < 2) a.decay[2 * cta + lane] = ex2(lane ? sum1 : sum0);
     }
   }
   tc_before();
   __syncthreads();
+  if (tid == 0 && *dead) atomicExch(&g_device_error, kErrTimeout);
   if (warp == 25)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
@@ -887,16 +843,66 @@ __global__ void __launch_bounds__(kChThreads, 1)
 // lane holds four tokens, eight lanes a block of 32.
 constexpr int kStepThreads = 256;
 
-__global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a) {
+// A warp finds the pieces of CTA c for both passes.
+__device__ __noinline__ void scan_plan(const ChunkArgs& a, int c, int ctas) {
+  int seq = 0, nth = 0, total = 0;
+  find_tile(a.pk, -1, kQ, 0, seq, nth, total);
+  const long long all = (long long)total * a.pairs;
+  const long long f0 = cut(all, c, ctas), f1 = cut(all, c + 1, ctas);
+  const int n = (int)(f1 - f0);
+  Plan p3{}, p1{};
+  if (n > 0) {
+    int before = c - 1, t;
+    while (before > 0 && cut(all, before, ctas) == f0) --before;
+    p3.pair = (int)(f0 / total);
+    p3.nth = (int)(f0 - (long long)p3.pair * total);
+    find_tile(a.pk, p3.nth, kQ, 0, p3.seq, p3.chunk, t);
+    p3.count = n;
+    p3.before = before;
+    p3.total = total;
+    // pass 1: its part of the sequence that its piece ends in, if that goes on
+    p1.pair = (int)((f1 - 1) / total);
+    const int last = (int)(f1 - 1 - (long long)p1.pair * total);
+    find_tile(a.pk, last, kQ, 0, p1.seq, p1.chunk, t);
+    int b, len;
+    seq_range(a.pk, p1.seq, b, len);
+    if (p1.chunk < chunks_of(len) - 1) {
+      p1.count = min(p1.chunk + 1, n);
+      p1.chunk += 1 - p1.count;
+      p1.nth = last + 1 - p1.count;
+      p1.total = total;
+    }
+  }
+  if ((threadIdx.x & 31) == 0) {
+    a.plan[c] = p1;
+    a.plan[kMaxCtas + c] = p3;
+    a.meta[c] = p1.count == 0 ? 0 : (p1.pair << 2) + (p1.chunk == 0 ? 1 : 2);
+  }
+}
+
+__global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a, int ctas) {
   const int lane = threadIdx.x & 31, chunk = blockIdx.x;
+  if (blockIdx.y == gridDim.y - 1) {  // the last row of blocks: pieces
+    const int c = blockIdx.x * (kStepThreads / 32) + (threadIdx.x >> 5);
+    if (c < ctas) scan_plan(a, c, ctas);
+    return;
+  }
   const int ph = blockIdx.y * (kStepThreads / 32) + (threadIdx.x >> 5);  // pair and head
   int seq = 0, nth = 0, total = 0;
   if (!find_tile(a.pk, chunk, kQ, 0, seq, nth, total) || ph >= 2 * a.pairs) return;
-  int seq_, nth_;
-  find_tile(a.pk, -1, kQ, 0, seq_, nth_, total);
+  if (a.pk.seqs > 1) {
+    int s, n;
+    find_tile(a.pk, -1, kQ, 0, s, n, total);
+  } else {
+    int b, len;
+    seq_range(a.pk, 0, b, len);
+    total = chunks_of(len);
+  }
   Walk wk;
   wk.at(a.pk, ph >> 1, seq, nth);
-  const int head = Heads(a, ph >> 1).h[ph & 1], valid = wk.valid(), row = wk.row0();
+  Heads hd;
+  hd.at(a, ph >> 1);
+  const int head = hd.h[ph & 1], valid = wk.valid(), row = wk.row0();
   const float bias = a.dt_bias ? a.dt_bias[head] : 0.0f, A2 = a.A[head] * 1.4426950408889634f;
   float d[4], e[4];
 #pragma unroll
@@ -1076,6 +1082,7 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   a.init = a.local + part;
   a.decay = a.init + part;
   a.meta = reinterpret_cast<int*>(a.decay + 2 * kMaxCtas);
+  a.plan = reinterpret_cast<Plan*>(a.meta + 2 * kMaxCtas);
   CUtensorMap xm, bm, cm;
   if (int e = ch_map(&xm, s.x, s.pk.tokens, s.heads * kP, s.x_stride)) return e;
   if (int e = ch_map(&bm, s.B, s.pk.tokens, s.groups * N, s.b_stride)) return e;
@@ -1088,8 +1095,11 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   int ctas = device_sm_count();
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (most < ctas) ctas = (int)most;
-  scan_steps_kernel<<<dim3((unsigned)chunks, (2 * a.pairs + kStepThreads / 32 - 1) / (kStepThreads / 32)), kStepThreads, 0,
-                      stream>>>(a);
+  // one warp a (chunk, head) and, in a last row of blocks, one a CTA's piece
+  const unsigned plans = (ctas + kStepThreads / 32 - 1) / (kStepThreads / 32);
+  scan_steps_kernel<<<dim3(chunks > plans ? (unsigned)chunks : plans,
+                           (2 * a.pairs + kStepThreads / 32 - 1) / (kStepThreads / 32) + 1),
+                      kStepThreads, 0, stream>>>(a, ctas);
   pass1<<<ctas, kChThreads, smem1, stream>>>(xm, bm, cm, a);
   scan_join_kernel<<<dim3((2 * kP * N / 4 + kJoinThreads - 1) / kJoinThreads, a.pairs), kJoinThreads, 0, stream>>>(a, ctas);
   pass3<<<ctas, kChThreads, smem3, stream>>>(xm, bm, cm, a);
@@ -1101,7 +1111,7 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
 size_t ssm_prompt_scratch_bytes(int type, int tokens, int seqs, int heads, int head_dim, int groups, int d_state) {
   if (!chunk_sizes(type, tokens, head_dim, d_state)) return 0;
   const size_t pairs = (size_t)(heads / groups + 1) / 2 * groups;
-  return ((size_t)tokens / kQ + seqs) * pairs * 2 * sizeof(Steps) + (size_t)kMaxCtas * (4 * kP * d_state * 4 + 16);
+  return ((size_t)tokens / kQ + seqs) * pairs * 2 * sizeof(Steps) + (size_t)kMaxCtas * (4 * kP * d_state * 4 + 16 + 2 * sizeof(Plan));
 }
 
 int launch_ssm_prompt(const ScanArgs& a, cudaStream_t stream) {
