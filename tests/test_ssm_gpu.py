@@ -124,7 +124,7 @@ def run_scan(k, cuda, c, dtype, slots=True, has=True, state=True, extras=True):
     h, p, gr, n = c["dims"]
     inner, bc = h * p, gr * n
     xbc, y = c["xbc"].to(cuda), torch.full((c["t"], inner), 9.0, dtype=dtype, device=cuda)
-    st = c["state"].to(cuda) if state else None
+    st = c["state"].to(cuda, copy=True) if state else None
     k.ssm_prompt(y, xbc[:, :inner], put(c["dt"], cuda), put(c["A"], cuda), xbc[:, inner:inner + bc],
                  xbc[:, inner + bc:], put(c["D"], cuda) if extras else None, put(c["bias"], cuda) if extras else None,
                  st, ints(c["cu"], cuda), c["s"], c["t"], h, p, gr, n,
@@ -181,6 +181,18 @@ def test_scan_f32(k, cuda, lens, lead, tail):
 @pytest.mark.parametrize("heads,groups", [(1, 1), (2, 2), (3, 1), (8, 1), (9, 1), (16, 2), (21, 3)])
 def test_scan_heads_and_groups(k, cuda, heads, groups):
     c = scan_case([150, 20], heads, 64, groups, 128, BF16, seed=heads)
+    y, st, want = run_scan(k, cuda, c, BF16)
+    check_scan(y, st, want, c, BF16)
+
+
+@pytest.mark.parametrize("lens,heads,groups,d_state", [
+    ([2100], 64, 8, 128), ([700, 3, 0, 1290, 128, 64], 64, 8, 128), ([1500, 400], 40, 8, 64), ([3000], 16, 2, 128),
+    ([257] * 9, 35, 7, 128)])
+def test_scan_many_chunks(k, cuda, lens, heads, groups, d_state):
+    """Several chunks to a CTA, pieces cut inside sequences and at their ends."""
+    c = scan_case(lens, heads, 64, groups, d_state, BF16, 1, 2, seed=heads)
+    for v in ("xbc", "dt", "A", "D", "bias", "state"):
+        c[v] = c[v].to(cuda)  # the reference runs there too
     y, st, want = run_scan(k, cuda, c, BF16)
     check_scan(y, st, want, c, BF16)
 
