@@ -12,7 +12,7 @@
 //   warp 0      producer: TMA of both operands' tiles into a ring of stages
 //   warp 1      one lane issues the tcgen05.mma of each stage into one of two
 //               accumulator buffers in tensor memory
-//   warps 2..9  epilogue: tcgen05.ld of a finished buffer (two warps a quarter
+//   the others  epilogue: tcgen05.ld of a finished buffer (two warps a quarter
 //               of its lanes, half the columns each), bias, activation,
 //               residual, store -- while the next tile's MMAs run; bias and
 //               residual are loaded one step ahead
@@ -36,7 +36,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
-#include "ssm.h"
+#include "ssm_dev.cuh"
 
 namespace ervf {
 
@@ -45,13 +45,14 @@ namespace {
 constexpr int kLinM = 128, kLinKB = 64;
 constexpr int kLinEpi = 8, kLinThreads = (2 + kLinEpi) * 32;
 constexpr int kLinATile = kLinM * kLinKB * 2;
+constexpr int kLinPitch = 20, kLinStage = 32 * kLinPitch * 4;  // an epilogue warp's staging, bytes
 
 template <int BN, int CH>
 struct LinShape {
   static constexpr int kBTile = BN * kLinKB * 2;
   static constexpr int kStage = kLinATile + kBTile;  // both multiples of 1024 bytes (swizzle period)
   static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
-  static constexpr int kSmem = 1024 + 1024 + kStages * kStage;  // barriers, alignment slack, ring
+  static constexpr int kSmem = 1024 + 1024 + kStages * kStage + kLinEpi * kLinStage;  // barriers, alignment slack, ring, staging
   static constexpr int kTmemCols = 2 * CH * BN;  // buffer d, chain c at columns (d CH + c) BN
   static_assert(BN % 16 == 0 && BN <= 256 && kTmemCols >= 32 && kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0,
                 "tile");
@@ -66,7 +67,18 @@ struct LinTile {
   int rows, cols, tokens;
   int act;
   int nkb, mtiles, ntiles, splits;
+  int vec;  // out, resid and bias take 16-byte accesses at every 16th feature
 };
+
+// Unit u's tile: along bands of eight tiles of M, so that the tiles in work at a
+// time share both operands' rows in L2.
+__device__ __forceinline__ void lin_place(const LinTile& a, int u, int& mt, int& nt) {
+  constexpr int kBand = 8;
+  const int per = kBand * a.ntiles, band = u / per, first = band * kBand, size = min(a.mtiles - first, kBand);
+  u -= band * per;
+  nt = u / size;
+  mt = first + u - nt * size;
+}
 
 __device__ __forceinline__ uint64_t lin_desc(uint32_t saddr) {
   // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart
@@ -108,14 +120,22 @@ __device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, volatil
   return true;
 }
 
-__device__ __forceinline__ float lin_act(float v, int act) {
+// One branch for all N values.
+template <int N>
+__device__ __forceinline__ void lin_act(float (&v)[N], int act) {
   if (act == kActRelu2) {
-    const float r = v < 0.0f ? 0.0f : v;  // a NaN stays one
-    return r * r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float r = v[i] < 0.0f ? 0.0f : v[i];  // a NaN stays one
+      v[i] = r * r;
+    }
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = silu(v[i]);
+  } else if (act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
   }
-  if (act == kActSilu) return v / (1.0f + expf(-v));
-  if (act == kActGelu) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-  return v;
 }
 
 template <typename T>
@@ -129,66 +149,89 @@ __device__ __forceinline__ void lin_put(T* p, float v) {
   else *p = v;
 }
 
-// What 16 consecutive features r.. of token t need beside their sums.
+// 16 features r.. of a warp's tokens t0 .. t0 + 31.  The sums arrive one token a
+// lane and go through shared memory, so that neighbouring lanes write one
+// token's features: whole sectors, where a lane's own row gave 32 half ones an
+// instruction (4096 x 4096 tokens x features of 512 columns: 30 us).  Bias and
+// residual are loaded ahead of the sums.
 template <typename T>
 struct LinRow {
-  static constexpr int V = 16 / sizeof(T), kVecs = 16 / V;
-  bool whole;  // 16 features, all aligned
-  float4 bias[4];
-  uint4 resid[kVecs];
-  __device__ __forceinline__ void load(const LinTile& a, int t, int r) {
-    whole = t < a.tokens && r + 16 <= a.rows;
+  static constexpr int V = 16 / sizeof(T), kLanes = 16 / V, kRows = 32 / kLanes, kIters = 32 / kRows;
+  bool whole;
+  float bias[V];
+  uint4 resid[kIters];
+  __device__ __forceinline__ void load(const LinTile& a, int t0, int r) {
+    whole = a.vec && r + 16 <= a.rows;
     if (!whole) return;
-    const T* o = static_cast<const T*>(a.out) + (size_t)t * a.out_stride + r;
-    const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + r : nullptr;
-    whole = ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(q) |
-              (a.bias ? reinterpret_cast<uintptr_t>(a.bias + r) : 0)) & 15) == 0;
-    if (!whole) return;
+    const int lane = threadIdx.x & 31, f = r + (lane % kLanes) * V, t = t0 + lane / kLanes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      bias[i] = a.bias ? *reinterpret_cast<const float4*>(a.bias + r + 4 * i) : make_float4(0, 0, 0, 0);
+    for (int i = 0; i < V; i += 4) {
+      const float4 b = a.bias ? *reinterpret_cast<const float4*>(a.bias + f + i) : make_float4(0, 0, 0, 0);
+      bias[i] = b.x; bias[i + 1] = b.y; bias[i + 2] = b.z; bias[i + 3] = b.w;
+    }
+    const T* q = static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + f;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      resid[i] = q ? *reinterpret_cast<const uint4*>(q + i * V) : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < kIters; ++k)
+      resid[k] = a.resid && t + k * kRows < a.tokens
+                     ? *reinterpret_cast<const uint4*>(q + (size_t)(k * kRows) * a.resid_stride)
+                     : make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void store(const LinTile& a, int t, int r, const float (&acc)[16]) const {
-    if (t >= a.tokens || r >= a.rows) return;
-    T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + r;
-    if (whole) {
+  __device__ __forceinline__ void store(const LinTile& a, int t0, int r, const float (&acc)[16], float* stage) const {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const T* re = reinterpret_cast<const T*>(&resid[i]);
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<float4*>(stage + lane * kLinPitch + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    __syncwarp();
+    if (whole) {
+      const int c = (lane % kLanes) * V, t = t0 + lane / kLanes;
+      T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + r + c;
+#pragma unroll
+      for (int k = 0; k < kIters; ++k) {
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(stage + (k * kRows + lane / kLanes) * kLinPitch + c + i);
+          v[i] = q.x + bias[i]; v[i + 1] = q.y + bias[i + 1]; v[i + 2] = q.z + bias[i + 2]; v[i + 3] = q.w + bias[i + 3];
+        }
+        lin_act(v, a.act);
+        const T* re = reinterpret_cast<const T*>(&resid[k]);
         uint4 oq;
         T* oe = reinterpret_cast<T*>(&oq);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int k = i * V + j;
-          const float4 b = bias[k / 4];
-          const float bb[4] = {b.x, b.y, b.z, b.w};
-          const float v = lin_act(acc[k] + bb[k % 4], a.act);
-          lin_put(oe + j, a.resid ? v + lin_get(re + j) : v);
-        }
-        *reinterpret_cast<uint4*>(o + i * V) = oq;
+        for (int i = 0; i < V; ++i) lin_put(oe + i, a.resid ? v[i] + lin_get(re + i) : v[i]);
+        if (t + k * kRows < a.tokens) *reinterpret_cast<uint4*>(o + (size_t)(k * kRows) * a.out_stride) = oq;
       }
-      return;
-    }
-    const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + r : nullptr;
+    } else if (r + (lane & 15) < a.rows) {
+      // rows of any alignment, the last features: 16 lanes to a token
+      const int f = r + (lane & 15), t = t0 + (lane >> 4);
+      const float b = a.bias ? a.bias[f] : 0.0f;
+      const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + f : nullptr;
+      T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + f;
 #pragma unroll 1
-    for (int i = 0; i < 16; ++i)
-      if (r + i < a.rows) {
-        float v = acc[0];
+      for (int i = 0; i < 16; i += 8) {
+        float v[8], res[8];
 #pragma unroll
-        for (int k = 1; k < 16; ++k) v = i == k ? acc[k] : v;
-        v = lin_act(v + (a.bias ? a.bias[r + i] : 0.0f), a.act);
-        lin_put(o + i, q ? v + lin_get(q + i) : v);
+        for (int k = 0; k < 8; ++k) {
+          res[k] = q && t + 2 * (i + k) < a.tokens ? lin_get(q + (size_t)(2 * (i + k)) * a.resid_stride) : 0.0f;
+          v[k] = stage[(2 * (i + k) + (lane >> 4)) * kLinPitch + (lane & 15)] + b;
+        }
+        lin_act(v, a.act);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (t + 2 * (i + k) < a.tokens) lin_put(o + (size_t)(2 * (i + k)) * a.out_stride, q ? v[k] + res[k] : v[k]);
       }
+    }
+    __syncwarp();
   }
 };
 
 // One sum of feature m of token t.
 template <typename T>
 __device__ __forceinline__ void lin_one(const LinTile& a, int t, int m, float bias, float f) {
-  float o = lin_act(f + bias, a.act);
+  float v[1] = {f + bias};
+  lin_act(v, a.act);
+  float o = v[0];
   if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + m);
   lin_put(static_cast<T*>(a.out) + (size_t)t * a.out_stride + m, o);
 }
@@ -306,6 +349,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
   } else {
     const int q = warp & 3;  // tensor-memory lanes 32 q ..
+    float* stage = reinterpret_cast<float*>(ring + Sh::kStages * Sh::kStage) + (warp - 2) * (kLinStage / 4);
     // 16 columns of buffer d, its chains added in order
     auto sums = [&](int d, int c, float (&f)[16]) {
 #pragma unroll
@@ -327,7 +371,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       float bias = 0.0f;
       if constexpr (!SPLIT) {
         if constexpr (SWAP) bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
-        else pre.load(a, m, nt * BN + c0);
+        else pre.load(a, m - lane, nt * BN + c0);
       }
       const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
       if (!__all_sync(0xffffffffu, w_ok)) break;
@@ -335,7 +379,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll 1
       for (int c = c0; c < c0 + kCols; c += 16) {
         LinRow<T> ahead;
-        if constexpr (!SPLIT && !SWAP) ahead.load(a, m, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
+        if constexpr (!SPLIT && !SWAP) ahead.load(a, m - lane, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
         float f[16];
         sums(d, c, f);
         if constexpr (SPLIT) {
@@ -348,7 +392,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           for (int i = 0; i < 16; ++i)
             if (m < a.rows && nt * BN + c + i < a.tokens) lin_one<T>(a, nt * BN + c + i, m, bias, f[i]);
         } else {
-          pre.store(a, m, nt * BN + c, f);
+          pre.store(a, m - lane, nt * BN + c, f, stage);
           pre = ahead;
         }
         __syncwarp();
@@ -366,6 +410,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       // tokens), or 16 of them (of features)
       const int q = warp & 3, mt = u0 % a.mtiles, nt = u0 / a.mtiles, m = mt * kLinM + 32 * q + lane;
       const int who = rank + a.splits * ((warp - 2) / 4), all = a.splits * (kLinEpi / 4);
+      float* stage = reinterpret_cast<float*>(ring + Sh::kStages * Sh::kStage) + (warp - 2) * (kLinStage / 4);
       const float* part = reinterpret_cast<const float*>(ring) + 32 * q + lane;
       if constexpr (SWAP) {
         const int cols = min(BN, a.tokens - nt * BN);
@@ -381,7 +426,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       } else {
         for (int c = 16 * who; c < BN; c += 16 * all) {
           LinRow<T> pre;
-          pre.load(a, m, nt * BN + c);
+          pre.load(a, m - lane, nt * BN + c);
           float f[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] = 0.0f;
@@ -393,7 +438,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) f[i] += v[i];
           }
-          pre.store(a, m, nt * BN + c, f);
+          pre.store(a, m - lane, nt * BN + c, f, stage);
         }
       }
     }
@@ -410,11 +455,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
 // One 256 x BN tile by two CTAs: each loads its 128 rows of x and half of the
 // tile's BN rows of W; the even one issues the MMAs of both.
+// Sixteen epilogue warps: with eight, a tile's epilogue took 4.1 us (4096 x 4096,
+// 64 columns), longer than its MMAs below 700 columns.
+constexpr int kPairEpi = 16, kPairThreads = (2 + kPairEpi) * 32;
 constexpr int kPairTile = 128 * kLinKB * 2;  // x's part in one CTA
 template <int BN>
 struct PairShape {
-  static constexpr int kStage = kPairTile + BN / 2 * kLinKB * 2, kStages = BN == 256 ? 6 : 8;
-  static constexpr int kSmem = 2048 + kStages * kStage;
+  static constexpr int kStage = kPairTile + BN / 2 * kLinKB * 2, kStages = BN == 256 ? 5 : 7;
+  static constexpr int kSmem = 2048 + kStages * kStage + kPairEpi * kLinStage;
 };
 
 __device__ __forceinline__ uint32_t lead_addr(const void* p) {
@@ -436,7 +484,7 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
 }
 
 template <int BN, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, LinTile a) {
   constexpr int kPairStages = PairShape<BN>::kStages, kPairStage = PairShape<BN>::kStage;
   extern __shared__ uint8_t smem_raw[];
@@ -460,7 +508,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&dfull[i], 1);
-      mbar_init(&dempty[i], 2 * kLinEpi);
+      mbar_init(&dempty[i], 2 * kPairEpi);
     }
     mbar_init(mma_done, 1);
     *dead = 0;
@@ -482,7 +530,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
     if (lane == 0) {
       uint32_t gk = 0;
       for (int u = u0; u < units && !*dead; u += step) {
-        const int mt = u % a.mtiles, nt = u / a.mtiles;
+        int mt, nt;
+        lin_place(a, u, mt, nt);
         for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
           const int s = (int)(gk % kPairStages);
           if (!lin_wait(&empty[s], ((gk / kPairStages) & 1) ^ 1, dead)) break;
@@ -539,27 +588,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLinThreads, 1)
     }
   } else {
     const int q = warp & 3;  // tensor-memory lanes 32 q ..
-    const int c0 = (warp - 2) / 4 * (BN / 2);
+    constexpr int kCols = BN / (kPairEpi / 4);  // columns of a warp
+    const int c0 = (warp - 2) / 4 * kCols;
+    float* stage = reinterpret_cast<float*>(ring + kPairStages * kPairStage) + (warp - 2) * (kLinStage / 4);
     int nu = 0;
     for (int u = u0; u < units && !*dead; u += step, ++nu) {
-      const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
+      const int d = nu & 1;
+      int mt, nt;
+      lin_place(a, u, mt, nt);
       const int m = (2 * mt + rank) * 128 + 32 * q + lane;
       LinRow<T> pre;
-      pre.load(a, m, nt * BN + c0);
+      pre.load(a, m - lane, nt * BN + c0);
       const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
       if (!__all_sync(0xffffffffu, w_ok)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-      for (int c = c0; c < c0 + BN / 2; c += 16) {
+      for (int c = c0; c < c0 + kCols; c += 16) {
         LinRow<T> ahead;
-        ahead.load(a, m, c + 16 < c0 + BN / 2 ? nt * BN + c + 16 : a.rows);
+        ahead.load(a, m - lane, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
         uint32_t v[16];
         lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-        pre.store(a, m, nt * BN + c, f);
+        pre.store(a, m - lane, nt * BN + c, f, stage);
         pre = ahead;
         __syncwarp();
       }
@@ -611,10 +664,18 @@ int lin_map(CUtensorMap* map, const uint16_t* p, int rows, int cols, long long s
              : kErrArg;
 }
 
+int lin_vec(const LinearArgs& l) {
+  const unsigned long long e = l.out_type == kTypeBF16 ? 2 : 4;
+  const unsigned long long all = reinterpret_cast<uintptr_t>(l.out) | reinterpret_cast<uintptr_t>(l.resid) |
+                                 reinterpret_cast<uintptr_t>(l.bias) | l.out_stride * e |
+                                 (l.resid ? l.resid_stride * e : 0);
+  return (all & 15) == 0;
+}
+
 template <int BN, int CH, bool SWAP, bool SPLIT, typename T>
 int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   using Sh = LinShape<BN, CH>;
-  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits};
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits, lin_vec(l)};
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   const int ma = SWAP ? l.rows : l.tokens, nb = SWAP ? l.tokens : l.rows;
   a.mtiles = (ma + kLinM - 1) / kLinM;
@@ -645,7 +706,7 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
 template <int BN, typename T>
 int linear_pair(const LinearArgs& l, cudaStream_t stream) {
   constexpr int kPairSmem = PairShape<BN>::kSmem;
-  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, 1};
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, 1, lin_vec(l)};
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   a.mtiles = (l.tokens + 255) / 256;
   a.ntiles = (l.rows + BN - 1) / BN;
@@ -658,7 +719,7 @@ int linear_pair(const LinearArgs& l, cudaStream_t stream) {
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess)
     return kErrLaunch;
   const int pairs = device_sm_count() / 2;
-  fn<<<2 * (unsigned)(units < pairs ? units : pairs), kLinThreads, kPairSmem, stream>>>(xm, wm, a);
+  fn<<<2 * (unsigned)(units < pairs ? units : pairs), kPairThreads, kPairSmem, stream>>>(xm, wm, a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
