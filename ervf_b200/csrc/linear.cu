@@ -226,14 +226,11 @@ struct LinRow {
   }
 };
 
-// One sum of feature m of token t.
+// Feature m of token t, behind its activation.
 template <typename T>
-__device__ __forceinline__ void lin_one(const LinTile& a, int t, int m, float bias, float f) {
-  float v[1] = {f + bias};
-  lin_act(v, a.act);
-  float o = v[0];
-  if (a.resid) o += lin_get(static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + m);
-  lin_put(static_cast<T*>(a.out) + (size_t)t * a.out_stride + m, o);
+__device__ __forceinline__ void lin_one(const LinTile& a, int t, int m, float v) {
+  if (a.resid) v += lin_get(static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + m);
+  lin_put(static_cast<T*>(a.out) + (size_t)t * a.out_stride + m, v);
 }
 
 __device__ __forceinline__ float lin_remote(const float* p, int rank) {
@@ -389,8 +386,11 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           for (int i = 0; i < 16; ++i) part[i * kLinM] = f[i];
         } else if constexpr (SWAP) {
 #pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] += bias;
+          lin_act(f, a.act);
+#pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (m < a.rows && nt * BN + c + i < a.tokens) lin_one<T>(a, nt * BN + c + i, m, bias, f[i]);
+            if (m < a.rows && nt * BN + c + i < a.tokens) lin_one<T>(a, nt * BN + c + i, m, f[i]);
         } else {
           pre.store(a, m - lane, nt * BN + c, f, stage);
           pre = ahead;
@@ -416,12 +416,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         const int cols = min(BN, a.tokens - nt * BN);
         const float bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
         for (int c = who; c < cols; c += all) {
-          float v[8], f = 0.0f;
+          float v[8], f[1] = {0.0f};
 #pragma unroll
           for (int r = 0; r < 8; ++r) v[r] = r < a.splits ? lin_remote(part + (size_t)c * kLinM, r) : 0.0f;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) f += v[r];  // in rank order
-          if (m < a.rows) lin_one<T>(a, nt * BN + c, m, bias, f);
+          for (int r = 0; r < 8; ++r) f[0] += v[r];  // in rank order
+          f[0] += bias;
+          lin_act(f, a.act);
+          if (m < a.rows) lin_one<T>(a, nt * BN + c, m, f[0]);
         }
       } else {
         for (int c = 16 * who; c < BN; c += 16 * all) {

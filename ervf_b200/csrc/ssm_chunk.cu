@@ -18,11 +18,11 @@
 // Exponents are sums of numbers of one sign (distances within blocks of 32
 // tokens plus whole blocks), so no difference of two long sums is taken but
 // inside a block.  Products meet the tensor cores in bf16: B, C and x are bf16
-// already.  The in-chunk weights P are rounded to bf16 once (2^-8 of each
-// term at most, as the output's own rounding; two parts would cost the tensor
-// memory that lets both heads' P be in work at once); D x is added in f32.  S is split into two
-// bf16 numbers for S C (2^-16), the state's new terms into three (2^-24: states
-// stay f32).
+// already.  The in-chunk weights P are rounded to bf16 once (2^-8 of each term
+// at most, as the output's own rounding; a second part would take the tensor
+// memory that keeps both heads' P in work at once); D x is added in f32.  S is
+// split into two bf16 numbers for S C (2^-16), the state's new terms into
+// three (2^-24: states stay f32).
 //
 // Warps (a warpgroup's register share in brackets), and what bounds them at
 // 128 state columns (clocks per step of two heads, measured tcgen05 rates):
@@ -39,9 +39,14 @@
 //          no zero weight
 // The MMAs take 4370 clocks.  Both operands of a 128-column MMA in shared
 // memory take its whole bandwidth (128 bytes a clock); with W, the split state
-// and the tiles a step moves 740 KB there, 5800 clocks.  The loops are kept short
-// (short waits, little unrolling): seven roles' code does not fit the
-// instruction cache otherwise.
+// and the tiles a step moves 740 KB there, 5800 clocks; its warps issue 5100
+// instructions a scheduler.  Measured: 11000 clocks, of which P takes 3500, P x
+// 1300 and y 3600 one after the other (64 heads, 8192 tokens: 153 us in all,
+// 27 of them pass 1, 15 passes 0 and 2).  Waits are short and loops little
+// unrolled on purpose: seven roles' code has to share the instruction cache
+// (waits that watched the clock and unrolled MMA loops: 97 KB, 179 us).  Tried
+// without gain: y of the second head by the W warps, S C ahead of the state's
+// new terms, W pieces of 16 tokens, C B^T pieces loaded once for both heads.
 // In pass 1 warps 0..7 do W's work too.
 // Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
 // dead, and every role leaves; copies and MMAs are drained first.
