@@ -97,12 +97,14 @@ __device__ __forceinline__ void lin_commit(uint64_t* bar) {
                ::"r"(smem_u32(bar)) : "memory");
 }
 
+// The wait in the same statement: nothing may use the registers before it.
 __device__ __forceinline__ void lin_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
+      : "r"(taddr) : "memory");
 }
 
 // Bounded wait that also gives up when another role of the CTA died.
@@ -353,7 +355,6 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       for (int h = 0; h < CH; ++h) {
         uint32_t v[16];
         lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)((d * CH + h) * BN + c), v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = h ? f[i] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
       }
@@ -610,7 +611,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         ahead.load(a, m - lane, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
         uint32_t v[16];
         lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);

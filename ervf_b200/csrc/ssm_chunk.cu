@@ -190,13 +190,14 @@ __device__ __forceinline__ void tm_ld16x2(uint32_t t, uint32_t t2, uint32_t (&v)
         "=r"(w[8]), "=r"(w[9]), "=r"(w[10]), "=r"(w[11]), "=r"(w[12]), "=r"(w[13]), "=r"(w[14]), "=r"(w[15])
       : "r"(t), "r"(t2) : "memory");
 }
+// The wait in the same statement: nothing may use the registers before it.
 __device__ __forceinline__ void tm_ld16(uint32_t t, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(t));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      : "r"(t) : "memory");
 }
 __device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -280,6 +281,12 @@ struct Walk {
   __device__ int row0() const { return begin + chunk * kQ; }
   __device__ int valid() const { return min(kQ, len - chunk * kQ); }
 };
+
+// The passes are launched with programmatic serialisation: each lets the next
+// one start as its own CTAs leave, and waits for the one before (and so for all
+// before that) ahead of its first read.
+__device__ __forceinline__ void pass_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pass_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Heads of a pair; an odd group's last pair has its head twice.
 struct Heads {
@@ -373,6 +380,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
 
+  pass_next();
+  pass_wait();
   if (warp == 0) {
     if (lane == 0) {
       const int4* pl = reinterpret_cast<const int4*>(a.plan + (WHOLE ? kMaxCtas : 0) + cta);
@@ -892,6 +901,7 @@ __device__ __noinline__ void scan_plan(const ChunkArgs& a, int c, int ctas) {
 
 __global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a, int ctas) {
   const int lane = threadIdx.x & 31, chunk = blockIdx.x;
+  pass_next();
   if (blockIdx.y == gridDim.y - 1) {  // the last row of blocks: pieces
     const int c = blockIdx.x * (kStepThreads / 32) + (threadIdx.x >> 5);
     if (c < ctas) scan_plan(a, c, ctas);
@@ -971,6 +981,8 @@ constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(ChunkArgs a, int ctas) {
   __shared__ int list[kMaxCtas], count[kJoinThreads / 32];
   const int pair = blockIdx.y, tid = threadIdx.x, size = 2 * kP * a.n;
+  pass_next();
+  pass_wait();
   // this pair's pieces, in order
   const int m = tid < ctas ? a.meta[tid] : 0;
   const bool mine = (m & 3) && (m >> 2) == pair;
@@ -1111,9 +1123,23 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   scan_steps_kernel<<<dim3(chunks > plans ? (unsigned)chunks : plans,
                            (2 * a.pairs + kStepThreads / 32 - 1) / (kStepThreads / 32) + 1),
                       kStepThreads, 0, stream>>>(a, ctas);
-  pass1<<<ctas, kChThreads, smem1, stream>>>(xm, bm, cm, a);
-  scan_join_kernel<<<dim3((2 * kP * N / 4 + kJoinThreads - 1) / kJoinThreads, a.pairs), kJoinThreads, 0, stream>>>(a, ctas);
-  pass3<<<ctas, kChThreads, smem3, stream>>>(xm, bm, cm, a);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t chunk{}, join{};
+  chunk.gridDim = dim3((unsigned)ctas);
+  chunk.blockDim = dim3(kChThreads);
+  chunk.dynamicSmemBytes = smem1;
+  join.gridDim = dim3((2 * kP * N / 4 + kJoinThreads - 1) / kJoinThreads, a.pairs);
+  join.blockDim = dim3(kJoinThreads);
+  chunk.stream = join.stream = stream;
+  chunk.attrs = join.attrs = &attr;
+  chunk.numAttrs = join.numAttrs = 1;
+  if (cudaLaunchKernelEx(&chunk, pass1, xm, bm, cm, a) != cudaSuccess ||
+      cudaLaunchKernelEx(&join, scan_join_kernel, a, ctas) != cudaSuccess)
+    return kErrLaunch;
+  chunk.dynamicSmemBytes = smem3;
+  if (cudaLaunchKernelEx(&chunk, pass3, xm, bm, cm, a) != cudaSuccess) return kErrLaunch;
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
