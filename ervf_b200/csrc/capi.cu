@@ -1220,7 +1220,7 @@ int ervf_ssm_token(const void* xbc, long long xbc_stride, const void* dt, long l
     return kErrNull;
   if (seqs < 0 || n_slots < 0 || heads <= 0 || groups <= 0 || heads % groups || head_dim <= 0 ||
       head_dim > kMaxHeadDim || d_state <= 0 || d_state > kMaxDState || d_state % 4 || width < 2 ||
-      width > kMaxConvWidth)
+      width > kMaxConvWidth || (long long)(heads / groups) * head_dim > kMaxGroupChannels)
     return kErrShape;
   const long long inner = (long long)heads * head_dim, ch = inner + 2LL * groups * d_state;
   if (xbc_stride < ch || dt_stride < heads || (z && z_stride < inner) || out_stride < inner) return kErrShape;

@@ -631,13 +631,19 @@ int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
   // batch of 96 with eight groups takes 117 us with eight CTAs a group, 93 with
   // four, 86 with two and 97 with one (each convolves B and C for itself); one
   // sequence's latency is least with eight
+  const size_t elem = a.type == kTypeBF16 ? 2 : 4;
+  auto smem_of = [&](int ctas) {
+    const size_t most = (hpg + ctas - 1) / ctas;
+    return (2 * (size_t)a.d_state + 2 * most * a.head_dim + 3 * most + kTokThreads / 32 + 16) * 4 +
+           (kMaxConvWidth - 1) * 2 * a.d_state * elem;
+  };
+  constexpr size_t kMost = 48 * 1024;
   int c = hpg < 8 ? hpg : 8;
-  while (c > 1 && (long long)a.seqs * a.groups * c > 12LL * device_sm_count()) c = (c + 1) / 2;
-  const size_t most = (hpg + c - 1) / c, elem = a.type == kTypeBF16 ? 2 : 4;
-  const size_t smem = (2 * (size_t)a.d_state + 2 * most * a.head_dim + 3 * most + kTokThreads / 32 + 16) * 4 +
-                      (kMaxConvWidth - 1) * 2 * a.d_state * elem;
+  while (c > 1 && (long long)a.seqs * a.groups * c > 12LL * device_sm_count() && smem_of((c + 1) / 2) <= kMost)
+    c = (c + 1) / 2;
+  const size_t smem = smem_of(c);
   const void* fn = a.type == kTypeBF16 ? token_kernel<__nv_bfloat16>(a.d_state) : token_kernel<float>(a.d_state);
-  if (smem > 48 * 1024) return kErrShape;
+  if (smem > kMost) return kErrShape;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.seqs * a.groups * c));
   cfg.blockDim = dim3(kTokThreads);

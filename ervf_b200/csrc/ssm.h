@@ -87,6 +87,6 @@ struct NormArgs {
 int launch_gated_norm(const NormArgs& a, cudaStream_t stream);
 
 // Limits of the scan and convolution kernels.
-constexpr int kMaxHeadDim = 256, kMaxDState = 256, kMaxConvWidth = 4;
+constexpr int kMaxHeadDim = 256, kMaxDState = 256, kMaxConvWidth = 4, kMaxGroupChannels = 32768;
 
 }  // namespace ervf

@@ -210,7 +210,9 @@ class GPUKernels:
         """Selective scan of packed prompts: with d_t = softplus(dt[t][h] + dt_bias[h]),
         S_t = exp(d_t A[h]) S_{t-1} + d_t x[t][h] B[t][g]^T and y[t][h] = S_t C[t][g] +
         D[h] x[t][h].  state f32 [n_slots, heads, head_dim, d_state] or None;
-        cu_seqlens, slots and has_state as in conv1d_prompt.  A is not above 0."""
+        cu_seqlens, slots and has_state as in conv1d_prompt.  A is not above 0.
+        bf16 with head_dim 64 and d_state 64 or 128 runs in chunks on the tensor
+        cores, everything else token by token."""
         code = _type_of(y, dtype, "y")
         inner, bc = heads * head_dim, groups * d_state
         py, sy = self._rows(y, tokens, inner, code, "y")

@@ -584,8 +584,11 @@ ERVF_API int ervf_cache_fetch(const uint8_t* bank_c, const uint8_t* bank_s, uint
  * W bf16 [rows][cols]; x bf16, out and resid of out_type, their rows *_stride
  * elements apart; bias f32.  bias, resid may be NULL; resid may be out
  * itself (then with its stride), x must not overlap out.  Sums and epilogue
- * in f32, one rounding to out_type, the same bits on every call.  cols and
- * x_stride multiples of 8, W and x 16-byte aligned.  tokens = 0 does nothing.
+ * in f32, one rounding to out_type, the same bits on every call; the tensor
+ * core's own sums are off by about 3e-6 (relative, 4096 columns) beyond 128
+ * tokens, a quarter of that up to 128.  cols and x_stride multiples of 8, W and
+ * x 16-byte aligned; any rows and tokens (out rows of 16-byte alignment are
+ * fastest).  tokens = 0 does nothing.
  * The reference projects one token at a time (gpu_kernels.py:21-49). */
 ERVF_API int ervf_linear_bf16(const uint16_t* W, const uint16_t* x, long long x_stride, const float* bias,
                               const void* resid, long long resid_stride, void* out, long long out_stride,
@@ -621,7 +624,13 @@ ERVF_API int ervf_conv1d_prompt(const void* x, long long x_stride, const float* 
  * [n_slots][heads][head_dim][d_state] or NULL.  head_dim and d_state <= 256.
  * scratch: ervf_ssm_prompt_scratch_bytes bytes, 16-byte aligned, need not be
  * cleared; calls that share it must not overlap on the GPU.  y must not
- * overlap an input.  The reference: softplus and ssm, one token at a time. */
+ * overlap an input.
+ * bf16 with head_dim 64, d_state 64 or 128 and rows of x, B, C, y of 16-byte
+ * alignment runs in chunks of 128 tokens on the tensor cores (above 32
+ * tokens); everything else token by token, whose time grows with the longest
+ * sequence.  In chunks a NaN or infinity in x may also reach tokens before it
+ * in its own sequence's chunk (a zero weight times it), never another
+ * sequence.  The reference: softplus and ssm, one token at a time. */
 ERVF_API int ervf_ssm_prompt(const void* x, long long x_stride, const void* dt, long long dt_stride,
                              const float* A, const void* B, long long b_stride, const void* C,
                              long long c_stride, const float* D, const float* dt_bias, float* state, int n_slots,
@@ -641,8 +650,8 @@ ERVF_API size_t ervf_ssm_prompt_scratch_bytes(int type, int tokens, int seqs, in
  * (z NULL: not) and normalised per group of heads * head_dim / groups channels
  * as ervf_gated_norm does (norm_w NULL: not).  Everything between the inputs
  * and the output's one rounding is f32.  slots as above; d_state a multiple
- * of 4, state 16-byte aligned.  out must not overlap an input.  The
- * reference: conv1d, softplus, ssm, gated_rmsnorm (gpu_kernels.py:77-1515). */
+ * of 4, state 16-byte aligned, heads / groups * head_dim <= 32768.  out must not
+ * overlap an input.  The reference: conv1d, softplus, ssm, gated_rmsnorm (gpu_kernels.py:77-1515). */
 ERVF_API int ervf_ssm_token(const void* xbc, long long xbc_stride, const void* dt, long long dt_stride,
                             const void* z, long long z_stride, const float* conv_w, const float* conv_bias,
                             void* conv_state, const float* A, const float* D, const float* dt_bias,

@@ -77,6 +77,7 @@ def test_token():
     assert token(x=None) == token(dt=None) == token(cw=None) == token(cst=None) == token(A=None) == _lib.ERR_NULL
     assert token(st=None) == token(out=None) == _lib.ERR_NULL
     assert token(h=3, g=2) == token(n=6) == token(n=260) == token(k=1) == token(k=5) == token(p=300) == _lib.ERR_SHAPE
+    assert token(h=129, p=256, xs=40000, os=40000, ds=200) == _lib.ERR_SHAPE
     assert token(xs=31) == token(ds=1) == token(os=15) == token(z=P, zs=15) == token(s=-1) == _lib.ERR_SHAPE
     assert token(ty=2) == token(out=P) == token(eps=-1.0) == token(eps=float("nan")) == _lib.ERR_ARG
     assert token(st=P + 4) == token(x=P + 2) == token(sl=P + 2) == _lib.ERR_ALIGN

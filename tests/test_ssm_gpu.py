@@ -377,7 +377,7 @@ def check_token(c, dtype, got, z=True, norm=True, extras=True):
 
 @pytest.mark.parametrize("seqs,heads,head_dim,groups,d_state,width", [
     (1, 1, 1, 1, 4, 2), (1, 8, 64, 1, 128, 4), (3, 6, 64, 2, 128, 4), (5, 9, 33, 1, 64, 3), (2, 16, 64, 2, 96, 4),
-    (4, 11, 64, 1, 128, 4), (2, 20, 32, 1, 256, 4), (7, 3, 256, 3, 16, 2), (33, 8, 64, 8, 128, 4)])
+    (4, 11, 64, 1, 128, 4), (2, 20, 32, 1, 256, 4), (7, 3, 256, 3, 16, 2), (33, 8, 64, 8, 128, 4), (230, 64, 256, 1, 4, 2), (200, 16, 64, 8, 128, 4)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_token(k, cuda, seqs, heads, head_dim, groups, d_state, width, dtype):
     c = token_case(seqs, heads, head_dim, groups, d_state, width, dtype, seed=seqs)
