@@ -369,22 +369,21 @@ __global__ void __launch_bounds__(kTokThreads, 4) ssm_token_kernel(TokenArgs a) 
   const int sub = tid / L, n0 = (tid % L) * 4;
   const int batches = (P + kBatch - 1) / kBatch, rounds = mine * batches;
   float4 next[kRows][NV];
-  auto state_of = [&](int k) {
-    return a.state + ((size_t)slot * a.heads + grp * hpg + r + k * c) * P * N;
+  // this lane's first element of head k's state from row p0, where there is a slot
+  auto state_at = [&](int k, int p0) {
+    return a.state + (((size_t)max(slot, 0) * a.heads + grp * hpg + r + k * c) * P + p0 + sub) * N + n0;
   };
-  // rows p0 + sub, p0 + sub + kStep, ... of the head's state of round i
-  auto load = [&](int i) {
-    const int k = i / batches, p0 = (i - k * batches) * kBatch;
+  // rows p0 + sub, p0 + sub + kStep, ...
+  auto load = [&](const float* st, int p0) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int p = p0 + i * kStep + sub, n = n0 + j * 4 * L;
-        next[i][j] = slot >= 0 && p < P && n < N ? *reinterpret_cast<const float4*>(state_of(k) + (size_t)p * N + n)
-                                                 : make_float4(0, 0, 0, 0);
-      }
+      for (int j = 0; j < NV; ++j)
+        next[i][j] = slot >= 0 && p0 + i * kStep + sub < P && n0 + j * 4 * L < N
+                         ? *reinterpret_cast<const float4*>(st + i * kStep * N + j * 4 * L)
+                         : make_float4(0, 0, 0, 0);
   };
-  load(0);
+  load(state_at(0, 0), 0);
   if (tid >= kTokThreads - 32)
     for (int k = lane; k < mine; k += 32) {
       const int head = grp * hpg + r + k * c;
@@ -417,45 +416,76 @@ __global__ void __launch_bounds__(kTokThreads, 4) ssm_token_kernel(TokenArgs a) 
   }
   cl.barrier_arrive();
   __syncthreads();
+  float4 b[NV], cc[NV];  // this lane's columns of B and C
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int n = n0 + j * 4 * L;
+    b[j] = n < N ? *reinterpret_cast<const float4*>(sBC + n) : make_float4(0, 0, 0, 0);
+    cc[j] = n < N ? *reinterpret_cast<const float4*>(sBC + N + n) : make_float4(0, 0, 0, 0);
+  }
   float ss = 0.0f;
+  int k = 0, p0 = 0;
+  float* st = state_at(0, 0);
   for (int i = 0; i < rounds; ++i) {
-    const int k = i / batches, p0 = (i - k * batches) * kBatch;
     float4 v[kRows][NV];
 #pragma unroll
     for (int q = 0; q < kRows; ++q)
 #pragma unroll
       for (int j = 0; j < NV; ++j) v[q][j] = next[q][j];
-    if (i + 1 < rounds) load(i + 1);
+    int k1 = k, p1 = p0 + kBatch;
+    float* st1 = st + kBatch * N;
+    if (p1 >= P) {
+      ++k1;
+      p1 = 0;
+      st1 = state_at(k1, 0);
+    }
+    if (i + 1 < rounds) load(st1, p1);
     const float d = sh[3 * k], da = sh[3 * k + 1], D = sh[3 * k + 2];
+    float x[kRows], y[kRows];
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
       const int p = p0 + q * kStep + sub;
-      const float x = p < P ? sy[k * P + p] : 0.0f, dx = d * x;
-      float y = 0.0f;
+      x[q] = p < P ? sy[k * P + p] : 0.0f;
+      const float dx = d * x[q];
+      y[q] = 0.0f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int n = n0 + j * 4 * L;
-        if (n < N) {
-          const float4 b = *reinterpret_cast<const float4*>(sBC + n);
-          const float4 cc = *reinterpret_cast<const float4*>(sBC + N + n);
-          float4 e = v[q][j];
-          e.x = fmaf(dx, b.x, da * e.x);
-          e.y = fmaf(dx, b.y, da * e.y);
-          e.z = fmaf(dx, b.z, da * e.z);
-          e.w = fmaf(dx, b.w, da * e.w);
-          if (slot >= 0 && p < P) *reinterpret_cast<float4*>(state_of(k) + (size_t)p * N + n) = e;
-          y += (e.x * cc.x + e.y * cc.y) + (e.z * cc.z + e.w * cc.w);
-        }
-      }
-#pragma unroll
-      for (int o = L / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-      if (n0 == 0 && p < P) {
-        y = fmaf(D, x, y) * sz[k * P + p];
-        ss = fmaf(y, y, ss);
-        sy[k * P + p] = y;  // its x was read by this row's lanes, together
+        float4 e = v[q][j];
+        e.x = fmaf(dx, b[j].x, da * e.x);
+        e.y = fmaf(dx, b[j].y, da * e.y);
+        e.z = fmaf(dx, b[j].z, da * e.z);
+        e.w = fmaf(dx, b[j].w, da * e.w);
+        if (slot >= 0 && p < P && n0 + j * 4 * L < N)
+          *reinterpret_cast<float4*>(st + q * kStep * N + j * 4 * L) = e;
+        y[q] = fmaf(e.x, cc[j].x, fmaf(e.y, cc[j].y, fmaf(e.z, cc[j].z, fmaf(e.w, cc[j].w, y[q]))));
       }
     }
+    // the rows' sums over their L lanes: each halving step leaves a lane half
+    // of the rows, until it has one
+    int off = L / 2, mine_q = 0;
+#pragma unroll
+    for (int rows = kRows; rows > 1; rows >>= 1, off >>= 1) {
+      const bool up = tid & off;
+#pragma unroll
+      for (int q = 0; q < rows / 2; ++q) {
+        const float keep = up ? y[q + rows / 2] : y[q], give = up ? y[q] : y[q + rows / 2];
+        y[q] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+        x[q] = up ? x[q + rows / 2] : x[q];
+      }
+      mine_q += up ? rows / 2 : 0;
+    }
+    for (; off; off >>= 1) y[0] += __shfl_xor_sync(0xffffffffu, y[0], off);
+    const int p = p0 + mine_q * kStep + sub;
+    __syncwarp();  // every x of these rows is read
+    if ((tid & (L / kRows - 1)) == 0 && p < P) {
+      const float g = fmaf(D, x[0], y[0]) * sz[k * P + p];
+      ss = fmaf(g, g, ss);
+      sy[k * P + p] = g;
+    }
     __syncwarp();
+    k = k1;
+    p0 = p1;
+    st = st1;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
