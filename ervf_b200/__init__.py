@@ -4,7 +4,8 @@ The compute lives in ``libervf_b200.so`` (C ABI: ``include/ervf_b200.h``),
 built by ``python -m ervf_b200.build``.  Python front ends:
 
   * ``FusedNVFP4``   -- drop-in for lightningstream_nemotron.fused_nvfp4.FusedNVFP4
-  * ``GPUKernels``   -- ``mv_bf16`` of lightningstream_nemotron.gpu_kernels
+  * ``GPUKernels``   -- ``mv_bf16`` of lightningstream_nemotron.gpu_kernels, the
+    dense projections and the state-space layers of the hybrid
   * ``ExpertBank``   -- HBM-resident expert storage (residency / upload path)
   * ``MoEDecoder``   -- routed-expert MoE layers and decode steps on the C ABI
 """
