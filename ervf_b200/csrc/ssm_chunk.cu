@@ -358,10 +358,14 @@ __device__ __forceinline__ bool scale_x(uint8_t* smem, Barriers& br, int team, i
   return true;
 }
 
+// A warpgroup's share: inc below the launch's count, or dec above it, is an
+// illegal instruction.
 template <int R>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
-template <int R>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+__device__ __forceinline__ void regs_to() {
+  static_assert(R % 8 == 0 && R >= 24, "setmaxnreg");
+  if constexpr (R > kRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+  if constexpr (R < kRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
 
 template <int N, bool WHOLE>
 __global__ void __launch_bounds__(kChThreads, 1)
@@ -437,7 +441,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
     // Lanes are tokens t; the two warps of a lane quarter share its blocks of
     // 32 tokens s: q, q - 2 for the first, q - 1, q - 3 for the second (of two
     // below the diagonal, the second takes both).
-    regs_up<kRegP>();
+    regs_to<kRegP>();
     if (!WHOLE) {
       for (int it = 0; it < count; ++it)
         if (!scale_x<N, WHOLE>(smem, br, 0, it, dead)) break;
@@ -559,7 +563,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
     }
   } else if (warp < 16) {
     // ------------------------------------------------------------- states
-    regs_up<kRegS>();
+    regs_to<kRegS>();
     const int half = (warp - 8) >> 2;  // state rows 32 q .., columns 32 half ..
     const int n = 32 * q + lane;
     const bool own = n < N;
@@ -668,12 +672,12 @@ __global__ void __launch_bounds__(kChThreads, 1)
     }
   } else if (warp < 24) {
     // ------------------------------------------------------------------ W
-    regs_down<kRegW>();
+    regs_to<kRegW>();
     const int team = WHOLE ? (warp - 16) >> 2 : 1;
     for (int it = 0; it < count; ++it)
       if (!scale_x<N, WHOLE>(smem, br, team, it, dead)) break;
   } else {
-    regs_down<kRegMisc>();
+    regs_to<kRegMisc>();
     if (warp == 24) {
       // --------------------------------------------- TMA of steps, C and B
       if (lane == 0) {
