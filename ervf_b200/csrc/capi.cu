@@ -1146,6 +1146,8 @@ int ervf_linear_bf16(const uint16_t* W, const uint16_t* x, long long x_stride, c
                      int out_type, int rows, int cols, int tokens, int act, void* stream) {
   if (!W || (tokens > 0 && (!x || !out))) return kErrNull;
   if (rows <= 0 || cols <= 0 || tokens < 0 || cols % 8) return kErrShape;
+  // tiles of 256 are counted in 32 bits
+  if (rows > 0x7fffff00 || cols > 0x7fffff00 || tokens > 0x7fffff00) return kErrShape;
   if (x_stride < cols || out_stride < rows || (resid && resid_stride < rows)) return kErrShape;
   if (!type_ok(out_type) || act < kActNone || act > kActGelu) return kErrArg;
   if (tokens > 0 && (out == x || (resid == out && resid_stride != out_stride))) return kErrArg;

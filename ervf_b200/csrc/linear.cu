@@ -21,8 +21,11 @@
 //     k-block's four MMAs has an accumulator of its own, added in the epilogue:
 //     the tensor core's sums lose a little with every step (rel. 3e-6 over 4096
 //     columns in one chain).
-//   few tiles: the k-blocks of a tile are dealt to a cluster of CTAs, whose
-//     sums meet in shared memory and are added in rank order.
+//   more tokens than 64: 128 x 128 or 128 x 256 tiles.  Where these are fewer
+//     than the SMs, a tile's k-blocks are dealt to a cluster of CTAs, whose sums
+//     meet in shared memory and are added in rank order.  Bound by what L2
+//     delivers to an SM (about 50 bytes a clock) and a start and end of 5 us
+//     (128 x 1024 x 64: 5.4 us).
 //   many tokens: a pair of CTAs computes a 256 x 256 tile (cta_group::2); each
 //     holds its 128 rows of x and half of W's.  Bound by the tensor cores and
 //     by what L2 delivers: 64 bytes a clock and SM at full rate, where a single
@@ -86,15 +89,18 @@ __device__ __forceinline__ uint64_t lin_desc(uint32_t saddr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-__device__ __forceinline__ void lin_tma(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+__device__ __forceinline__ void lin_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void lin_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n}"
+               ::"r"(bar), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ void lin_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void lin_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // The wait in the same statement: nothing may use the registers before it.
@@ -108,10 +114,14 @@ __device__ __forceinline__ void lin_ld16(uint32_t taddr, uint32_t (&v)[16]) {
 }
 
 // Bounded wait that also gives up when another role of the CTA died.
-__device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-  if (mbar_try_wait(bar, parity)) return true;
+__device__ __noinline__ bool lin_wait_slow(uint32_t bar, uint32_t parity, volatile int* dead) {
   const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
     if (*dead) return false;
     if (clock64() - t0 > 2000000000LL) {
       atomicExch(&g_device_error, kErrTimeout);
@@ -119,8 +129,32 @@ __device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, volatil
       return false;
     }
   }
-  return true;
 }
+__device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok || lin_wait_slow(bar, parity, dead);
+}
+__device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  return lin_wait(smem_u32(bar), parity, dead);
+}
+
+// A place in a ring of N stages: the producer's and the issuing thread's loops
+// are one thread's, so their few instructions a k-block are what a k-block
+// costs at least.
+template <int N>
+struct Ring {
+  uint32_t s = 0, parity;
+  __device__ explicit Ring(uint32_t p) : parity(p) {}
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      parity ^= 1;
+    }
+  }
+};
 
 // One branch for all N values.
 template <int N>
@@ -242,6 +276,14 @@ __device__ __forceinline__ float lin_remote(const float* p, int rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 lin_remote4(const float* p, int rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -293,57 +335,60 @@ __global__ void __launch_bounds__(kLinThreads, 1)
   const int step = SPLIT ? units : (int)gridDim.x;
   const int kb0 = SPLIT ? a.nkb * rank / a.splits : 0, kb1 = SPLIT ? a.nkb * (rank + 1) / a.splits : a.nkb;
 
+  const uint32_t ring_at = smem_u32(ring), full_at = smem_u32(full), empty_at = smem_u32(empty);
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t gk = 0;
+      Ring<Sh::kStages> r(1);
+      uint32_t loads = 0;
       for (int u = u0; u < units && !*dead; u += step) {
-        const int mt = u % a.mtiles, nt = u / a.mtiles;
-        for (int kb = kb0; kb < kb1; ++kb, ++gk) {
-          const int s = (int)(gk % Sh::kStages);
-          if (!lin_wait(&empty[s], ((gk / Sh::kStages) & 1) ^ 1, dead)) break;
-          mbar_arrive_expect_tx(&full[s], Sh::kStage);
-          uint8_t* st = ring + s * Sh::kStage;
-          lin_tma(st, &a_map, kb * kLinKB, mt * kLinM, &full[s]);
-          lin_tma(st + kLinATile, &b_map, kb * kLinKB, nt * BN, &full[s]);
+        const int my = u % a.mtiles * kLinM, ny = u / a.mtiles * BN;
+#pragma unroll 1
+        for (int kb = kb0; kb < kb1; ++kb, r.next(), ++loads) {
+          if (!lin_wait(empty_at + 8 * r.s, r.parity, dead)) break;
+          const uint32_t bar = full_at + 8 * r.s, st = ring_at + r.s * Sh::kStage;
+          lin_expect(bar, Sh::kStage);
+          lin_tma(st, &a_map, kb * kLinKB, my, bar);
+          lin_tma(st + kLinATile, &b_map, kb * kLinKB, ny, bar);
         }
       }
       // leave no tensor copy in flight
-      for (uint32_t k = gk > (uint32_t)Sh::kStages ? gk - Sh::kStages : 0; k < gk; ++k)
-        lin_wait(&full[k % Sh::kStages], (k / Sh::kStages) & 1, dead);
+      for (uint32_t k = loads > (uint32_t)Sh::kStages ? loads - Sh::kStages : 0; k < loads; ++k)
+        lin_wait(full_at + 8 * (k % Sh::kStages), (k / Sh::kStages) & 1, dead);
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      uint32_t gk = 0;
+      Ring<Sh::kStages> r(0);
+      const uint64_t da0 = lin_desc(ring_at), db0 = lin_desc(ring_at + kLinATile);
       int nu = 0;
       for (int u = u0; u < units && !*dead; u += step, ++nu) {
         const int d = nu & 1;
         if (!lin_wait(&dempty[d], ((nu >> 1) & 1) ^ 1, dead)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb, ++gk) {
-          const int s = (int)(gk % Sh::kStages);
-          if (!lin_wait(&full[s], (gk / Sh::kStages) & 1, dead)) {
+#pragma unroll 1
+        for (int kb = kb0; kb < kb1; ++kb, r.next()) {
+          if (!lin_wait(full_at + 8 * r.s, r.parity, dead)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t st = smem_u32(ring + s * Sh::kStage);
+          const uint64_t da = da0 + r.s * (Sh::kStage >> 4), db = db0 + r.s * (Sh::kStage >> 4);
 #pragma unroll
           for (int j = 0; j < kLinKB / 16; ++j) {
             const uint32_t acc = kb > kb0 || j >= CH ? 1u : 0u;
             asm volatile(
                 "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                ::"r"(tmem + (uint32_t)((d * CH + j % CH) * BN)), "l"(lin_desc(st + 32 * j)),
-                  "l"(lin_desc(st + kLinATile + 32 * j)), "r"(idesc), "r"(acc) : "memory");
+                ::"r"(tmem + (uint32_t)((d * CH + j % CH) * BN)), "l"(da + 2 * j), "l"(db + 2 * j), "r"(idesc),
+                  "r"(acc) : "memory");
           }
-          lin_commit(&empty[s]);
+          lin_commit(empty_at + 8 * r.s);
         }
         if (!ok) break;
-        lin_commit(&dfull[d]);
+        lin_commit(smem_u32(&dfull[d]));
       }
       // every MMA is complete before tensor memory is freed
-      lin_commit(mma_done);
+      lin_commit(smem_u32(mma_done));
       mbar_wait(mma_done, 0, 2000000000LL);
     }
   } else {
@@ -381,10 +426,15 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         float f[16];
         sums(d, c, f);
         if constexpr (SPLIT) {
-          // all MMAs are done: the ring holds the sums, [column][row]
-          float* part = reinterpret_cast<float*>(ring) + (size_t)c * kLinM + 32 * q + lane;
+          // all MMAs are done: the ring holds the sums, [column][row], or four
+          // columns of a row together
+          float* part = reinterpret_cast<float*>(ring) + (size_t)c * kLinM;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[i * kLinM] = f[i];
+          for (int i = 0; i < 16; ++i) {
+            if constexpr (SWAP) part[i * kLinM + 32 * q + lane] = f[i];
+            else if (i % 4 == 0)
+              *reinterpret_cast<float4*>(part + i * kLinM + 4 * (32 * q + lane)) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+          }
         } else if constexpr (SWAP) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] += bias;
@@ -412,7 +462,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       const int q = warp & 3, mt = u0 % a.mtiles, nt = u0 / a.mtiles, m = mt * kLinM + 32 * q + lane;
       const int who = rank + a.splits * ((warp - 2) / 4), all = a.splits * (kLinEpi / 4);
       float* stage = reinterpret_cast<float*>(ring + Sh::kStages * Sh::kStage) + (warp - 2) * (kLinStage / 4);
-      const float* part = reinterpret_cast<const float*>(ring) + 32 * q + lane;
+      const float* part = reinterpret_cast<const float*>(ring) + (SWAP ? 1 : 4) * (32 * q + lane);
       if constexpr (SWAP) {
         const int cols = min(BN, a.tokens - nt * BN);
         const float bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
@@ -433,13 +483,15 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           float f[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] = 0.0f;
-#pragma unroll 2
+#pragma unroll 4
           for (int r = 0; r < a.splits; ++r) {
-            float v[16];
+            float4 v[4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = lin_remote(part + (size_t)(c + i) * kLinM, r);
+            for (int i = 0; i < 4; ++i) v[i] = lin_remote4(part + (size_t)(c + 4 * i) * kLinM, r);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] += v[i];
+            for (int i = 0; i < 4; ++i) {
+              f[4 * i] += v[i].x; f[4 * i + 1] += v[i].y; f[4 * i + 2] += v[i].z; f[4 * i + 3] += v[i].w;
+            }
           }
           pre.store(a, m - lane, nt * BN + c, f, stage);
         }
@@ -456,17 +508,14 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
 // ------------------------------------------------------- a pair of CTAs
 
-// One 256 x BN tile by two CTAs: each loads its 128 rows of x and half of the
-// tile's BN rows of W; the even one issues the MMAs of both.
+// One 256 x 256 tile by two CTAs: each loads its 128 rows of x and half of the
+// tile's 256 rows of W; the even one issues the MMAs of both.
 // Sixteen epilogue warps: with eight, a tile's epilogue took 4.1 us (4096 x 4096,
 // 64 columns), longer than its MMAs below 700 columns.
 constexpr int kPairEpi = 16, kPairThreads = (2 + kPairEpi) * 32;
 constexpr int kPairTile = 128 * kLinKB * 2;  // x's part in one CTA
-template <int BN>
-struct PairShape {
-  static constexpr int kStage = kPairTile + BN / 2 * kLinKB * 2, kStages = BN == 256 ? 5 : 7;
-  static constexpr int kSmem = 2048 + kStages * kStage + kPairEpi * kLinStage;
-};
+constexpr int kPairStage = kPairTile + 128 * kLinKB * 2, kPairStages = 5;
+constexpr int kPairSmem = 2048 + kPairStages * kPairStage + kPairEpi * kLinStage;
 
 __device__ __forceinline__ uint32_t lead_addr(const void* p) {
   uint32_t at;
@@ -474,22 +523,22 @@ __device__ __forceinline__ uint32_t lead_addr(const void* p) {
   return at;
 }
 // This GPU's own memory only, into this CTA; the bytes count at the even CTA's barrier.
-__device__ __forceinline__ void pair_tma(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void pair_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3}], [%4];" ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+      "%3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 // Arrives at the same barrier of both CTAs.
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+      ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-template <int BN, typename T>
+template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, LinTile a) {
-  constexpr int kPairStages = PairShape<BN>::kStages, kPairStage = PairShape<BN>::kStage;
+  constexpr int BN = 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);  // counted at the even CTA
@@ -529,25 +578,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int units = a.mtiles * a.ntiles, u0 = blockIdx.x >> 1, step = gridDim.x >> 1;
 
+  const uint32_t ring_at = smem_u32(ring), full_at = smem_u32(full), empty_at = smem_u32(empty);
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t gk = 0;
+      Ring<kPairStages> r(1);
+      const uint32_t lead_full = lead_addr(full);
+      uint32_t loads = 0;
       for (int u = u0; u < units && !*dead; u += step) {
         int mt, nt;
         lin_place(a, u, mt, nt);
-        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
-          const int s = (int)(gk % kPairStages);
-          if (!lin_wait(&empty[s], ((gk / kPairStages) & 1) ^ 1, dead)) break;
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStage);
-          const uint32_t bar = lead_addr(&full[s]);
-          uint8_t* st = ring + s * kPairStage;
-          pair_tma(st, &x_map, kb * kLinKB, (2 * mt + rank) * 128, bar);
-          pair_tma(st + kPairTile, &w_map, kb * kLinKB, nt * BN + rank * (BN / 2), bar);
+        const int my = (2 * mt + rank) * 128, ny = nt * BN + rank * (BN / 2);
+#pragma unroll 1
+        for (int kb = 0; kb < a.nkb; ++kb, r.next(), ++loads) {
+          if (!lin_wait(empty_at + 8 * r.s, r.parity, dead)) break;
+          if (rank == 0) lin_expect(full_at + 8 * r.s, 2 * kPairStage);
+          const uint32_t bar = lead_full + 8 * r.s, st = ring_at + r.s * kPairStage;
+          pair_tma(st, &x_map, kb * kLinKB, my, bar);
+          pair_tma(st + kPairTile, &w_map, kb * kLinKB, ny, bar);
         }
       }
       // leave no tensor copy in flight: each stage's release follows its arrival
-      for (uint32_t k = gk > (uint32_t)kPairStages ? gk - kPairStages : 0; k < gk; ++k)
-        lin_wait(&empty[k % kPairStages], (k / kPairStages) & 1, dead);
+      for (uint32_t k = loads > (uint32_t)kPairStages ? loads - kPairStages : 0; k < loads; ++k)
+        lin_wait(empty_at + 8 * (k % kPairStages), (k / kPairStages) & 1, dead);
       if (*dead) {
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000) {
@@ -556,33 +608,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      uint32_t gk = 0;
+      Ring<kPairStages> r(0);
+      const uint64_t da0 = lin_desc(ring_at), db0 = lin_desc(ring_at + kPairTile);
       int nu = 0;
       for (int u = u0; u < units && !*dead; u += step, ++nu) {
         const int d = nu & 1;
         if (!lin_wait(&dempty[d], ((nu >> 1) & 1) ^ 1, dead)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool ok = true;
-        for (int kb = 0; kb < a.nkb; ++kb, ++gk) {
-          const int s = (int)(gk % kPairStages);
-          if (!lin_wait(&full[s], (gk / kPairStages) & 1, dead)) {
+#pragma unroll 1
+        for (int kb = 0; kb < a.nkb; ++kb, r.next()) {
+          if (!lin_wait(full_at + 8 * r.s, r.parity, dead)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t st = smem_u32(ring + s * kPairStage);
+          const uint64_t da = da0 + r.s * (kPairStage >> 4), db = db0 + r.s * (kPairStage >> 4);
 #pragma unroll
           for (int j = 0; j < kLinKB / 16; ++j) {
             asm volatile(
                 "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                 " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
-                ::"r"(tmem + (uint32_t)(d * BN)), "l"(lin_desc(st + 32 * j)),
-                  "l"(lin_desc(st + kPairTile + 32 * j)), "r"(idesc), "r"((uint32_t)(kb | j)) : "memory");
+                ::"r"(tmem + (uint32_t)(d * BN)), "l"(da + 2 * j), "l"(db + 2 * j), "r"(idesc), "r"((uint32_t)(kb | j))
+                : "memory");
           }
-          pair_commit(&empty[s]);
+          pair_commit(empty_at + 8 * r.s);
         }
         if (!ok) break;
-        pair_commit(&dfull[d]);
+        pair_commit(smem_u32(&dfull[d]));
       }
       // every MMA is complete before tensor memory is freed
       asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];"
@@ -689,7 +742,7 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
     return kErrLaunch;
   const long long units = (long long)a.mtiles * a.ntiles;
-  if (units > 0x7fffffffLL) return kErrShape;
+  if (units > 0x3fffffffLL) return kErrShape;
   const int sms = device_sm_count();
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(SPLIT ? units * splits : units < sms ? units : sms));
@@ -705,19 +758,18 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, fn, SWAP ? wm : xm, SWAP ? xm : wm, a) == cudaSuccess ? kOk : kErrLaunch;
 }
 
-template <int BN, typename T>
+template <typename T>
 int linear_pair(const LinearArgs& l, cudaStream_t stream) {
-  constexpr int kPairSmem = PairShape<BN>::kSmem;
   LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, 1, lin_vec(l)};
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   a.mtiles = (l.tokens + 255) / 256;
-  a.ntiles = (l.rows + BN - 1) / BN;
+  a.ntiles = (l.rows + 255) / 256;
   const long long units = (long long)a.mtiles * a.ntiles;
   if (units > 0x3fffffffLL) return kErrShape;
   CUtensorMap wm, xm;
-  if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, BN / 2)) return e;
+  if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, 128)) return e;
   if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, 128)) return e;
-  auto fn = linear_pair_kernel<BN, T>;
+  auto fn = linear_pair_kernel<T>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess)
     return kErrLaunch;
   const int pairs = device_sm_count() / 2;
@@ -776,11 +828,28 @@ int linear_single(const LinearArgs& l, cudaStream_t stream) {
 template <typename T>
 int linear_pick(const LinearArgs& l, cudaStream_t stream) {
   if (l.tokens <= 32) return linear_single<32, 4, true, T>(l, stream);
-  if (l.tokens <= 128) return linear_single<64, 4, true, T>(l, stream);
-  const long long mt = ((long long)l.tokens + 255) / 256, sms = device_sm_count();
-  if (4 * mt * ((l.rows + 255LL) / 256) >= 3 * sms) return linear_pair<256, T>(l, stream);
-  if (4 * mt * ((l.rows + 127LL) / 128) >= sms) return linear_pair<128, T>(l, stream);
-  return linear_single<256, 1, false, T>(l, stream);
+  if (l.tokens <= 64) return linear_single<64, 4, true, T>(l, stream);
+  // Three tiles, by their time in units of 10 ns: a start and an epilogue, the
+  // k-blocks that one CTA (pair) goes through, and a split's sums through the
+  // cluster.  Measured with W in L2, tokens x features x columns, for 128 x 128,
+  // 128 x 256 and pairs' 256 x 256:
+  //   128 x 3712 x 2688    10.2   15.4   19.7 us
+  //   512 x 2688 x 5376    29.6   21.4   33.2
+  //   1024 x 1024 x 2048   11.8   13.2   16.9
+  //   1024 x 3712 x 2688   30.7   23.3   21.5
+  //   2048 x 2688 x 5376   78.9   69.6   60.9
+  // Pairs of 256 x 128 were within 5% of the best of these at best.
+  const long long sms = device_sm_count(), nkb = (l.cols + kLinKB - 1) / kLinKB;
+  const long long t128 = (l.tokens + 127LL) / 128, t256 = (l.tokens + 255LL) / 256;
+  const long long r128 = (l.rows + 127LL) / 128, r256 = (l.rows + 255LL) / 256;
+  const auto cost = [&](long long units, int kblock, int sums) {
+    const int s = linear_splits(units, l.cols);
+    return 600 + (units + sms - 1) / sms * ((nkb + s - 1) / s) * kblock + (s > 1 ? sums : 0);
+  };
+  const long long small = cost(t128 * r128, 28, 200), single = cost(t128 * r256, 48, 400);
+  const long long pairs = 900 + (t256 * r256 + sms / 2 - 1) / (sms / 2) * nkb * 33;
+  if (pairs <= small && pairs <= single) return linear_pair<T>(l, stream);
+  return small <= single ? linear_single<128, 2, false, T>(l, stream) : linear_single<256, 1, false, T>(l, stream);
 }
 
 }  // namespace

@@ -27,6 +27,13 @@ def test_linear():
     assert linear(t=0, x=None, out=None) == _lib.OK
 
 
+def test_linear_sizes_that_tiles_cannot_count():
+    most, over = 0x7fffff00, 0x7fffff01
+    big = dict(xs=2 ** 31, os=2 ** 31)
+    assert linear(rows=over, **big) == linear(t=over, **big) == linear(cols=0x7ffffff8, **big) == _lib.ERR_SHAPE
+    assert linear(rows=most, t=0, **big) == _lib.OK
+
+
 def conv(x=P, xs=8, w=P, b=None, st=None, ns=0, sl=None, has=None, cu=P, s=1, out=Q, os=8, ty=0, t=4, ch=8, k=4, silu=1):
     return _lib.load().ervf_conv1d_prompt(x, xs, w, b, st, ns, sl, has, cu, s, out, os, ty, t, ch, k, silu, None)
 

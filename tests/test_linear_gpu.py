@@ -55,6 +55,20 @@ def test_linear(k, cuda, rows, cols, tokens, dtype):
     ref.within(out, want, bound(want, size, cols, dtype))
 
 
+@pytest.mark.parametrize("rows,cols,tokens", [
+    (2688, 4096, 100), (1111, 2056, 129),        # 128 x 128, a tile's columns shared
+    (2600, 2200, 401), (8000, 200, 300),         # 128 x 256, shared and not
+    (3700, 1400, 1000), (5000, 1400, 3001)])     # pairs, one and several tiles each
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiles(k, cuda, rows, cols, tokens, dtype):
+    W, x, b, r = make(rows, cols, tokens, dtype, True, True, seed=6)
+    out = torch.full((tokens, rows), float("nan"), dtype=dtype, device=cuda)
+    k.linear_bf16(out, put(W, cuda), put(x, cuda), rows, cols, tokens, bias=put(b, cuda), act="relu2",
+                  resid=put(r, cuda))
+    want, size = ref.linear(W, x, b, "relu2", r)
+    ref.within(out, want, bound(want, size, cols, dtype))
+
+
 @pytest.mark.parametrize("act", ["none", "relu2", "silu", "gelu"])
 @pytest.mark.parametrize("bias,resid", [(False, False), (True, False), (False, True)])
 @pytest.mark.parametrize("tokens", [3, 140])
