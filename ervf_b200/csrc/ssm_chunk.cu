@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
 
-  pass_next();
+  if (!WHOLE) pass_next();  // what follows pass 3 is not ours
   pass_wait();
   if (warp == 0) {
     if (lane == 0) {
@@ -934,7 +934,9 @@ __global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a, i
   for (int i = 0; i < 4; ++i) {
     const int t = 4 * lane + i;
     d[i] = t < valid ? softplus(__bfloat162float(a.dt[(size_t)(row + t) * a.dt_stride + head]) + bias) : 0.0f;
-    e[i] = d[i] * A2;
+    // exp2(-150) is 0 as every power below it; sums that held a longer step
+    // would lose the distances between the tokens behind it (a NaN stays one)
+    e[i] = d[i] * A2 < -150.0f ? -150.0f : d[i] * A2;
   }
   const float own = (e[0] + e[1]) + (e[2] + e[3]);
   float pre = own, post = own;

@@ -207,6 +207,15 @@ def test_scan_large_steps(k, cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scan_steps_that_forget_everything(k, cuda, dtype):
+    """A few steps of 30000 among ordinary ones: the exponents behind them keep their precision."""
+    c = scan_case([200, 140], 4, 64, 2, 128, dtype, seed=8)
+    c["dt"][7::40] = 30000.0
+    y, st, want = run_scan(k, cuda, c, dtype)
+    check_scan(y, st, want, c, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_scan_no_decay(k, cuda, dtype):
     c = scan_case([200], 2, 64, 1, 128, dtype, seed=6)
     c["A"] *= 0
