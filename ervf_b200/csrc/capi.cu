@@ -1134,7 +1134,7 @@ inline bool type_ok(int t) { return t == kTypeF32 || t == kTypeBF16; }
 inline uintptr_t elem(int t) { return t == kTypeBF16 ? 2 : 4; }
 
 int check_packing(const int32_t* cu, int seqs, int n_slots) {
-  if (seqs < 0 || n_slots < 0) return kErrShape;
+  if (seqs < 0 || seqs > kMaxSeqs || n_slots < 0) return kErrShape;
   if (!cu && seqs != 1) return kErrArg;
   return kOk;
 }
@@ -1164,7 +1164,7 @@ int ervf_conv1d_prompt(const void* x, long long x_stride, const float* w, const 
                        int seqs, void* out, long long out_stride, int type, int tokens, int channels, int width,
                        int silu, void* stream) {
   if (!w || (tokens > 0 && (!x || !out))) return kErrNull;
-  if (tokens < 0 || channels <= 0 || width < 2 || width > kMaxConvWidth) return kErrShape;
+  if (tokens < 0 || channels <= 0 || channels > kMaxConvChannels || width < 2 || width > kMaxConvWidth) return kErrShape;
   if (x_stride < channels || out_stride < channels) return kErrShape;
   if (int e = check_packing(cu_seqlens, seqs, n_slots)) return e;
   if (!type_ok(type) || silu < 0 || silu > 1 || (tokens > 0 && out == x)) return kErrArg;
@@ -1225,6 +1225,7 @@ int ervf_ssm_token(const void* xbc, long long xbc_stride, const void* dt, long l
       width > kMaxConvWidth || (long long)(heads / groups) * head_dim > kMaxGroupChannels)
     return kErrShape;
   const long long inner = (long long)heads * head_dim, ch = inner + 2LL * groups * d_state;
+  if (ch > 0x7fffffffLL || (long long)seqs * groups * 8 > 0x7fffffffLL) return kErrShape;
   if (xbc_stride < ch || dt_stride < heads || (z && z_stride < inner) || out_stride < inner) return kErrShape;
   if (!type_ok(type) || (seqs > 0 && (out == xbc || out == dt || out == z)) || !(eps >= 0.0f)) return kErrArg;
   const uintptr_t b = elem(type);
@@ -1243,7 +1244,7 @@ int ervf_gated_norm(const void* y, long long y_stride, const void* z, long long 
                     float eps, void* out, long long out_stride, int type, int tokens, int groups, int group_size,
                     void* stream) {
   if (!w || (tokens > 0 && (!y || !out))) return kErrNull;
-  if (tokens < 0 || groups <= 0 || group_size <= 0) return kErrShape;
+  if (tokens < 0 || groups <= 0 || group_size <= 0 || group_size > 0x7fffff00) return kErrShape;
   const long long n = (long long)groups * group_size;
   if (y_stride < n || (z && z_stride < n) || out_stride < n || (long long)tokens * groups > 0x7fffffffLL)
     return kErrShape;

@@ -88,5 +88,7 @@ int launch_gated_norm(const NormArgs& a, cudaStream_t stream);
 
 // Limits of the scan and convolution kernels.
 constexpr int kMaxHeadDim = 256, kMaxDState = 256, kMaxConvWidth = 4, kMaxGroupChannels = 32768;
+constexpr int kMaxConvChannels = 65535 * 128;  // a grid's second dimension, a thread a channel
+constexpr int kMaxSeqs = 1 << 26;              // with the most tokens' chunks, a grid's first
 
 }  // namespace ervf

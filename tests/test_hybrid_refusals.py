@@ -103,6 +103,14 @@ def test_norm():
     assert norm(t=0, y=None, out=None) == _lib.OK
 
 
+def test_sizes_that_a_grid_or_an_index_cannot_hold():
+    wide = 2 ** 33
+    assert conv(ch=65535 * 128 + 1, xs=wide, os=wide) == conv(s=2 ** 27) == scan(s=2 ** 27) == _lib.ERR_SHAPE
+    assert token(h=2 ** 24, g=2 ** 24, p=256, xs=wide, os=wide, ds=2 ** 24) == _lib.ERR_SHAPE
+    assert token(s=2 ** 20, h=2 ** 9, g=2 ** 9, p=1, xs=wide, os=wide, ds=2 ** 9) == _lib.ERR_SHAPE
+    assert norm(g=1, n=0x7fffff01, ys=wide, os=wide) == _lib.ERR_SHAPE
+
+
 @pytest.fixture()
 def k():
     return GPUKernels(device="cuda:0")
