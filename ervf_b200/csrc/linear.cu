@@ -48,7 +48,8 @@ namespace {
 constexpr int kLinM = 128, kLinKB = 64;
 constexpr int kLinEpi = 8, kLinThreads = (2 + kLinEpi) * 32;
 constexpr int kLinATile = kLinM * kLinKB * 2;
-constexpr int kLinPitch = 20, kLinStage = 32 * kLinPitch * 4;  // an epilogue warp's staging, bytes
+constexpr int kLinStage = 4096, kLinPitch = 20;  // an epilogue warp's staging, bytes; its row in lin_ragged, floats
+constexpr int kLinPart = 32 * 32 * 4;            // a part of a tile's sums, 32 x 32
 
 template <int BN, int CH>
 struct LinShape {
@@ -59,7 +60,8 @@ struct LinShape {
   static constexpr int kTmemCols = 2 * CH * BN;  // buffer d, chain c at columns (d CH + c) BN
   static_assert(BN % 16 == 0 && BN <= 256 && kTmemCols >= 32 && kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0,
                 "tile");
-  static_assert(BN * kLinM * 4 <= kStages * kStage, "a split's sums fit the ring");
+  // ceil(parts / splits) splits parts, 8 splits at most
+  static_assert((BN / 8 + 7) * kLinPart <= kStages * kStage, "a split's sums fit the ring");
 };
 
 struct LinTile {
@@ -185,82 +187,138 @@ __device__ __forceinline__ void lin_put(T* p, float v) {
   else *p = v;
 }
 
-// 16 features r.. of a warp's tokens t0 .. t0 + 31.  The sums arrive one token a
-// lane and go through shared memory, so that neighbouring lanes write one
-// token's features: whole sectors, where a lane's own row gave 32 half ones an
-// instruction (4096 x 4096 tokens x features of 512 columns: 30 us).  Bias and
-// residual are loaded ahead of the sums.
+// The bias of 32 features from r, a lane's one.
+__device__ __forceinline__ float lin_bias(const LinTile& a, int r) {
+  r += threadIdx.x & 31;
+  return a.bias && r < a.rows ? a.bias[r] : 0.0f;
+}
+
+// The epilogue of 16 features of one token, a lane's; the residual is loaded
+// ahead of the sums.
 template <typename T>
-struct LinRow {
-  static constexpr int V = 16 / sizeof(T), kLanes = 16 / V, kRows = 32 / kLanes, kIters = 32 / kRows;
-  bool whole;
-  float bias[V];
-  uint4 resid[kIters];
-  __device__ __forceinline__ void load(const LinTile& a, int t0, int r) {
-    whole = a.vec && r + 16 <= a.rows;
-    if (!whole) return;
-    const int lane = threadIdx.x & 31, f = r + (lane % kLanes) * V, t = t0 + lane / kLanes;
+struct LinEdge {
+  static constexpr int kWords = 16 * sizeof(T) / 4;
+  uint32_t resid[kWords];
+  __device__ __forceinline__ void load(const LinTile& a, int t, int r) {
+    if (!a.vec) return;
+    const bool whole = r + 16 <= a.rows;
+    if (a.resid && t < a.tokens) {
+      const T* q = static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + r;
+      if (whole) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 b = a.bias ? *reinterpret_cast<const float4*>(a.bias + f + i) : make_float4(0, 0, 0, 0);
-      bias[i] = b.x; bias[i + 1] = b.y; bias[i + 2] = b.z; bias[i + 3] = b.w;
+        for (int i = 0; i < kWords; i += 4) {
+          const uint4 v = reinterpret_cast<const uint4*>(q)[i / 4];
+          resid[i] = v.x; resid[i + 1] = v.y; resid[i + 2] = v.z; resid[i + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          if constexpr (sizeof(T) == 2) {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(q) + 2 * i;
+            resid[i] = (r + 2 * i < a.rows ? h[0] : 0u) | (r + 2 * i + 1 < a.rows ? (uint32_t)h[1] << 16 : 0u);
+          } else {
+            resid[i] = r + i < a.rows ? reinterpret_cast<const uint32_t*>(q)[i] : 0u;
+          }
+        }
+      }
     }
-    const T* q = static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + f;
-#pragma unroll
-    for (int k = 0; k < kIters; ++k)
-      resid[k] = a.resid && t + k * kRows < a.tokens
-                     ? *reinterpret_cast<const uint4*>(q + (size_t)(k * kRows) * a.resid_stride)
-                     : make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void store(const LinTile& a, int t0, int r, const float (&acc)[16], float* stage) const {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
+  // the 16 results, as they lie in memory; their bias from lane 16 h on
+  __device__ __forceinline__ void finish(const LinTile& a, float bias, int h, float (&f)[16],
+                                         uint32_t (&w)[kWords]) const {
+    if (a.bias) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *reinterpret_cast<float4*>(stage + lane * kLinPitch + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-    __syncwarp();
-    if (whole) {
-      const int c = (lane % kLanes) * V, t = t0 + lane / kLanes;
-      T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + r + c;
+      for (int i = 0; i < 16; ++i) f[i] += __shfl_sync(0xffffffffu, bias, 16 * h + i);
+    }
+    lin_act(f, a.act);
 #pragma unroll
-      for (int k = 0; k < kIters; ++k) {
-        float v[V];
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-          const float4 q = *reinterpret_cast<const float4*>(stage + (k * kRows + lane / kLanes) * kLinPitch + c + i);
-          v[i] = q.x + bias[i]; v[i + 1] = q.y + bias[i + 1]; v[i + 2] = q.z + bias[i + 2]; v[i + 3] = q.w + bias[i + 3];
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        if (a.resid) {
+          f[2 * i] += __uint_as_float(resid[i] << 16);
+          f[2 * i + 1] += __uint_as_float(resid[i] & 0xFFFF0000u);
         }
-        lin_act(v, a.act);
-        const T* re = reinterpret_cast<const T*>(&resid[k]);
-        uint4 oq;
-        T* oe = reinterpret_cast<T*>(&oq);
-#pragma unroll
-        for (int i = 0; i < V; ++i) lin_put(oe + i, a.resid ? v[i] + lin_get(re + i) : v[i]);
-        if (t + k * kRows < a.tokens) *reinterpret_cast<uint4*>(o + (size_t)(k * kRows) * a.out_stride) = oq;
-      }
-    } else if (r + (lane & 15) < a.rows) {
-      // rows of any alignment, the last features: 16 lanes to a token
-      const int f = r + (lane & 15), t = t0 + (lane >> 4);
-      const float b = a.bias ? a.bias[f] : 0.0f;
-      const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + f : nullptr;
-      T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + f;
-#pragma unroll 1
-      for (int i = 0; i < 16; i += 8) {
-        float v[8], res[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          res[k] = q && t + 2 * (i + k) < a.tokens ? lin_get(q + (size_t)(2 * (i + k)) * a.resid_stride) : 0.0f;
-          v[k] = stage[(2 * (i + k) + (lane >> 4)) * kLinPitch + (lane & 15)] + b;
-        }
-        lin_act(v, a.act);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (t + 2 * (i + k) < a.tokens) lin_put(o + (size_t)(2 * (i + k)) * a.out_stride, q ? v[k] + res[k] : v[k]);
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+      } else {
+        w[i] = __float_as_uint(a.resid ? f[i] + __uint_as_float(resid[i]) : f[i]);
       }
     }
-    __syncwarp();
   }
 };
+
+// 16 features r.. of a warp's tokens t0 .. t0 + 31 where rows have any
+// alignment: from shared memory, 16 lanes to a token.
+template <typename T>
+__device__ __noinline__ void lin_ragged(const LinTile& a, int t0, int r, const float* stage) {
+  const int lane = threadIdx.x & 31;
+  if (r + (lane & 15) < a.rows) {
+    const int f = r + (lane & 15), t = t0 + (lane >> 4);
+    const float b = a.bias ? a.bias[f] : 0.0f;
+    const T* q = a.resid ? static_cast<const T*>(a.resid) + (size_t)t * a.resid_stride + f : nullptr;
+    T* o = static_cast<T*>(a.out) + (size_t)t * a.out_stride + f;
+#pragma unroll 1
+    for (int i = 0; i < 16; i += 8) {
+      float v[8], res[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        res[k] = q && t + 2 * (i + k) < a.tokens ? lin_get(q + (size_t)(2 * (i + k)) * a.resid_stride) : 0.0f;
+        v[k] = stage[(2 * (i + k) + (lane >> 4)) * kLinPitch + (lane & 15)] + b;
+      }
+      lin_act(v, a.act);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (t + 2 * (i + k) < a.tokens) lin_put(o + (size_t)(2 * (i + k)) * a.out_stride, q ? v[k] + res[k] : v[k]);
+    }
+  }
+  __syncwarp();
+}
+
+// 16 features r.. of a warp's 32 tokens, the first (h 0) or second half of 32
+// that leave by one tensor store, which cuts them at the output's edges: a row
+// of 32 lies in the staging buffer as the store's swizzle has it (64 bytes of
+// bf16, 128 of f32).  Stores from registers, 32 bytes a row, took 900 clocks for
+// what takes 300 so: their addresses and branches, with two to four warps a
+// scheduler to hide them.
+template <typename T>
+__device__ __forceinline__ void lin_store(const LinTile& a, const CUtensorMap* map, const LinEdge<T>& e, float bias,
+                                          int t0, int r, int h, float (&f)[16], uint8_t* stage) {
+  const int lane = threadIdx.x & 31;
+  if (!a.vec) {
+    float* p = reinterpret_cast<float*>(stage);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<float4*>(p + lane * kLinPitch + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    __syncwarp();
+    lin_ragged<T>(a, t0, r, p);
+    return;
+  }
+  uint32_t w[LinEdge<T>::kWords];
+  e.finish(a, bias, h, f, w);
+  if (h == 0) {  // the store before has read the buffer
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+  }
+  constexpr int kRow = 32 * sizeof(T), kHalf = kRow / 32;  // 16-byte pieces of 16 features
+  const int turn = kRow == 64 ? (lane >> 1) & 3 : lane & 7;
+#pragma unroll
+  for (int i = 0; i < kHalf; ++i)
+    *reinterpret_cast<uint4*>(stage + lane * kRow + (((kHalf * h + i) ^ turn) << 4)) =
+        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  if (h == 1) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0 && t0 < a.tokens && r - 16 < a.rows)
+      asm volatile(
+          "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+          "cp.async.bulk.commit_group;"
+          ::"l"(map), "r"(r - 16), "r"(t0), "r"(smem_u32(stage)) : "memory");
+  }
+}
+// Behind a warp's last store: shared memory may go.
+__device__ __forceinline__ void lin_stored() {
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
 
 // Feature m of token t, behind its activation.
 template <typename T>
@@ -276,13 +334,35 @@ __device__ __forceinline__ float lin_remote(const float* p, int rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
 }
-__device__ __forceinline__ float4 lin_remote4(const float* p, int rank) {
+// A cluster shares a tile's k-blocks.  Of the tile's parts of 32 x 32 (part
+// 4 c + q: 32 columns, rows 32 q ..) CTA (or pair) k % splits gets everyone's sums
+// of the k-th, in its ring, whose tiles are used up by then: four columns of a
+// row together.  Half h of part k's columns of a lane's row, sent there:
+__device__ __forceinline__ void lin_send(const uint8_t* ring, int k, int h, int splits, int from, int to_rank,
+                                         const float (&f)[16]) {
   uint32_t at;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(at)
+      : "r"(smem_u32(ring) + (k / splits * splits + from) * kLinPart + h * (kLinPart / 2) + (threadIdx.x & 31) * 16),
+        "r"(to_rank));
+#pragma unroll
+  for (int i = 0; i < 16; i += 4)
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(at + i * 128), "f"(f[i]), "f"(f[i + 1]), "f"(f[i + 2]), "f"(f[i + 3]) : "memory");
+}
+// and the sum of this CTA's i-th part, in the order of the CTAs
+__device__ __forceinline__ void lin_sum(const uint8_t* ring, int i, int h, int splits, float (&f)[16]) {
+  const uint8_t* at = ring + i * splits * kLinPart + h * (kLinPart / 2) + (threadIdx.x & 31) * 16;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) f[j] = 0.0f;
+#pragma unroll 2
+  for (int r = 0; r < splits; ++r, at += kLinPart) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(at + j * 128);
+      f[j] += v.x; f[j + 1] += v.y; f[j + 2] += v.z; f[j + 3] += v.w;
+    }
+  }
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -291,7 +371,8 @@ __device__ __forceinline__ void cluster_sync() {
 // CH accumulator chains a buffer; SPLIT: a cluster shares one tile's k-blocks.
 template <int BN, int CH, bool SWAP, bool SPLIT, typename T>
 __global__ void __launch_bounds__(kLinThreads, 1)
-    linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, LinTile a) {
+    linear_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
+                  const __grid_constant__ CUtensorMap out_map, const __grid_constant__ LinTile a) {
   using Sh = LinShape<BN, CH>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -393,7 +474,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
   } else {
     const int q = warp & 3;  // tensor-memory lanes 32 q ..
-    float* stage = reinterpret_cast<float*>(ring + Sh::kStages * Sh::kStage) + (warp - 2) * (kLinStage / 4);
+    uint8_t* stage = ring + Sh::kStages * Sh::kStage + (warp - 2) * kLinStage;
     // 16 columns of buffer d, its chains added in order
     auto sums = [&](int d, int c, float (&f)[16]) {
 #pragma unroll
@@ -406,95 +487,114 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     };
     constexpr int kCols = BN >= 32 ? BN / 2 : BN;  // columns of a warp
     const int c0 = (warp - 2) / 4 * kCols;
-    int nu = 0;
-    for (int u = u0; u < units && !*dead; u += step, ++nu) {
-      const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
-      const int m = mt * kLinM + 32 * q + lane;
-      LinRow<T> pre;
-      float bias = 0.0f;
-      if constexpr (!SPLIT) {
-        if constexpr (SWAP) bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
-        else pre.load(a, m - lane, nt * BN + c0);
-      }
-      const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
-      if (!__all_sync(0xffffffffu, w_ok)) break;
+    if constexpr (SPLIT && !SWAP) {
+      const bool ok = __all_sync(0xffffffffu, lin_wait(&dfull[0], 0, dead));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      cluster_sync();  // every CTA's ring is used up
 #pragma unroll 1
-      for (int c = c0; c < c0 + kCols; c += 16) {
-        LinRow<T> ahead;
-        if constexpr (!SPLIT && !SWAP) ahead.load(a, m - lane, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
+      for (int c = c0; ok && c < c0 + kCols; c += 16) {
         float f[16];
-        sums(d, c, f);
-        if constexpr (SPLIT) {
-          // all MMAs are done: the ring holds the sums, [column][row], or four
-          // columns of a row together
-          float* part = reinterpret_cast<float*>(ring) + (size_t)c * kLinM;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if constexpr (SWAP) part[i * kLinM + 32 * q + lane] = f[i];
-            else if (i % 4 == 0)
-              *reinterpret_cast<float4*>(part + i * kLinM + 4 * (32 * q + lane)) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-          }
-        } else if constexpr (SWAP) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] += bias;
-          lin_act(f, a.act);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (m < a.rows && nt * BN + c + i < a.tokens) lin_one<T>(a, nt * BN + c + i, m, f[i]);
-        } else {
-          pre.store(a, m - lane, nt * BN + c, f, stage);
-          pre = ahead;
-        }
-        __syncwarp();
+        sums(0, c, f);
+        const int k = c / 32 * 4 + q;
+        lin_send(ring, k, (c >> 4) & 1, a.splits, rank, k % a.splits, f);
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&dempty[d]);  // the buffer is read
+      cluster_sync();
+      const int mt = u0 % a.mtiles, nt = u0 / a.mtiles;
+      for (int i = warp - 2, k; (k = i * a.splits + rank) < BN / 8; i += kLinEpi)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t0 = mt * kLinM + 32 * (k & 3), r = nt * BN + (k >> 2) * 32 + 16 * h;
+          LinEdge<T> e;
+          e.load(a, t0 + lane, r);
+          const float bias = lin_bias(a, r - 16 * h);
+          float f[16];
+          lin_sum(ring, i, h, a.splits, f);
+          lin_store<T>(a, &out_map, e, bias, t0, r, h, f, stage);
+        }
+      lin_stored();
+    } else {
+      int nu = 0;
+      for (int u = u0; u < units && !*dead; u += step, ++nu) {
+        const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
+        const int m = mt * kLinM + 32 * q + lane;
+        LinEdge<T> pre;
+        float bias = 0.0f;
+        if constexpr (!SPLIT) {
+          if constexpr (SWAP) bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
+          else pre.load(a, m, nt * BN + c0), bias = lin_bias(a, nt * BN + c0);
+        }
+        const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
+        if (!__all_sync(0xffffffffu, w_ok)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if constexpr (SWAP) {
+#pragma unroll 1
+          for (int c = c0; c < c0 + kCols; c += 16) {
+            float f[16];
+            sums(d, c, f);
+            if constexpr (SPLIT) {
+              // all MMAs are done: the ring holds the sums, [column][row]
+              float* part = reinterpret_cast<float*>(ring) + (size_t)c * kLinM + 32 * q + lane;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) part[i * kLinM] = f[i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i] += bias;
+              lin_act(f, a.act);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (m < a.rows && nt * BN + c + i < a.tokens) lin_one<T>(a, nt * BN + c + i, m, f[i]);
+            }
+            __syncwarp();
+          }
+        } else {
+#pragma unroll 1
+          for (int c = c0; c < c0 + kCols; c += 32) {
+            const float b = bias;
+            if (c + 32 < c0 + kCols) bias = lin_bias(a, nt * BN + c + 32);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = nt * BN + c + 16 * h;
+              LinEdge<T> ahead;
+              if (c + 16 * h + 16 < c0 + kCols) ahead.load(a, m, r + 16);
+              float f[16];
+              sums(d, c + 16 * h, f);
+              lin_store<T>(a, &out_map, pre, b, m - lane, r, h, f, stage);
+              pre = ahead;
+            }
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dempty[d]);  // the buffer is read
+      }
+      if constexpr (!SWAP) lin_stored();
     }
   }
-  if constexpr (SPLIT) {
+  if constexpr (SPLIT && !SWAP) {
+    if (warp < 2) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
+  } else if constexpr (SPLIT) {
     __syncwarp();
     cluster_sync();
     if (warp >= 2) {
-      // this rank's share of the tile, dealt to its warps: columns (of
-      // tokens), or 16 of them (of features)
+      // this rank's share of the tile's columns, dealt to its warps
       const int q = warp & 3, mt = u0 % a.mtiles, nt = u0 / a.mtiles, m = mt * kLinM + 32 * q + lane;
       const int who = rank + a.splits * ((warp - 2) / 4), all = a.splits * (kLinEpi / 4);
-      float* stage = reinterpret_cast<float*>(ring + Sh::kStages * Sh::kStage) + (warp - 2) * (kLinStage / 4);
-      const float* part = reinterpret_cast<const float*>(ring) + (SWAP ? 1 : 4) * (32 * q + lane);
-      if constexpr (SWAP) {
-        const int cols = min(BN, a.tokens - nt * BN);
-        const float bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
-        for (int c = who; c < cols; c += all) {
-          float v[8], f[1] = {0.0f};
+      const float* part = reinterpret_cast<const float*>(ring) + 32 * q + lane;
+      const int cols = min(BN, a.tokens - nt * BN);
+      const float bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
+      for (int c = who; c < cols; c += all) {
+        float v[8], f[1] = {0.0f};
 #pragma unroll
-          for (int r = 0; r < 8; ++r) v[r] = r < a.splits ? lin_remote(part + (size_t)c * kLinM, r) : 0.0f;
+        for (int r = 0; r < 8; ++r) v[r] = r < a.splits ? lin_remote(part + (size_t)c * kLinM, r) : 0.0f;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) f[0] += v[r];  // in rank order
-          f[0] += bias;
-          lin_act(f, a.act);
-          if (m < a.rows) lin_one<T>(a, nt * BN + c, m, f[0]);
-        }
-      } else {
-        for (int c = 16 * who; c < BN; c += 16 * all) {
-          LinRow<T> pre;
-          pre.load(a, m - lane, nt * BN + c);
-          float f[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = 0.0f;
-#pragma unroll 4
-          for (int r = 0; r < a.splits; ++r) {
-            float4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = lin_remote4(part + (size_t)(c + 4 * i) * kLinM, r);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[4 * i] += v[i].x; f[4 * i + 1] += v[i].y; f[4 * i + 2] += v[i].z; f[4 * i + 3] += v[i].w;
-            }
-          }
-          pre.store(a, m - lane, nt * BN + c, f, stage);
-        }
+        for (int r = 0; r < 8; ++r) f[0] += v[r];  // in rank order
+        f[0] += bias;
+        lin_act(f, a.act);
+        if (m < a.rows) lin_one<T>(a, nt * BN + c, m, f[0]);
       }
     }
     __syncwarp();
@@ -515,11 +615,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 constexpr int kPairEpi = 16, kPairThreads = (2 + kPairEpi) * 32;
 constexpr int kPairTile = 128 * kLinKB * 2;  // x's part in one CTA
 constexpr int kPairStage = kPairTile + 128 * kLinKB * 2, kPairStages = 5;
+static_assert((256 / 8 + 3) * kLinPart <= kPairStages * kPairStage, "a split's sums fit the ring");
 constexpr int kPairSmem = 2048 + kPairStages * kPairStage + kPairEpi * kLinStage;
 
-__device__ __forceinline__ uint32_t lead_addr(const void* p) {
+__device__ __forceinline__ uint32_t remote_addr(const void* p, int rank) {
   uint32_t at;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(0));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
   return at;
 }
 // This GPU's own memory only, into this CTA; the bytes count at the even CTA's barrier.
@@ -528,16 +629,18 @@ __device__ __forceinline__ void pair_tma(uint32_t dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
       "%3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-// Arrives at the same barrier of both CTAs.
-__device__ __forceinline__ void pair_commit(uint32_t bar) {
+// Arrives at the same barrier of both CTAs, the even one of which is `lead`.
+__device__ __forceinline__ void pair_commit(uint32_t bar, int lead) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(bar), "h"((uint16_t)3) : "memory");
+      ::"r"(bar), "h"((uint16_t)(3 << lead)) : "memory");
 }
 
-template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, LinTile a) {
+// SPLIT: a cluster of pairs shares one tile's k-blocks.
+template <bool SPLIT, typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
+                       const __grid_constant__ CUtensorMap out_map, const __grid_constant__ LinTile a) {
   constexpr int BN = 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -550,6 +653,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   volatile int* dead = reinterpret_cast<volatile int*>(smem + 516);
   uint8_t* ring = smem + 1024;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x & 1;
+  // its pair's place in the cluster, and the even CTA's rank there
+  const int pair = SPLIT ? (int)(blockIdx.x / 2 % a.splits) : 0, lead = 2 * pair;
   constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
                              (16u << 24);  // M 256
 
@@ -576,20 +681,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();  // the other CTA's barriers are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
-  const int units = a.mtiles * a.ntiles, u0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int units = a.mtiles * a.ntiles, u0 = SPLIT ? blockIdx.x / (2 * a.splits) : blockIdx.x >> 1;
+  const int step = SPLIT ? units : (int)(gridDim.x >> 1);
+  const int kb0 = SPLIT ? a.nkb * pair / a.splits : 0, kb1 = SPLIT ? a.nkb * (pair + 1) / a.splits : a.nkb;
 
   const uint32_t ring_at = smem_u32(ring), full_at = smem_u32(full), empty_at = smem_u32(empty);
   if (warp == 0) {
     if (lane == 0) {
       Ring<kPairStages> r(1);
-      const uint32_t lead_full = lead_addr(full);
+      const uint32_t lead_full = remote_addr(full, lead);
       uint32_t loads = 0;
       for (int u = u0; u < units && !*dead; u += step) {
         int mt, nt;
         lin_place(a, u, mt, nt);
         const int my = (2 * mt + rank) * 128, ny = nt * BN + rank * (BN / 2);
 #pragma unroll 1
-        for (int kb = 0; kb < a.nkb; ++kb, r.next(), ++loads) {
+        for (int kb = kb0; kb < kb1; ++kb, r.next(), ++loads) {
           if (!lin_wait(empty_at + 8 * r.s, r.parity, dead)) break;
           if (rank == 0) lin_expect(full_at + 8 * r.s, 2 * kPairStage);
           const uint32_t bar = lead_full + 8 * r.s, st = ring_at + r.s * kPairStage;
@@ -617,7 +724,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool ok = true;
 #pragma unroll 1
-        for (int kb = 0; kb < a.nkb; ++kb, r.next()) {
+        for (int kb = kb0; kb < kb1; ++kb, r.next()) {
           if (!lin_wait(full_at + 8 * r.s, r.parity, dead)) {
             ok = false;
             break;
@@ -629,13 +736,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             asm volatile(
                 "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                 " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
-                ::"r"(tmem + (uint32_t)(d * BN)), "l"(da + 2 * j), "l"(db + 2 * j), "r"(idesc), "r"((uint32_t)(kb | j))
+                ::"r"(tmem + (uint32_t)(d * BN)), "l"(da + 2 * j), "l"(db + 2 * j), "r"(idesc), "r"((uint32_t)((kb - kb0) | j))
                 : "memory");
           }
-          pair_commit(empty_at + 8 * r.s);
+          pair_commit(empty_at + 8 * r.s, lead);
         }
         if (!ok) break;
-        pair_commit(smem_u32(&dfull[d]));
+        pair_commit(smem_u32(&dfull[d]), lead);
       }
       // every MMA is complete before tensor memory is freed
       asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];"
@@ -646,35 +753,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int q = warp & 3;  // tensor-memory lanes 32 q ..
     constexpr int kCols = BN / (kPairEpi / 4);  // columns of a warp
     const int c0 = (warp - 2) / 4 * kCols;
-    float* stage = reinterpret_cast<float*>(ring + kPairStages * kPairStage) + (warp - 2) * (kLinStage / 4);
-    int nu = 0;
-    for (int u = u0; u < units && !*dead; u += step, ++nu) {
-      const int d = nu & 1;
-      int mt, nt;
-      lin_place(a, u, mt, nt);
-      const int m = (2 * mt + rank) * 128 + 32 * q + lane;
-      LinRow<T> pre;
-      pre.load(a, m - lane, nt * BN + c0);
-      const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
-      if (!__all_sync(0xffffffffu, w_ok)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-      for (int c = c0; c < c0 + kCols; c += 16) {
-        LinRow<T> ahead;
-        ahead.load(a, m - lane, c + 16 < c0 + kCols ? nt * BN + c + 16 : a.rows);
-        uint32_t v[16];
-        lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
-        float f[16];
+    uint8_t* stage = ring + kPairStages * kPairStage + (warp - 2) * kLinStage;
+    const auto sums = [&](int d, int c, float (&f)[16]) {
+      uint32_t v[16];
+      lin_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(d * BN + c), v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-        pre.store(a, m - lane, nt * BN + c, f, stage);
-        pre = ahead;
-        __syncwarp();
+      for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+    };
+    if constexpr (SPLIT) {
+      const bool ok = __all_sync(0xffffffffu, lin_wait(&dfull[0], 0, dead));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      cluster_sync();  // every CTA's ring is used up
+#pragma unroll 1
+      for (int c = c0; ok && c < c0 + kCols; c += 16) {
+        float f[16];
+        sums(0, c, f);
+        const int k = c / 32 * 4 + q;
+        lin_send(ring, k, (c >> 4) & 1, a.splits, pair, 2 * (k % a.splits) + rank, f);
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      cluster_sync();
+      int mt, nt;
+      lin_place(a, u0, mt, nt);
+      for (int i = warp - 2, k; (k = i * a.splits + pair) < BN / 8; i += kPairEpi)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t0 = (2 * mt + rank) * 128 + 32 * (k & 3), r = nt * BN + (k >> 2) * 32 + 16 * h;
+          LinEdge<T> e;
+          e.load(a, t0 + lane, r);
+          const float bias = lin_bias(a, r - 16 * h);
+          float f[16];
+          lin_sum(ring, i, h, a.splits, f);
+          lin_store<T>(a, &out_map, e, bias, t0, r, h, f, stage);
+        }
+    } else {
+      int nu = 0;
+      for (int u = u0; u < units && !*dead; u += step, ++nu) {
+        const int d = nu & 1;
+        int mt, nt;
+        lin_place(a, u, mt, nt);
+        const int m = (2 * mt + rank) * 128 + 32 * q + lane;
+        LinEdge<T> pre;
+        pre.load(a, m, nt * BN + c0);
+        float bias = lin_bias(a, nt * BN + c0);
+        const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
+        if (!__all_sync(0xffffffffu, w_ok)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+        for (int c = c0; c < c0 + kCols; c += 32) {
+          const float b = bias;
+          if (c + 32 < c0 + kCols) bias = lin_bias(a, nt * BN + c + 32);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = nt * BN + c + 16 * h;
+            LinEdge<T> ahead;
+            if (c + 16 * h + 16 < c0 + kCols) ahead.load(a, m, r + 16);
+            float f[16];
+            sums(d, c + 16 * h, f);
+            lin_store<T>(a, &out_map, pre, b, m - lane, r, h, f, stage);
+            pre = ahead;
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)  // the buffer is read
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_addr(&dempty[d], lead)) : "memory");
+      }
+    }
+    lin_stored();
+  }
+  if constexpr (SPLIT) {
+    if (warp < 2) {
       __syncwarp();
-      if (lane == 0)  // the buffer is read
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_addr(&dempty[d])) : "memory");
+      cluster_sync();
+      cluster_sync();
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -719,6 +870,27 @@ int lin_map(CUtensorMap* map, const uint16_t* p, int rows, int cols, long long s
              : kErrArg;
 }
 
+// The output, boxes of 32 tokens x 32 features, swizzled by their row's width.
+// Where its rows are not on 16-byte boundaries the kernel takes none.
+int lin_out_map(CUtensorMap* map, const LinearArgs& l, const CUtensorMap& other, bool vec) {
+  if (!vec) {
+    *map = other;
+    return kOk;
+  }
+  LinEncodeFn enc = lin_encode_fn();
+  if (!enc) return kErrLaunch;
+  const bool half = l.out_type == kTypeBF16;
+  const cuuint64_t dims[2] = {(cuuint64_t)l.rows, (cuuint64_t)l.tokens};
+  const cuuint64_t strides[1] = {(cuuint64_t)l.out_stride * (half ? 2 : 4)};
+  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, l.out, dims, strides,
+             box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? kOk
+             : kErrArg;
+}
+
 int lin_vec(const LinearArgs& l) {
   const unsigned long long e = l.out_type == kTypeBF16 ? 2 : 4;
   const unsigned long long all = reinterpret_cast<uintptr_t>(l.out) | reinterpret_cast<uintptr_t>(l.resid) |
@@ -735,9 +907,10 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   const int ma = SWAP ? l.rows : l.tokens, nb = SWAP ? l.tokens : l.rows;
   a.mtiles = (ma + kLinM - 1) / kLinM;
   a.ntiles = (nb + BN - 1) / BN;
-  CUtensorMap wm, xm;
+  CUtensorMap wm, xm, om;
   if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, SWAP ? kLinM : BN)) return e;
   if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, SWAP ? BN : kLinM)) return e;
+  if (int e = lin_out_map(&om, l, xm, !SWAP && a.vec)) return e;
   auto fn = linear_kernel<BN, CH, SWAP, SPLIT, T>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
     return kErrLaunch;
@@ -755,26 +928,37 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = SPLIT ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, fn, SWAP ? wm : xm, SWAP ? xm : wm, a) == cudaSuccess ? kOk : kErrLaunch;
+  return cudaLaunchKernelEx(&cfg, fn, SWAP ? wm : xm, SWAP ? xm : wm, om, a) == cudaSuccess ? kOk : kErrLaunch;
 }
 
-template <typename T>
-int linear_pair(const LinearArgs& l, cudaStream_t stream) {
-  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, 1, lin_vec(l)};
+template <bool SPLIT, typename T>
+int linear_pair(const LinearArgs& l, int splits, cudaStream_t stream) {
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits, lin_vec(l)};
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   a.mtiles = (l.tokens + 255) / 256;
   a.ntiles = (l.rows + 255) / 256;
   const long long units = (long long)a.mtiles * a.ntiles;
   if (units > 0x3fffffffLL) return kErrShape;
-  CUtensorMap wm, xm;
+  CUtensorMap wm, xm, om;
   if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, 128)) return e;
   if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, 128)) return e;
-  auto fn = linear_pair_kernel<T>;
+  if (int e = lin_out_map(&om, l, xm, a.vec)) return e;
+  auto fn = linear_pair_kernel<SPLIT, T>;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess)
     return kErrLaunch;
   const int pairs = device_sm_count() / 2;
-  fn<<<2 * (unsigned)(units < pairs ? units : pairs), kPairThreads, kPairSmem, stream>>>(xm, wm, a);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * (unsigned)(SPLIT ? units * splits : units < pairs ? units : pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2 * splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, xm, wm, om, a) == cudaSuccess ? kOk : kErrLaunch;
 }
 
 // Clusters of s CTAs (one an SM) that the current device runs at a time: SMs
@@ -808,12 +992,13 @@ int linear_clusters(int s) {
   return n;
 }
 
-// CTAs that share a tile's k-blocks: the most (8 is a portable cluster) whose
-// clusters all run at once, each CTA with two k-blocks or more.
-int linear_splits(long long units, int cols) {
-  const int nkb = (cols + kLinKB - 1) / kLinKB;
-  for (int s = nkb / 2 < 8 ? nkb / 2 : 8; s > 1; --s)
-    if (units * s <= device_sm_count() && units <= linear_clusters(s)) return s;
+// CTAs, or pairs of them (`each` 2), that share a tile's k-blocks: the most (8
+// CTAs are a portable cluster) whose clusters all run at once, each CTA with two
+// k-blocks or more.
+int linear_splits(long long units, int cols, int each = 1) {
+  const int nkb = (cols + kLinKB - 1) / kLinKB, most = 8 / each;
+  for (int s = nkb / 2 < most ? nkb / 2 : most; s > 1; --s)
+    if (units * s * each <= device_sm_count() && units <= linear_clusters(s * each)) return s;
   return 1;
 }
 
@@ -842,13 +1027,16 @@ int linear_pick(const LinearArgs& l, cudaStream_t stream) {
   const long long sms = device_sm_count(), nkb = (l.cols + kLinKB - 1) / kLinKB;
   const long long t128 = (l.tokens + 127LL) / 128, t256 = (l.tokens + 255LL) / 256;
   const long long r128 = (l.rows + 127LL) / 128, r256 = (l.rows + 255LL) / 256;
-  const auto cost = [&](long long units, int kblock, int sums) {
-    const int s = linear_splits(units, l.cols);
-    return 600 + (units + sms - 1) / sms * ((nkb + s - 1) / s) * kblock + (s > 1 ? sums : 0);
+  const auto cost = [&](long long units, int each, int start, int kblock, int sums) {
+    const int s = linear_splits(units, l.cols, each);
+    return start + (units * each + sms - 1) / sms * ((nkb + s - 1) / s) * kblock + (s > 1 ? sums : 0);
   };
-  const long long small = cost(t128 * r128, 28, 200), single = cost(t128 * r256, 48, 400);
-  const long long pairs = 900 + (t256 * r256 + sms / 2 - 1) / (sms / 2) * nkb * 33;
-  if (pairs <= small && pairs <= single) return linear_pair<T>(l, stream);
+  const long long small = cost(t128 * r128, 1, 600, 28, 200), single = cost(t128 * r256, 1, 600, 48, 400);
+  const long long pairs = cost(t256 * r256, 2, 900, 33, 400);
+  if (pairs <= small && pairs <= single) {
+    const int s = linear_splits(t256 * r256, l.cols, 2);
+    return s > 1 ? linear_pair<true, T>(l, s, stream) : linear_pair<false, T>(l, 1, stream);
+  }
   return small <= single ? linear_single<128, 2, false, T>(l, stream) : linear_single<256, 1, false, T>(l, stream);
 }
 
