@@ -24,8 +24,8 @@
 //   more tokens than 64: 128 x 128 or 128 x 256 tiles.  Where these are fewer
 //     than the SMs, a tile's k-blocks are dealt to a cluster of CTAs, whose sums
 //     meet in shared memory and are added in rank order.  Bound by what L2
-//     delivers to an SM (about 50 bytes a clock) and a start and end of 5 us
-//     (128 x 1024 x 64: 5.4 us).
+//     delivers to an SM (about 55 bytes a clock) and a start and end of 4 to 6 us
+//     (512 x 3712 x 64: 4.5 and 5.7 us).
 //   many tokens: a pair of CTAs computes a 256 x 256 tile (cta_group::2); each
 //     holds its 128 rows of x and half of W's.  Bound by the tensor cores and
 //     by what L2 delivers: 64 bytes a clock and SM at full rate, where a single
@@ -73,6 +73,7 @@ struct LinTile {
   int act;
   int nkb, mtiles, ntiles, splits;
   int vec;  // out, resid and bias take 16-byte accesses at every 16th feature
+  int whole;  // features in whole 16-byte pieces
 };
 
 // Unit u's tile: along bands of eight tiles of M, so that the tiles in work at a
@@ -276,9 +277,9 @@ __device__ __noinline__ void lin_ragged(const LinTile& a, int t0, int r, const f
 // 16 features r.. of a warp's 32 tokens, the first (h 0) or second half of 32
 // that leave by one tensor store, which cuts them at the output's edges: a row
 // of 32 lies in the staging buffer as the store's swizzle has it (64 bytes of
-// bf16, 128 of f32).  Stores from registers, 32 bytes a row, took 900 clocks for
-// what takes 300 so: their addresses and branches, with two to four warps a
-// scheduler to hide them.
+// bf16, 128 of f32).  Stores from registers, 32 bytes a row, took 1000 clocks for
+// what takes 570 so: their addresses and branches, with two to four warps a
+// scheduler to hide them (18944 x 1024 x 64: 21.8 -> 15.1 us).
 template <typename T>
 __device__ __forceinline__ void lin_store(const LinTile& a, const CUtensorMap* map, const LinEdge<T>& e, float bias,
                                           int t0, int r, int h, float (&f)[16], uint8_t* stage) {
@@ -304,10 +305,21 @@ __device__ __forceinline__ void lin_store(const LinTile& a, const CUtensorMap* m
   for (int i = 0; i < kHalf; ++i)
     *reinterpret_cast<uint4*>(stage + lane * kRow + (((kHalf * h + i) ^ turn) << 4)) =
         make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  // a tensor store cuts at 16 bytes: the features behind the last whole piece
+  // are stored one by one
+  if (a.whole < a.rows && a.whole >= r && a.whole < r + 16 && t0 + lane < a.tokens) {
+    T* o = static_cast<T*>(a.out) + (size_t)(t0 + lane) * a.out_stride + r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (r + i >= a.whole && r + i < a.rows) {
+        if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(o)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        else reinterpret_cast<uint32_t*>(o)[i] = w[i];
+      }
+  }
   if (h == 1) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-    if (lane == 0 && t0 < a.tokens && r - 16 < a.rows)
+    if (lane == 0 && t0 < a.tokens && r - 16 < a.whole)
       asm volatile(
           "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
           "cp.async.bulk.commit_group;"
@@ -610,13 +622,18 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
 // One 256 x 256 tile by two CTAs: each loads its 128 rows of x and half of the
 // tile's 256 rows of W; the even one issues the MMAs of both.
-// Sixteen epilogue warps: with eight, a tile's epilogue took 4.1 us (4096 x 4096,
-// 64 columns), longer than its MMAs below 700 columns.
-constexpr int kPairEpi = 16, kPairThreads = (2 + kPairEpi) * 32;
+// Eight epilogue warps leave room for a sixth stage and have registers enough
+// (8192 x 2688 x 3712 with bias and f32 residual: 159 us with sixteen, 144 with
+// eight); a split's sums, which nothing overlaps, are faster with sixteen (509 x
+// 3712 x 2688: 19.0 us instead of 19.9).
 constexpr int kPairTile = 128 * kLinKB * 2;  // x's part in one CTA
-constexpr int kPairStage = kPairTile + 128 * kLinKB * 2, kPairStages = 5;
-static_assert((256 / 8 + 3) * kLinPart <= kPairStages * kPairStage, "a split's sums fit the ring");
-constexpr int kPairSmem = 2048 + kPairStages * kPairStage + kPairEpi * kLinStage;
+constexpr int kPairStage = kPairTile + 128 * kLinKB * 2;
+template <bool SPLIT>
+struct PairShape {
+  static constexpr int kEpi = SPLIT ? 16 : 8, kThreads = (2 + kEpi) * 32, kStages = SPLIT ? 5 : 6;
+  static constexpr int kSmem = 2048 + kStages * kPairStage + kEpi * kLinStage;
+  static_assert((256 / 8 + 3) * kLinPart <= kStages * kPairStage, "a split's sums fit the ring");
+};
 
 __device__ __forceinline__ uint32_t remote_addr(const void* p, int rank) {
   uint32_t at;
@@ -638,10 +655,10 @@ __device__ __forceinline__ void pair_commit(uint32_t bar, int lead) {
 
 // SPLIT: a cluster of pairs shares one tile's k-blocks.
 template <bool SPLIT, typename T>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(PairShape<SPLIT>::kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map,
                        const __grid_constant__ CUtensorMap out_map, const __grid_constant__ LinTile a) {
-  constexpr int BN = 256;
+  constexpr int BN = 256, kPairEpi = PairShape<SPLIT>::kEpi, kPairStages = PairShape<SPLIT>::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);  // counted at the even CTA
@@ -870,6 +887,8 @@ int lin_map(CUtensorMap* map, const uint16_t* p, int rows, int cols, long long s
              : kErrArg;
 }
 
+int lin_whole(const LinearArgs& l) { return l.rows & ~(l.out_type == kTypeBF16 ? 7 : 3); }
+
 // The output, boxes of 32 tokens x 32 features, swizzled by their row's width.
 // Where its rows are not on 16-byte boundaries the kernel takes none.
 int lin_out_map(CUtensorMap* map, const LinearArgs& l, const CUtensorMap& other, bool vec) {
@@ -880,7 +899,7 @@ int lin_out_map(CUtensorMap* map, const LinearArgs& l, const CUtensorMap& other,
   LinEncodeFn enc = lin_encode_fn();
   if (!enc) return kErrLaunch;
   const bool half = l.out_type == kTypeBF16;
-  const cuuint64_t dims[2] = {(cuuint64_t)l.rows, (cuuint64_t)l.tokens};
+  const cuuint64_t dims[2] = {(cuuint64_t)lin_whole(l), (cuuint64_t)l.tokens};
   const cuuint64_t strides[1] = {(cuuint64_t)l.out_stride * (half ? 2 : 4)};
   const cuuint32_t box[2] = {32, 32};
   const cuuint32_t estr[2] = {1, 1};
@@ -902,7 +921,8 @@ int lin_vec(const LinearArgs& l) {
 template <int BN, int CH, bool SWAP, bool SPLIT, typename T>
 int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
   using Sh = LinShape<BN, CH>;
-  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits, lin_vec(l)};
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits, 0, lin_whole(l)};
+  a.vec = lin_vec(l) && a.whole > 0;
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   const int ma = SWAP ? l.rows : l.tokens, nb = SWAP ? l.tokens : l.rows;
   a.mtiles = (ma + kLinM - 1) / kLinM;
@@ -933,7 +953,8 @@ int linear_run(const LinearArgs& l, int splits, cudaStream_t stream) {
 
 template <bool SPLIT, typename T>
 int linear_pair(const LinearArgs& l, int splits, cudaStream_t stream) {
-  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits, lin_vec(l)};
+  LinTile a{l.bias, l.resid, l.out, l.resid_stride, l.out_stride, l.rows, l.cols, l.tokens, l.act, 0, 0, 0, splits, 0, lin_whole(l)};
+  a.vec = lin_vec(l) && a.whole > 0;
   a.nkb = (l.cols + kLinKB - 1) / kLinKB;
   a.mtiles = (l.tokens + 255) / 256;
   a.ntiles = (l.rows + 255) / 256;
@@ -943,14 +964,15 @@ int linear_pair(const LinearArgs& l, int splits, cudaStream_t stream) {
   if (int e = lin_map(&wm, l.W, l.rows, l.cols, l.cols, 128)) return e;
   if (int e = lin_map(&xm, l.x, l.tokens, l.cols, l.x_stride, 128)) return e;
   if (int e = lin_out_map(&om, l, xm, a.vec)) return e;
+  using Sh = PairShape<SPLIT>;
   auto fn = linear_pair_kernel<SPLIT, T>;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess)
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
     return kErrLaunch;
   const int pairs = device_sm_count() / 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (unsigned)(SPLIT ? units * splits : units < pairs ? units : pairs));
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.blockDim = dim3(Sh::kThreads);
+  cfg.dynamicSmemBytes = Sh::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -1018,11 +1040,11 @@ int linear_pick(const LinearArgs& l, cudaStream_t stream) {
   // k-blocks that one CTA (pair) goes through, and a split's sums through the
   // cluster.  Measured with W in L2, tokens x features x columns, for 128 x 128,
   // 128 x 256 and pairs' 256 x 256:
-  //   128 x 3712 x 2688    10.2   15.4   19.7 us
-  //   512 x 2688 x 5376    29.6   21.4   33.2
-  //   1024 x 1024 x 2048   11.8   13.2   16.9
-  //   1024 x 3712 x 2688   30.7   23.3   21.5
-  //   2048 x 2688 x 5376   78.9   69.6   60.9
+  //   96 x 3712 x 2688     10.1   11.7   13.4 us
+  //   384 x 3712 x 2688    17.1   14.7   16.0
+  //   512 x 2688 x 5376    29.0   21.2   20.0
+  //   1024 x 3712 x 2688   31.5   22.2   19.9
+  //   2048 x 2688 x 5376   86.0   68.6   60.0
   // Pairs of 256 x 128 were within 5% of the best of these at best.
   const long long sms = device_sm_count(), nkb = (l.cols + kLinKB - 1) / kLinKB;
   const long long t128 = (l.tokens + 127LL) / 128, t256 = (l.tokens + 255LL) / 256;
@@ -1031,8 +1053,8 @@ int linear_pick(const LinearArgs& l, cudaStream_t stream) {
     const int s = linear_splits(units, l.cols, each);
     return start + (units * each + sms - 1) / sms * ((nkb + s - 1) / s) * kblock + (s > 1 ? sums : 0);
   };
-  const long long small = cost(t128 * r128, 1, 600, 28, 200), single = cost(t128 * r256, 1, 600, 48, 400);
-  const long long pairs = cost(t256 * r256, 2, 900, 33, 400);
+  const long long small = cost(t128 * r128, 1, 450, 30, 220), single = cost(t128 * r256, 1, 570, 46, 330);
+  const long long pairs = cost(t256 * r256, 2, 680, 33, 330);
   if (pairs <= small && pairs <= single) {
     const int s = linear_splits(t256 * r256, l.cols, 2);
     return s > 1 ? linear_pair<true, T>(l, s, stream) : linear_pair<false, T>(l, 1, stream);

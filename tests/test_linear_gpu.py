@@ -57,8 +57,10 @@ def test_linear(k, cuda, rows, cols, tokens, dtype):
 
 @pytest.mark.parametrize("rows,cols,tokens", [
     (2688, 4096, 100), (1111, 2056, 129),        # 128 x 128, a tile's columns shared
-    (2600, 2200, 401), (8000, 200, 300),         # 128 x 256, shared and not
-    (3700, 1400, 1000), (5000, 1400, 3001)])     # pairs, one and several tiles each
+    (8000, 200, 300),                            # not shared
+    (3700, 2696, 380), (10000, 1000, 300),       # 128 x 256, shared and not
+    (2600, 2200, 401), (3712, 2688, 512),        # pairs, shared
+    (3700, 1400, 1000), (5000, 1400, 3001)])     # one and several tiles each
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_tiles(k, cuda, rows, cols, tokens, dtype):
     W, x, b, r = make(rows, cols, tokens, dtype, True, True, seed=6)
@@ -95,6 +97,20 @@ def test_strides_guards_and_residual_in_place(k, cuda, tokens, dtype):
     want, size = ref.linear(W, x, b, "none", r)
     ref.within(view, want, bound(want, size, cols, dtype))
     assert (wide[:, :3] == 7).all() and (wide[:, 3 + rows:] == 7).all() and (wide[tokens] == 7).all()
+
+
+@pytest.mark.parametrize("rows,cols,tokens", [(331, 136, 200), (334, 1048, 70), (2699, 2696, 381), (3705, 1400, 1001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_aligned_rows_that_end_inside_a_tile(k, cuda, rows, cols, tokens, dtype):
+    """Rows on 16-byte boundaries, neither rows nor tokens whole tiles: what lies beside them stays."""
+    W, x, b, r = make(rows, cols, tokens, dtype, True, True, seed=7)
+    wide = torch.full((tokens + 40, rows // 8 * 8 + 64), 7.0, dtype=dtype, device=cuda)
+    view = wide[:tokens, 8:8 + rows]
+    view.copy_(r)
+    k.linear_bf16(view, put(W, cuda), put(x, cuda), rows, cols, tokens, bias=put(b, cuda), act="silu", resid=view)
+    want, size = ref.linear(W, x, b, "silu", r)
+    ref.within(view, want, bound(want, size, cols, dtype))
+    assert (wide[:, :8] == 7).all() and (wide[:, 8 + rows:] == 7).all() and (wide[tokens:] == 7).all()
 
 
 @pytest.mark.parametrize("tokens", [1, 40, 200])
