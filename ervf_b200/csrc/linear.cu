@@ -305,18 +305,16 @@ __device__ __forceinline__ void lin_store(const LinTile& a, const CUtensorMap* m
   for (int i = 0; i < kHalf; ++i)
     *reinterpret_cast<uint4*>(stage + lane * kRow + (((kHalf * h + i) ^ turn) << 4)) =
         make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  // a tensor store cuts at 16 bytes: the features behind the last whole piece
-  // are stored one by one
-  if (a.whole < a.rows && a.whole >= r && a.whole < r + 16 && t0 + lane < a.tokens) {
-    T* o = static_cast<T*>(a.out) + (size_t)(t0 + lane) * a.out_stride + r;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (r + i >= a.whole && r + i < a.rows) {
-        if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(o)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-        else reinterpret_cast<uint32_t*>(o)[i] = w[i];
-      }
-  }
   if (h == 1) {
+    // a tensor store cuts at 16 bytes: the features behind the last whole piece
+    // are stored one by one
+    if (a.whole < a.rows && a.whole >= r - 16 && a.whole < r + 16 && t0 + lane < a.tokens) {
+      const uint8_t* row = stage + lane * kRow;
+      T* o = static_cast<T*>(a.out) + (size_t)(t0 + lane) * a.out_stride;
+      const int piece = (a.whole - (r - 16)) * (int)sizeof(T) / 16 ^ turn;
+#pragma unroll 1
+      for (int i = a.whole; i < a.rows; ++i) o[i] = reinterpret_cast<const T*>(row + piece * 16)[i - a.whole];
+    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0 && t0 < a.tokens && r - 16 < a.whole)
