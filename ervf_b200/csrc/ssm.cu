@@ -658,9 +658,10 @@ int launch_scan_tokens(const ScanArgs& a, cudaStream_t stream) {
 int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
   const int hpg = a.heads / a.groups;
   // as many CTAs a group as its heads, but no more than three waves of them: a
-  // batch of 96 with eight groups takes 117 us with eight CTAs a group, 93 with
-  // four, 86 with two and 97 with one (each convolves B and C for itself); one
-  // sequence's latency is least with eight
+  // batch of 96 with eight groups took 117 us with eight CTAs a group, 93 with
+  // four, 86 with two and 97 with one (each convolves B and C for itself; two take
+  // 79 since the rows' sums go by halves); one sequence's latency is least with
+  // eight
   const size_t elem = a.type == kTypeBF16 ? 2 : 4;
   auto smem_of = [&](int ctas) {
     const size_t most = (hpg + ctas - 1) / ctas;

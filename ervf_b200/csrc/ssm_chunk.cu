@@ -41,8 +41,8 @@
 // memory take its whole bandwidth (128 bytes a clock); with W, the split state
 // and the tiles a step moves 740 KB there, 5800 clocks; its warps issue 5100
 // instructions a scheduler.  Measured: 11000 clocks, of which P takes 3500, P x
-// 1300 and y 3600 one after the other (64 heads, 8192 tokens: 153 us in all,
-// 27 of them pass 1, 15 passes 0 and 2).  Waits are short and loops little
+// 1300 and y 3600 one after the other (64 heads, 8192 tokens: 148 us in all,
+// 27 of them pass 1).  Waits are short and loops little
 // unrolled on purpose: seven roles' code has to share the instruction cache
 // (waits that watched the clock and unrolled MMA loops: 97 KB, 179 us).  Tried
 // without gain: y of the second head by the W warps, S C ahead of the state's

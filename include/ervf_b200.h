@@ -602,11 +602,11 @@ ERVF_API int ervf_linear_bf16(const uint16_t* W, const uint16_t* x, long long x_
  * where has_state[i] is not zero (u8, device; NULL: nowhere) and left holding
  * the state behind the sequence's last token.  A slot outside [0, n_slots)
  * means none: a zero state, and nothing is stored.  No two sequences of one
- * call may name the same slot. */
+ * call may name the same slot.  seqs <= 2^26. */
 
 /* Causal depthwise convolution of packed prompts: out[t][c] = act(bias[c] +
  * sum_j w[c][j] x[t-width+1+j][c]), act = silu or none.  x, out, state of
- * `type`; w f32 [channels][width], width 2..4; bias f32 or NULL; state
+ * `type`; w f32 [channels][width], width 2..4, channels <= 65535 * 128; bias f32 or NULL; state
  * [n_slots][width-1][channels], the last inputs, oldest first, or NULL (no
  * sequence carries any).  out must not overlap x.  The reference: conv1d, one
  * token at a time (gpu_kernels.py:77-1515). */
