@@ -113,6 +113,19 @@ def test_aligned_rows_that_end_inside_a_tile(k, cuda, rows, cols, tokens, dtype)
     assert (wide[:, :8] == 7).all() and (wide[:, 8 + rows:] == 7).all() and (wide[tokens:] == 7).all()
 
 
+@pytest.mark.parametrize("rows,cols,tokens", [
+    (331, 1048, 70), (8001, 200, 300), (3699, 2696, 380), (10001, 1000, 300), (2599, 2200, 401), (3699, 1400, 1001)])
+def test_rows_of_any_alignment_in_every_tile(k, cuda, rows, cols, tokens):
+    W, x, b, r = make(rows, cols, tokens, torch.bfloat16, True, True, seed=9)
+    wide = torch.full((tokens + 1, rows + 10), 7.0, dtype=torch.bfloat16, device=cuda)
+    view = wide[:tokens, 3:3 + rows]
+    k.linear_bf16(view, put(W, cuda), put(x, cuda), rows, cols, tokens, bias=put(b, cuda), act="gelu",
+                  resid=put(r, cuda))
+    want, size = ref.linear(W, x, b, "gelu", r)
+    ref.within(view, want, bound(want, size, cols, torch.bfloat16))
+    assert (wide[:, :3] == 7).all() and (wide[:, 3 + rows:] == 7).all() and (wide[tokens] == 7).all()
+
+
 @pytest.mark.parametrize("tokens", [1, 40, 200])
 def test_same_bits_every_call(k, cuda, tokens):
     W, x, _, _ = make(2688, 4096, tokens, torch.float32, False, False, seed=3)
