@@ -186,3 +186,39 @@ def test_wrong_arrays_are_refused(k, cuda):
     with pytest.raises(ValueError):
         k.linear_bf16(out.half(), W, x, 32, 64, 4)
     assert (out == 0).all()
+
+
+def test_two_streams_and_a_graph_beside_them(k, cuda):
+    """Calls of every tile form at once on two streams, and the same calls captured, give the bits
+    of one after the other."""
+    shapes = [(1200, 1160, 1), (2688, 2696, 100), (3700, 2696, 380), (2600, 2200, 401), (3700, 1400, 1000)]
+    data = []
+    for i, (rows, cols, tokens) in enumerate(shapes):
+        W, x, b, r = (v.to(cuda) for v in make(rows, cols, tokens, torch.bfloat16, True, True, seed=20 + i))
+        data.append((W, x, b, r, rows, cols, tokens))
+
+    def run(which, outs):
+        for i in which:
+            W, x, b, r, rows, cols, tokens = data[i]
+            k.linear_bf16(outs[i], W, x, rows, cols, tokens, bias=b, act="silu", resid=r)
+
+    def fresh():
+        return [torch.zeros(d[6], d[4], dtype=torch.bfloat16, device=cuda) for d in data]
+
+    every = range(len(data))
+    want, first, second, third = fresh(), fresh(), fresh(), fresh()
+    run(every, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        run(every, third)
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s):
+            run(every, first)
+            g.replay()
+        with torch.cuda.stream(t):
+            run(reversed(every), second)
+    torch.cuda.synchronize()
+    for i in every:
+        assert torch.equal(want[i], first[i]) and torch.equal(want[i], second[i]) and torch.equal(want[i], third[i])
