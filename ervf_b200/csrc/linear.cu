@@ -72,7 +72,7 @@ struct LinTile {
   int rows, cols, tokens;
   int act;
   int nkb, mtiles, ntiles, splits;
-  int vec;  // out, resid and bias take 16-byte accesses at every 16th feature
+  int vec;  // out and resid take 16-byte accesses at every 16th feature
   int whole;  // features in whole 16-byte pieces
 };
 
@@ -911,8 +911,7 @@ int lin_out_map(CUtensorMap* map, const LinearArgs& l, const CUtensorMap& other,
 int lin_vec(const LinearArgs& l) {
   const unsigned long long e = l.out_type == kTypeBF16 ? 2 : 4;
   const unsigned long long all = reinterpret_cast<uintptr_t>(l.out) | reinterpret_cast<uintptr_t>(l.resid) |
-                                 reinterpret_cast<uintptr_t>(l.bias) | l.out_stride * e |
-                                 (l.resid ? l.resid_stride * e : 0);
+                                 l.out_stride * e | (l.resid ? l.resid_stride * e : 0);
   return (all & 15) == 0;
 }
 

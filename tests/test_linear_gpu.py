@@ -146,6 +146,16 @@ def test_infinities_stay_in_their_rows(k, cuda):
     assert torch.isnan(out[140]).all()
 
 
+@pytest.mark.parametrize("tokens", [5, 150, 700])
+def test_bias_of_any_alignment(k, cuda, tokens):
+    W, x, b, _ = make(1024, 512, tokens, torch.float32, True, False, seed=10)
+    shifted = torch.cat([torch.zeros(1), b]).to(cuda)[1:]
+    out = torch.empty(tokens, 1024, device=cuda)
+    k.linear_bf16(out, put(W, cuda), put(x, cuda), 1024, 512, tokens, bias=shifted)
+    want, size = ref.linear(W, x, b, "none", None)
+    ref.within(out, want, bound(want, size, 512, torch.float32))
+
+
 def test_no_tokens(k, cuda):
     W = torch.zeros(16, 16, dtype=torch.bfloat16, device=cuda)
     k.linear_bf16(torch.empty(0, 16, device=cuda), W, torch.empty(0, 16, dtype=torch.bfloat16, device=cuda), 16, 16, 0)
