@@ -143,6 +143,12 @@ __device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ bool lin_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
   return lin_wait(smem_u32(bar), parity, dead);
 }
+// The same for a whole warp: one decision.  Warps that work as one look at
+// `dead` nowhere else, or a lane could leave a loop without the others and the
+// next warp-wide instruction wait for ever.
+__device__ __forceinline__ bool lin_wait_w(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  return __all_sync(0xffffffffu, lin_wait(bar, parity, dead));
+}
 
 // A place in a ring of N stages: the producer's and the issuing thread's loops
 // are one thread's, so their few instructions a k-block are what a k-block
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     constexpr int kCols = BN >= 32 ? BN / 2 : BN;  // columns of a warp
     const int c0 = (warp - 2) / 4 * kCols;
     if constexpr (SPLIT && !SWAP) {
-      const bool ok = __all_sync(0xffffffffu, lin_wait(&dfull[0], 0, dead));
+      const bool ok = lin_wait_w(&dfull[0], 0, dead);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       cluster_sync();  // every CTA's ring is used up
 #pragma unroll 1
@@ -524,7 +530,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
       lin_stored();
     } else {
       int nu = 0;
-      for (int u = u0; u < units && !*dead; u += step, ++nu) {
+      for (int u = u0; u < units; u += step, ++nu) {
         const int mt = u % a.mtiles, nt = u / a.mtiles, d = nu & 1;
         const int m = mt * kLinM + 32 * q + lane;
         LinEdge<T> pre;
@@ -533,8 +539,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           if constexpr (SWAP) bias = a.bias && m < a.rows ? a.bias[m] : 0.0f;
           else pre.load(a, m, nt * BN + c0), bias = lin_bias(a, nt * BN + c0);
         }
-        const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
-        if (!__all_sync(0xffffffffu, w_ok)) break;
+        if (!lin_wait_w(&dfull[d], (nu >> 1) & 1, dead)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if constexpr (SWAP) {
 #pragma unroll 1
@@ -776,7 +781,7 @@ __global__ void __launch_bounds__(PairShape<SPLIT>::kThreads, 1)
       for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
     };
     if constexpr (SPLIT) {
-      const bool ok = __all_sync(0xffffffffu, lin_wait(&dfull[0], 0, dead));
+      const bool ok = lin_wait_w(&dfull[0], 0, dead);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       cluster_sync();  // every CTA's ring is used up
 #pragma unroll 1
@@ -802,7 +807,7 @@ __global__ void __launch_bounds__(PairShape<SPLIT>::kThreads, 1)
         }
     } else {
       int nu = 0;
-      for (int u = u0; u < units && !*dead; u += step, ++nu) {
+      for (int u = u0; u < units; u += step, ++nu) {
         const int d = nu & 1;
         int mt, nt;
         lin_place(a, u, mt, nt);
@@ -810,8 +815,7 @@ __global__ void __launch_bounds__(PairShape<SPLIT>::kThreads, 1)
         LinEdge<T> pre;
         pre.load(a, m, nt * BN + c0);
         float bias = lin_bias(a, nt * BN + c0);
-        const bool w_ok = lin_wait(&dfull[d], (nu >> 1) & 1, dead);
-        if (!__all_sync(0xffffffffu, w_ok)) break;
+        if (!lin_wait_w(&dfull[d], (nu >> 1) & 1, dead)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
         for (int c = c0; c < c0 + kCols; c += 32) {
