@@ -448,9 +448,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
           lin_tma(st + kLinATile, &b_map, kb * kLinKB, ny, bar);
         }
       }
-      // leave no tensor copy in flight
+      // leave no tensor copy in flight, in a dead CTA neither: these waits, bounded
+      // too, end by the copies' arrival and not by the flag
       for (uint32_t k = loads > (uint32_t)Sh::kStages ? loads - Sh::kStages : 0; k < loads; ++k)
-        lin_wait(full_at + 8 * (k % Sh::kStages), (k / Sh::kStages) & 1, dead);
+        mbar_wait(&full[k % Sh::kStages], (k / Sh::kStages) & 1, 200000000LL);
     }
   } else if (warp == 1) {
     if (lane == 0) {

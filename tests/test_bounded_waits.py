@@ -53,3 +53,15 @@ def test_dead_is_read_by_single_lanes_and_by_the_waits_alone(name):
             alone = any(re.search(r"lane == 0|tid == 0|lin_wait_slow", h) for h in around)
             assert alone, f"{name}: a whole warp branches on the flag: {at.strip()}"
     assert reads
+
+
+def test_no_tensor_copy_outlives_a_dead_cta():
+    """The loop behind a producer's last load waits for the copies in flight: by their arrival, or,
+    where it goes by waits that a dead CTA ends at once, by the clock behind it."""
+    lines = stripped("linear.cu")
+    drains = [i for i, line in enumerate(lines) if "k = loads >" in line]
+    assert len(drains) == 2
+    for i in drains:
+        by_arrival = re.search(r"\bmbar_wait\(", lines[i + 1])
+        by_clock = "*dead" in lines[i + 2] and "clock64()" in "".join(lines[i + 3:i + 5])
+        assert by_arrival or by_clock, lines[i + 1].strip()
