@@ -251,10 +251,6 @@ __device__ __forceinline__ void ch_arrive_w(uint64_t* bar) {
 
 __device__ __forceinline__ int chunks_of(int len) { return (len + kQ - 1) / kQ; }
 
-// No more chunks than this, which is what the tables hold, whatever the offsets
-// say (decreasing ones could name a token twice).
-__host__ __device__ __forceinline__ int most_chunks(const Packing& p) { return p.tokens / kQ + p.seqs; }
-
 // A place in the list of steps.
 struct Walk {
   int pair, seq, chunk, begin, len, nch;
@@ -869,7 +865,7 @@ constexpr int kStepThreads = 256;
 __device__ __noinline__ void scan_plan(const ChunkArgs& a, int c, int ctas) {
   int seq = 0, nth = 0, total = 0;
   find_tile(a.pk, -1, kQ, 0, seq, nth, total);
-  total = min(total, most_chunks(a.pk));
+  total = min(total, most_chunks(a.pk, kQ));
   const long long all = (long long)total * a.pairs;
   const long long f0 = cut(all, c, ctas), f1 = cut(all, c + 1, ctas);
   const int n = (int)(f1 - f0);
@@ -922,7 +918,9 @@ __global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a, i
     seq_range(a.pk, 0, b, len);
     total = chunks_of(len);
   }
-  total = min(total, most_chunks(a.pk));
+  total = min(total, most_chunks(a.pk, kQ));
+  const long long entry = step_entry(ph, chunk, total);
+  if (entry < 0) return;
   Walk wk;
   wk.at(a.pk, ph >> 1, seq, nth);
   Heads hd;
@@ -965,7 +963,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a, i
     w[i] = d[i] * ex2(suf + after);
     suf += e[i];
   }
-  Steps& st = a.steps[2 * ((size_t)(ph >> 1) * total + chunk) + (ph & 1)];
+  Steps& st = a.steps[entry];
   *reinterpret_cast<float4*>(&st.lp[4 * lane]) = make_float4(lp[0], lp[1], lp[2], lp[3]);
   *reinterpret_cast<float4*>(&st.d[4 * lane]) = make_float4(d[0], d[1], d[2], d[3]);
   *reinterpret_cast<float4*>(&st.v[4 * lane]) = make_float4(v[0], v[1], v[2], v[3]);
@@ -1105,7 +1103,7 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
   a.pairs = a.ppg * s.groups;
   a.n = N;
   const size_t part = (size_t)kMaxCtas * 2 * kP * N;
-  const long long chunks = most_chunks(s.pk);
+  const long long chunks = most_chunks(s.pk, kQ);
   a.steps = static_cast<Steps*>(s.scratch);
   a.local = reinterpret_cast<float*>(a.steps + 2 * chunks * a.pairs);
   a.init = a.local + part;

@@ -26,7 +26,7 @@ __device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1
 
 // Tokens [begin, begin + len) of sequence i, kept inside the token array
 // whatever the offsets say.
-__device__ __forceinline__ void seq_range(const Packing& p, int i, int& begin, int& len) {
+__host__ __device__ __forceinline__ void seq_range(const Packing& p, int i, int& begin, int& len) {
   if (!p.cu) {
     begin = 0;
     len = p.tokens;
@@ -76,6 +76,16 @@ __device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, 
   }
   total = base;
   return false;
+}
+
+// The chunked scan's table of steps: pairs of entries (a pair's two heads) for
+// each head pair and each chunk of `total`, pair after pair.  It holds
+// most_chunks chunks a pair, whatever the offsets say (decreasing ones could
+// name a token twice); entry of head k = 2 pair + (0 or 1), or -1 for a chunk
+// behind the last.
+__host__ __device__ __forceinline__ int most_chunks(const Packing& p, int size) { return p.tokens / size + p.seqs; }
+__host__ __device__ __forceinline__ long long step_entry(int k, int chunk, int total) {
+  return chunk < total ? 2 * ((long long)(k >> 1) * total + chunk) + (k & 1) : -1;
 }
 
 }  // namespace ervf
