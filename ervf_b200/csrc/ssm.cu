@@ -92,12 +92,12 @@ constexpr int kConvThreads = 128;
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kConvThreads, sizeof(T) == 2 ? 5 : 6) conv_prompt_kernel(ConvArgs a) {
   const int ch = (blockIdx.y * kConvThreads + threadIdx.x) * V;
-  int seq, nth, total;
-  if (!find_tile(a.pk, blockIdx.x, a.tile, 1, seq, nth, total)) return;
-  if (ch >= a.channels) return;
-  int begin, len;
-  seq_range(a.pk, seq, begin, len);
-  const int t0 = nth * a.tile, t1 = min(t0 + a.tile, len);
+  int seq, nth, begin, len;
+  if (!find_place(a.pk, blockIdx.x, a.shift, seq, nth, begin, len)) return;
+  const int tile = 1 << a.shift;
+  // an empty sequence's first tile carries its state on
+  if (ch >= a.channels || (nth > 0 && (long long)nth * tile >= len)) return;
+  const int t0 = nth * tile, t1 = min(t0 + tile, len);
   const T* x = static_cast<const T*>(a.x) + (size_t)(begin + t0) * a.x_stride + ch;
   T* out = static_cast<T*>(a.out) + (size_t)(begin + t0) * a.out_stride + ch;
   int left = t1 - t0;
@@ -189,8 +189,8 @@ int launch_conv(ConvArgs a, cudaStream_t stream) {
   // 64 tokens a tile spread the weights' loads further; 32 where that would
   // leave the SMs short of CTAs
   const long long cols = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
-  a.tile = (a.pk.tokens / 64 + a.pk.seqs) * cols >= 12LL * device_sm_count() ? 64 : 32;
-  const dim3 grid((unsigned)(a.pk.tokens / a.tile + a.pk.seqs), (unsigned)cols);
+  a.shift = (a.pk.tokens / 64 + a.pk.seqs) * cols >= 12LL * device_sm_count() ? 6 : 5;
+  const dim3 grid((unsigned)((a.pk.tokens >> a.shift) + a.pk.seqs), (unsigned)cols);
   if (a.width == 2) conv_prompt_kernel<T, 2, V><<<grid, kConvThreads, 0, stream>>>(a);
   else if (a.width == 3) conv_prompt_kernel<T, 3, V><<<grid, kConvThreads, 0, stream>>>(a);
   else conv_prompt_kernel<T, 4, V><<<grid, kConvThreads, 0, stream>>>(a);

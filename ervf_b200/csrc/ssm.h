@@ -43,7 +43,7 @@ struct ConvArgs {
   void* state;        // [n_slots][width - 1][channels], oldest input first, or NULL
   long long x_stride, out_stride;
   int type, channels, width, silu;
-  int tile;  // set by the launcher: tokens of a CTA
+  int shift;  // set by the launcher: tokens of a CTA, 2^shift
 };
 int launch_conv1d_prompt(const ConvArgs& a, cudaStream_t stream);
 

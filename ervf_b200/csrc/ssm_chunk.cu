@@ -864,7 +864,7 @@ constexpr int kStepThreads = 256;
 // A warp finds the pieces of CTA c for both passes.
 __device__ __noinline__ void scan_plan(const ChunkArgs& a, int c, int ctas) {
   int seq = 0, nth = 0, total = 0;
-  find_tile(a.pk, -1, kQ, 0, seq, nth, total);
+  find_tile(a.pk, -1, kQ, seq, nth, total);
   total = min(total, most_chunks(a.pk, kQ));
   const long long all = (long long)total * a.pairs;
   const long long f0 = cut(all, c, ctas), f1 = cut(all, c + 1, ctas);
@@ -875,14 +875,14 @@ __device__ __noinline__ void scan_plan(const ChunkArgs& a, int c, int ctas) {
     while (before > 0 && cut(all, before, ctas) == f0) --before;
     p3.pair = (int)(f0 / total);
     p3.nth = (int)(f0 - (long long)p3.pair * total);
-    find_tile(a.pk, p3.nth, kQ, 0, p3.seq, p3.chunk, t);
+    find_tile(a.pk, p3.nth, kQ, p3.seq, p3.chunk, t);
     p3.count = n;
     p3.before = before;
     p3.total = total;
     // pass 1: its part of the sequence that its piece ends in, if that goes on
     p1.pair = (int)((f1 - 1) / total);
     const int last = (int)(f1 - 1 - (long long)p1.pair * total);
-    find_tile(a.pk, last, kQ, 0, p1.seq, p1.chunk, t);
+    find_tile(a.pk, last, kQ, p1.seq, p1.chunk, t);
     int b, len;
     seq_range(a.pk, p1.seq, b, len);
     if (p1.chunk < chunks_of(len) - 1) {
@@ -909,10 +909,10 @@ __global__ void __launch_bounds__(kStepThreads) scan_steps_kernel(ChunkArgs a, i
   }
   const int ph = blockIdx.y * (kStepThreads / 32) + (threadIdx.x >> 5);  // pair and head
   int seq = 0, nth = 0, total = 0;
-  if (!find_tile(a.pk, chunk, kQ, 0, seq, nth, total) || ph >= 2 * a.pairs) return;
+  if (!find_tile(a.pk, chunk, kQ, seq, nth, total) || ph >= 2 * a.pairs) return;
   if (a.pk.seqs > 1) {
     int s, n;
-    find_tile(a.pk, -1, kQ, 0, s, n, total);
+    find_tile(a.pk, -1, kQ, s, n, total);
   } else {
     int b, len;
     seq_range(a.pk, 0, b, len);

@@ -44,11 +44,10 @@ __device__ __forceinline__ int seq_slot(const Packing& p, int i) {
 }
 
 // Tile `tile` of the packed sequences, each cut into tiles of `size` tokens
-// from its own first token, an empty one into `empty` (0 or 1): which
-// sequence, and the tile's place in it.  One warp; false past the last tile,
-// with `total` the number of tiles.
-__device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, int empty, int& seq, int& nth,
-                                          int& total) {
+// from its own first token: which sequence, and the tile's place in it.  One
+// warp; false past the last tile, with `total` the number of tiles.  Walks the
+// offsets: for few sequences.
+__device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, int& seq, int& nth, int& total) {
   const int lane = threadIdx.x & 31;
   int base = 0;
   for (int i0 = 0; i0 < p.seqs; i0 += 32) {
@@ -56,7 +55,7 @@ __device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, 
     if (i0 + lane < p.seqs) {
       int b, len;
       seq_range(p, i0 + lane, b, len);
-      n = max(empty, (len - 1) / size + (len > 0));
+      n = (len - 1) / size + (len > 0);
     }
     int inc = n;
 #pragma unroll
@@ -76,6 +75,35 @@ __device__ __forceinline__ bool find_tile(const Packing& p, int tile, int size, 
   }
   total = base;
   return false;
+}
+
+// Tiles of 2^shift tokens in places of their own, with gaps: sequence i owns the
+// places from cu[i] >> shift, plus i, up to the next one's first.  These are
+// at least its tiles and never none, and all of them at most (tokens >> shift) +
+// seqs; so a tile is found by a search in the offsets instead of their running
+// sum.
+__host__ __device__ __forceinline__ int first_place(int begin, int i, int shift) { return (begin >> shift) + i; }
+// Which sequence owns a place (for falling offsets: some sequence), and its
+// tokens; one warp, 32 offsets at a time.  False before the first sequence's.
+__device__ __forceinline__ bool find_place(const Packing& p, int place, int shift, int& seq, int& nth, int& begin,
+                                           int& len) {
+  const int lane = threadIdx.x & 31;
+  seq = 0;
+  for (int n = p.seqs;;) {
+    const int step = (n + 31) / 32, i = lane * step;
+    int b = 0, l = 0;
+    if (i < n) seq_range(p, seq + i, b, l);
+    const unsigned m = __ballot_sync(0xffffffffu, i < n && first_place(b, seq + i, shift) <= place);
+    if (!m) return false;
+    const int at = 31 - __clz(m);
+    seq += at * step;
+    n = min(step, n - at * step);
+    if (step > 1) continue;
+    begin = __shfl_sync(0xffffffffu, b, at);
+    len = __shfl_sync(0xffffffffu, l, at);
+    nth = place - first_place(begin, seq, shift);
+    return true;
+  }
 }
 
 // The chunked scan's table of steps: pairs of entries (a pair's two heads) for

@@ -51,6 +51,20 @@ int main() {
           CHECK(b >= 0 && len >= 0 && b + len <= tokens);
           tiles += (len + kQ - 1) / kQ;
         }
+        // places: one for each tile, found by the largest first place not behind it
+        for (int shift : {5, 6, 7}) {
+          const int size = 1 << shift;
+          std::vector<int> taken(tokens / size + seqs);
+          for (int i = 0; which == 0 && i < seqs; ++i) {
+            int b, len;
+            seq_range(p, i, b, len);
+            for (int k = 0; k < (len ? (len + size - 1) / size : 1); ++k) {
+              const int place = first_place(b, i, shift) + k;
+              CHECK(place >= 0 && place < (int)taken.size() && taken[place]++ == 0);
+              CHECK(i + 1 == seqs || place < first_place(cu[i + 1], i + 1, shift));
+            }
+          }
+        }
         const int most = most_chunks(p, kQ), total = tiles < most ? tiles : most, pairs = 5;
         CHECK(which != 0 || tiles <= most);
         // a launch has as many blocks as chunks or as pieces to plan, whichever is more
