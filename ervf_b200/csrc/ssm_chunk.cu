@@ -1072,9 +1072,14 @@ bool rows16(const void* p, long long stride) {
 
 // The chunked form takes bf16, head_dim 64 and 64 or 128 state columns; and
 // enough tokens: below, the token-by-token kernel's time (0.55 us a token)
-// is less than three launches and a chunk's latency.
-bool chunk_sizes(int type, int tokens, int head_dim, int d_state) {
-  return type == kTypeBF16 && head_dim == kP && (d_state == 64 || d_state == 128) && tokens > 32;
+// is less than three launches and a chunk's latency.  And no more than
+// kMaxChunkSeqs sequences: pass 0 walks all offsets for every chunk, and every
+// role of passes 1 and 3 steps through empty sequences one by one while the
+// others' waits, which are bounded, run.
+constexpr int kMaxChunkSeqs = 16384;
+bool chunk_sizes(int type, int tokens, int seqs, int head_dim, int d_state) {
+  return type == kTypeBF16 && head_dim == kP && (d_state == 64 || d_state == 128) && tokens > 32 &&
+         seqs <= kMaxChunkSeqs;
 }
 
 // The register shares need every register that the block is launched with: a
@@ -1150,14 +1155,14 @@ int launch_chunks(const ScanArgs& s, cudaStream_t stream) {
 }  // namespace
 
 size_t ssm_prompt_scratch_bytes(int type, int tokens, int seqs, int heads, int head_dim, int groups, int d_state) {
-  if (!chunk_sizes(type, tokens, head_dim, d_state)) return 0;
+  if (!chunk_sizes(type, tokens, seqs, head_dim, d_state)) return 0;
   const size_t pairs = (size_t)(heads / groups + 1) / 2 * groups;
   return ((size_t)tokens / kQ + seqs) * pairs * 2 * sizeof(Steps) + (size_t)kMaxCtas * (4 * kP * d_state * 4 + 16 + 2 * sizeof(Plan));
 }
 
 int launch_ssm_prompt(const ScanArgs& a, cudaStream_t stream) {
-  if (chunk_sizes(a.type, a.pk.tokens, a.head_dim, a.d_state) && rows16(a.x, a.x_stride) && rows16(a.B, a.b_stride) &&
-      rows16(a.C, a.c_stride) && rows16(a.y, a.y_stride))
+  if (chunk_sizes(a.type, a.pk.tokens, a.pk.seqs, a.head_dim, a.d_state) && rows16(a.x, a.x_stride) &&
+      rows16(a.B, a.b_stride) && rows16(a.C, a.c_stride) && rows16(a.y, a.y_stride))
     return a.d_state == 128 ? launch_chunks<128>(a, stream) : launch_chunks<64>(a, stream);
   return launch_scan_tokens(a, stream);
 }

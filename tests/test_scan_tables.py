@@ -7,7 +7,7 @@ import subprocess
 
 import pytest
 
-from ervf_b200 import build
+from ervf_b200 import _lib, build
 
 CODE = r"""
 #include <cstdio>
@@ -96,3 +96,11 @@ def program(tmp_path_factory):
 def test_entries_stay_in_the_table(program):
     r = subprocess.run([str(program)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and "tables ok" in r.stdout, r.stdout
+
+
+def test_packs_of_more_sequences_than_the_tables_are_walked_for():
+    """They go token by token, which takes no scratch."""
+    need = _lib.load().ervf_ssm_prompt_scratch_bytes
+    assert need(_lib.BF16, 1 << 20, 16384, 64, 64, 8, 128) > 0
+    assert need(_lib.BF16, 1 << 20, 16385, 64, 64, 8, 128) == 0
+    assert need(_lib.BF16, 1 << 26, 1 << 26, 64, 64, 8, 128) == 0
