@@ -668,13 +668,18 @@ int launch_ssm_token(const TokenArgs& a, cudaStream_t stream) {
     return (2 * (size_t)a.d_state + 2 * most * a.head_dim + 3 * most + kTokThreads / 32 + 16) * 4 +
            (kMaxConvWidth - 1) * 2 * a.d_state * elem;
   };
-  constexpr size_t kMost = 48 * 1024;
+  constexpr size_t kMost = 48 * 1024;  // fewer CTAs a group, as long as each needs no more than this
   int c = hpg < 8 ? hpg : 8;
   while (c > 1 && (long long)a.seqs * a.groups * c > 12LL * device_sm_count() && smem_of((c + 1) / 2) <= kMost)
     c = (c + 1) / 2;
   const size_t smem = smem_of(c);
   const void* fn = a.type == kTypeBF16 ? token_kernel<__nv_bfloat16>(a.d_state) : token_kernel<float>(a.d_state);
-  if (smem > kMost) return kErrShape;
+  // eight CTAs of the widest group of one-channel heads take 90 KB
+  static_assert((2 * kMaxDState + 5 * (kMaxGroupChannels / 8) + kTokThreads / 32 + 16 +
+                 (kMaxConvWidth - 1) * 2 * kMaxDState) * 4 <= 227 * 1024, "any group fits");
+  if (smem > kMost &&
+      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return kErrLaunch;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.seqs * a.groups * c));
   cfg.blockDim = dim3(kTokThreads);
