@@ -209,10 +209,11 @@ bool vec_ok(const void* p, long long stride, size_t elem, unsigned bytes = 16) {
 // head's state, NL columns each (columns n with (n / 4) % 4 == lane part), in
 // registers; B, C, x and the steps of kSeqTile tokens at a time lie in shared
 // memory.  Serves every type and size; its time is the length of a sequence
-// times the latency of one step.
+// times the latency of one step.  PAD: fewer state columns than 4 NL; those
+// behind them take no part in a step, whose x may be infinite (0 times it is NaN).
 constexpr int kSeqRows = 32, kSeqThreads = 4 * kSeqRows, kSeqTile = 16;
 
-template <typename T, int NL>
+template <typename T, int NL, bool PAD>
 __global__ void __launch_bounds__(kSeqThreads) scan_seq_kernel(ScanArgs a) {
   constexpr int N = 4 * NL;
   __shared__ __align__(16) float sB[kSeqTile][N], sC[kSeqTile][N];
@@ -264,10 +265,11 @@ __global__ void __launch_bounds__(kSeqThreads) scan_seq_kernel(ScanArgs a) {
       for (int i = 0; i < NL; i += 4) {
         const float4 b = *reinterpret_cast<const float4*>(&sB[t][i * 4 + part * 4]);
         const float4 c = *reinterpret_cast<const float4*>(&sC[t][i * 4 + part * 4]);
-        s[i] = fmaf(dx, b.x, da * s[i]);
-        s[i + 1] = fmaf(dx, b.y, da * s[i + 1]);
-        s[i + 2] = fmaf(dx, b.z, da * s[i + 2]);
-        s[i + 3] = fmaf(dx, b.w, da * s[i + 3]);
+        const int left = n_real - (i * 4 + part * 4);  // real columns from here on
+        s[i] = fmaf(!PAD || left > 0 ? dx : 0.0f, b.x, da * s[i]);
+        s[i + 1] = fmaf(!PAD || left > 1 ? dx : 0.0f, b.y, da * s[i + 1]);
+        s[i + 2] = fmaf(!PAD || left > 2 ? dx : 0.0f, b.z, da * s[i + 2]);
+        s[i + 3] = fmaf(!PAD || left > 3 ? dx : 0.0f, b.w, da * s[i + 3]);
         y[0] = fmaf(s[i], c.x, y[0]);
         y[1] = fmaf(s[i + 1], c.y, y[1]);
         y[2] = fmaf(s[i + 2], c.z, y[2]);
@@ -288,13 +290,19 @@ __global__ void __launch_bounds__(kSeqThreads) scan_seq_kernel(ScanArgs a) {
   }
 }
 
+template <typename T, int NL>
+void scan_seq(const ScanArgs& a, cudaStream_t stream) {
+  const dim3 grid(a.pk.seqs, a.heads, (a.head_dim + kSeqRows - 1) / kSeqRows);
+  if (a.d_state == 4 * NL) scan_seq_kernel<T, NL, false><<<grid, kSeqThreads, 0, stream>>>(a);
+  else scan_seq_kernel<T, NL, true><<<grid, kSeqThreads, 0, stream>>>(a);
+}
+
 template <typename T>
 int launch_scan_seq(const ScanArgs& a, cudaStream_t stream) {
-  const dim3 grid(a.pk.seqs, a.heads, (a.head_dim + kSeqRows - 1) / kSeqRows);
-  if (a.d_state <= 16) scan_seq_kernel<T, 4><<<grid, kSeqThreads, 0, stream>>>(a);
-  else if (a.d_state <= 64) scan_seq_kernel<T, 16><<<grid, kSeqThreads, 0, stream>>>(a);
-  else if (a.d_state <= 128) scan_seq_kernel<T, 32><<<grid, kSeqThreads, 0, stream>>>(a);
-  else scan_seq_kernel<T, 64><<<grid, kSeqThreads, 0, stream>>>(a);
+  if (a.d_state <= 16) scan_seq<T, 4>(a, stream);
+  else if (a.d_state <= 64) scan_seq<T, 16>(a, stream);
+  else if (a.d_state <= 128) scan_seq<T, 32>(a, stream);
+  else scan_seq<T, 64>(a, stream);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
@@ -455,9 +463,10 @@ __global__ void __launch_bounds__(kTokThreads, 4) ssm_token_kernel(TokenArgs a) 
         e.y = fmaf(dx, b[j].y, da * e.y);
         e.z = fmaf(dx, b[j].z, da * e.z);
         e.w = fmaf(dx, b[j].w, da * e.w);
-        if (slot >= 0 && p < P && n0 + j * 4 * L < N)
-          *reinterpret_cast<float4*>(st + q * kStep * N + j * 4 * L) = e;
-        y[q] = fmaf(e.x, cc[j].x, fmaf(e.y, cc[j].y, fmaf(e.z, cc[j].z, fmaf(e.w, cc[j].w, y[q]))));
+        const bool real = n0 + j * 4 * L < N;  // the others' 0 times an infinite x is NaN
+        if (slot >= 0 && p < P && real) *reinterpret_cast<float4*>(st + q * kStep * N + j * 4 * L) = e;
+        const float sum = fmaf(e.x, cc[j].x, fmaf(e.y, cc[j].y, fmaf(e.z, cc[j].z, fmaf(e.w, cc[j].w, y[q]))));
+        y[q] = real ? sum : y[q];
       }
     }
     // the rows' sums over their L lanes: each halving step leaves a lane half
