@@ -47,7 +47,8 @@
 // (waits that watched the clock and unrolled MMA loops: 97 KB, 179 us).  Tried
 // without gain: y of the second head by the W warps, S C ahead of the state's
 // new terms, W pieces of 16 tokens, C B^T pieces loaded once for both heads.
-// In pass 1 warps 0..7 do W's work too.
+// In pass 1 warps 0..7 do W's work too.  y's test for sums that a NaN or an
+// infinity behind their token has spoiled costs 1% (causal_rows).
 // Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
 // dead, and every role leaves; copies and MMAs are drained first.
 #include <cuda.h>  // CUtensorMap and the encode function's types (driver entry point)
@@ -307,6 +308,60 @@ __device__ __forceinline__ void split2(float e, float o, uint32_t& hi, uint32_t&
   lo = pack2(e - lo_f(hi), o - hi_f(hi));
 }
 
+// A NaN or an infinity in x meets the zero weights of the tokens before it in
+// the tensor cores.  Where that spoiled sums of a warp's 32 tokens (16 columns
+// of one head from piece `piece` of x's rows), their lanes form them anew here,
+// token by token up to their own, from the weights in tensor memory, and store
+// their outputs over the first ones (out: a lane's, or null).  Sums that the
+// state before the chunk has spoiled as well stay as they are.
+__device__ __forceinline__ void causal_rows(uint32_t p_at, uint32_t y_at, uint32_t px_at, const uint8_t* x, int t,
+                                            int piece, float D, float e, __nv_bfloat16* out) {
+  uint32_t u[16], v[16];
+  tm_ld16x2(y_at, px_at, u, v);
+  bool spoiled = false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    spoiled = spoiled || (!isfinite(__uint_as_float(v[i])) && isfinite(e * __uint_as_float(u[i])));
+  if (!__any_sync(0xffffffffu, spoiled)) return;
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = 0.0f;
+#pragma unroll 1
+  for (int s = 0; s <= (t | 31); ++s) {
+    uint32_t w;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(w) : "r"(p_at + (s >> 1)) : "memory");
+    if (s <= t) {
+      const float p = s & 1 ? hi_f(w) : lo_f(w);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4 xv = *reinterpret_cast<const uint4*>(x + s * 128 + (((piece + k) ^ (s & 7)) << 4));
+        const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[8 * k + 2 * i] = fmaf(p, lo_f(xs[i]), f[8 * k + 2 * i]);
+          f[8 * k + 2 * i + 1] = fmaf(p, hi_f(xs[i]), f[8 * k + 2 * i + 1]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  if (!spoiled || !out) return;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint4 xv = *reinterpret_cast<const uint4*>(x + t * 128 + (((piece + k) ^ (t & 7)) << 4));
+    const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = 8 * k + 2 * i;
+      o[i] = pack2(fmaf(D, lo_f(xs[i]), fmaf(e, __uint_as_float(u[m]), f[m])),
+                   fmaf(D, hi_f(xs[i]), fmaf(e, __uint_as_float(u[m + 1]), f[m + 1])));
+    }
+    reinterpret_cast<uint4*>(out)[k] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
 // W: a team scales x of step `it` to the chunk's end and splits it into three,
 // kWRows tokens of both heads at a time: every second such piece of the chunk.
 template <int N, bool WHOLE>
@@ -513,6 +568,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
         const int left = wk.valid() - 32 * q;  // rows of this warp inside the sequence
         __nv_bfloat16* rows = a.y + (size_t)(wk.row0() + 32 * q) * a.y_stride + 32 * side;
         uint8_t* stage = smem + Sm::kY + warp * 1024;
+        uint32_t odd = 0;  // not 0 once an output is no finite number
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           const Steps& st = steps[2 * ph + h];
@@ -539,6 +595,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
               }
               *reinterpret_cast<uint4*>(stage + lane * 32 + ((k ^ ((lane >> 2) & 1)) << 4)) =
                   make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(odd) : "r"(o[i]), "r"(0));
             }
             __syncwarp();
 #pragma unroll
@@ -548,6 +606,19 @@ __global__ void __launch_bounds__(kChThreads, 1)
               if (put && r < left) *reinterpret_cast<uint4*>(y + (size_t)r * a.y_stride + 8 * (c + i)) = val;
             }
             __syncwarp();
+          }
+        }
+        if (__any_sync(0xffffffffu, (odd & 0x7FFF7FFFu) != 0)) {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            const int h = i >> 1, c = 2 * (i & 1), col = 64 * h + 32 * side + 8 * c;
+            const Steps& st = steps[2 * ph + h];
+            const float e = ex2(st.lp[t] + (q > 0 ? st.blk[0] : 0.0f) + (q > 1 ? st.blk[1] : 0.0f) +
+                                (q > 2 ? st.blk[2] : 0.0f));
+            const bool put = lane < left && (h == 0 || hd.h[1] != hd.h[0]);
+            causal_rows(lanes + kTmP + 64 * h, lanes + kTmY + col, lanes + kTmCB + col, smem + Sm::kX + h * kPanel, t,
+                        4 * side + c, st.D, e,
+                        put ? rows + (size_t)(h ? hd.h[1] : hd.h[0]) * kP + (size_t)lane * a.y_stride + 8 * c : nullptr);
           }
         }
         tc_before();

@@ -628,9 +628,8 @@ ERVF_API int ervf_conv1d_prompt(const void* x, long long x_stride, const float* 
  * bf16 with head_dim 64, d_state 64 or 128 and rows of x, B, C, y of 16-byte
  * alignment runs in chunks of 128 tokens on the tensor cores (above 32
  * tokens); everything else token by token, whose time grows with the longest
- * sequence.  In chunks a NaN or infinity in x may also reach tokens before it
- * in its own sequence's chunk (a zero weight times it), never another
- * sequence.  The reference: softplus and ssm, one token at a time. */
+ * sequence.  A NaN or infinity reaches what the recurrence lets it reach, in
+ * both forms; in chunks an infinity may become NaN on the way.  The reference: softplus and ssm, one token at a time. */
 ERVF_API int ervf_ssm_prompt(const void* x, long long x_stride, const void* dt, long long dt_stride,
                              const float* A, const void* B, long long b_stride, const void* C,
                              long long c_stride, const float* D, const float* dt_bias, float* state, int n_slots,
