@@ -34,6 +34,7 @@ _ACTS = {"none": _lib.ACT_NONE, "relu2": _lib.ACT_RELU2, "silu": _lib.ACT_SILU, 
 _F32, _I32, _U8 = (torch.float32,), (torch.int32,), (torch.uint8, torch.bool)
 _BF16 = (torch.bfloat16, torch.uint16, torch.int16)
 _CODE_TYPES = {_lib.F32: _F32, _lib.BF16: _BF16}
+_CAI_NAMES = {_F32: ("<f4",), _I32: ("<i4",), _U8: ("|u1", "|b1"), _BF16: ("<u2", "<i2")}
 
 
 # handle of torch's current stream on a device, without making a Stream object
@@ -52,6 +53,18 @@ def _type_of(a, dtype, what: str) -> int:
     if code is None:
         raise ValueError(f"{what}: float32 or bfloat16 elements are needed")
     return code
+
+
+def _contiguous(cai) -> bool:
+    """Whether a CUDA array's elements lie in C order without gaps."""
+    strides, step = cai.get("strides"), int(cai["typestr"][2:])
+    if strides is None:
+        return True
+    for n, s in zip(reversed(cai["shape"]), reversed(strides)):
+        if n > 1 and s != step:
+            return False
+        step *= n
+    return True
 
 
 class GPUKernels:
@@ -120,7 +133,7 @@ class GPUKernels:
         if not isinstance(a, int):
             if _type_of(a, None, what) != code:
                 raise ValueError(f"{what}: its elements do not fit the other arrays")
-            if a.__cuda_array_interface__.get("strides") is not None:
+            if not _contiguous(a.__cuda_array_interface__):
                 raise ValueError(f"{what}: a contiguous array is needed")
             _need(a, rows * cols, what)
         return ptr(a), cols
@@ -135,6 +148,10 @@ class GPUKernels:
                 return a.data_ptr()
             self._refuse(a, n, dtypes, what)
         if not isinstance(a, int):
+            cai = a.__cuda_array_interface__
+            if cai["typestr"] not in _CAI_NAMES[dtypes] or not _contiguous(cai):
+                raise ValueError(f"{what}: a contiguous array of {_CAI_NAMES[dtypes]} is needed, not "
+                                 f"{cai['typestr']} with strides {cai.get('strides')}")
             _need(a, n, what)
         return ptr(a)
 

@@ -1,0 +1,82 @@
+"""What the dense and state-space methods take from objects with
+``__cuda_array_interface__``: checked as tensors are, before any CUDA call."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from ervf_b200 import GPUKernels
+
+AT = 1 << 20
+
+
+class Array:
+    def __init__(self, shape, typestr, strides=None, at=AT):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (at, False), "version": 3,
+                                         "strides": strides}
+
+
+class Launches:
+    """Takes the place of the launch: nothing here has a GPU."""
+
+    def __init__(self, monkeypatch):
+        self.seen = []
+        monkeypatch.setattr(GPUKernels, "_launch", lambda k, name, *args: self.seen.append((name, args)))
+
+
+@pytest.fixture()
+def k():
+    return GPUKernels(device="cuda:0")
+
+
+def calls(k, **over):
+    """One call of each method with arrays of the right kind, but for those in `over`."""
+    f, u, i, b = (lambda *s: Array(s, "<f4")), (lambda *s: Array(s, "<u2")), (lambda *s: Array(s, "<i4")), \
+        (lambda *s: Array(s, "|b1"))
+    v = dict(W=u(16, 8), bias=f(16), cw=f(8, 4), cb=f(8), cs=u(2, 3, 8), cu=i(2), slots=i(1), has=b(1), A=f(2), D=f(2),
+             dtb=f(2), st=f(2, 2, 2, 4), nw=f(4), tw=f(12, 2), tb=f(12), tcs=u(2, 1, 12))
+    v.update(over)
+    bf = torch.bfloat16
+    return {
+        "linear": lambda: k.linear_bf16(AT, v["W"], AT, 16, 8, 3, bias=v["bias"], dtype=bf),
+        "conv": lambda: k.conv1d_prompt(AT, AT, v["cw"], v["cb"], v["cs"], v["cu"], 1, 3, 8, 4, slots=v["slots"],
+                                        has_state=v["has"], n_slots=2, dtype=bf),
+        "scan": lambda: k.ssm_prompt(AT, AT, AT, v["A"], AT, AT, v["D"], v["dtb"], v["st"], v["cu"], 1, 3, 2, 2, 1, 4,
+                                     slots=v["slots"], has_state=v["has"], n_slots=2, dtype=bf),
+        "token": lambda: k.ssm_token(AT, AT, AT, v["tw"], v["tb"], v["tcs"], v["A"], v["D"], v["dtb"], v["st"], 1, 2, 2,
+                                     1, 4, 2, norm_w=v["nw"], slots=v["slots"], n_slots=2, dtype=bf),
+        "norm": lambda: k.gated_norm(AT, AT, None, v["nw"], 3, 2, 2, dtype=bf),
+    }
+
+
+def test_arrays_of_the_right_kind_are_taken(k, monkeypatch):
+    seen = Launches(monkeypatch).seen
+    for call in calls(k).values():
+        call()
+    assert len(seen) == 5
+    calls(k, W=Array((16, 8), "<u2", strides=(16, 2)), bias=Array((1, 16, 1), "<f4", strides=(0, 4, 12)))["linear"]()
+    k.gated_norm(Array((3, 4), "<f4", strides=(16, 4)), AT, None, AT, 3, 2, 2)
+    assert len(seen) == 7
+
+
+@pytest.mark.parametrize("name,what,array", [
+    ("linear", "W", Array((16, 8), "<f4")), ("linear", "W", Array((16, 8), "<u2", (2, 32))),
+    ("linear", "W", Array((16, 8), "<u2", (32, 2))), ("linear", "bias", Array((16,), "<f8")),
+    ("linear", "bias", Array((16,), "<f4", (8,))), ("conv", "cw", Array((8, 4), "<u2")),
+    ("conv", "cs", Array((2, 3, 8), "<f4")), ("conv", "cu", Array((2,), "<i8")), ("conv", "slots", Array((1,), "<u4")),
+    ("conv", "has", Array((1,), "<i4")), ("scan", "A", Array((2,), "<f8")), ("scan", "st", Array((2, 2, 2, 4), "<u2")),
+    ("scan", "cu", Array((2,), "<i4", (8,))), ("token", "tcs", Array((2, 1, 12), "<f4")),
+    ("token", "D", Array((2,), "<f2")), ("norm", "nw", Array((4,), "<f4", (-4,)))])
+def test_arrays_of_another_type_or_order_are_refused(k, monkeypatch, name, what, array):
+    """Their bytes would be read as the elements of the right kind."""
+    seen = Launches(monkeypatch).seen
+    with pytest.raises(ValueError):
+        calls(k, **{what: array})[name]()
+    assert not seen
+
+
+def test_rows_are_taken_contiguous(k, monkeypatch):
+    Launches(monkeypatch)
+    with pytest.raises(ValueError):
+        k.gated_norm(Array((3, 4), "<f4", strides=(32, 4)), AT, None, AT, 3, 2, 2)
