@@ -18,6 +18,10 @@ tensors on this object's device, activations in one row per token.  A 2-D
 tensor may have any row stride (a slice of a wider row); other shapes are
 read as contiguous rows.  Objects with ``__cuda_array_interface__`` and int
 addresses are contiguous rows too, and an int output needs ``dtype``.
+
+Launches go on ``self.stream`` if set (a torch or CuPy stream or a raw handle),
+else on torch's current stream -- with CuPy too: a program whose arrays are on
+a CuPy stream sets it.
 """
 
 from __future__ import annotations
@@ -25,7 +29,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .fused_nvfp4 import _need, ptr
+from .fused_nvfp4 import _need, current_stream, ptr
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.uint16: _lib.BF16,
           torch.int16: _lib.BF16}
@@ -80,7 +84,7 @@ class GPUKernels:
 
     def _s(self) -> int:
         if self.stream is not None:
-            return int(self.stream.cuda_stream)
+            return current_stream(self.stream, self.device)
         return int(torch.cuda.current_stream(self.device).cuda_stream)
 
     def mv_bf16(self, out, W, x, rows: int, cols: int) -> None:
@@ -175,7 +179,7 @@ class GPUKernels:
         return state.numel() // per_slot
 
     def _launch(self, name: str, *args) -> None:
-        stream = _raw_stream(self._index) if self.stream is None else int(self.stream.cuda_stream)
+        stream = _raw_stream(self._index) if self.stream is None else current_stream(self.stream, self.device)
         if torch.cuda.current_device() == self._index:
             _lib.call(name, *args, stream)
         else:
@@ -289,5 +293,10 @@ class GPUKernels:
             return None
         if self.stream is None:
             return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        with torch.cuda.stream(self.stream):
+        stream = self.stream
+        if not isinstance(stream, torch.cuda.Stream):
+            handle = current_stream(stream, self.device)
+            stream = torch.cuda.ExternalStream(handle, self.device) if handle else \
+                torch.cuda.default_stream(self.device)
+        with torch.cuda.stream(stream):
             return torch.empty(nbytes, dtype=torch.uint8, device=self.device)

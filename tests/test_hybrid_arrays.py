@@ -80,3 +80,17 @@ def test_rows_are_taken_contiguous(k, monkeypatch):
     Launches(monkeypatch)
     with pytest.raises(ValueError):
         k.gated_norm(Array((3, 4), "<f4", strides=(32, 4)), AT, None, AT, 3, 2, 2)
+
+
+@pytest.mark.parametrize("stream,handle", [
+    (type("Torch", (), {"cuda_stream": 64})(), 64), (type("Cupy", (), {"ptr": 128})(), 128), (256, 256), (0, 0)])
+def test_a_stream_of_any_kind(k, monkeypatch, stream, handle):
+    from ervf_b200 import _lib
+
+    seen = []
+    monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append(args[-1]))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    k.stream = stream
+    k.gated_norm(AT, AT, None, AT, 3, 2, 2, dtype=torch.float32)
+    k.mv_bf16(AT, AT, AT, 8, 8)
+    assert seen == [handle, handle]
