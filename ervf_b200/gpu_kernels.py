@@ -176,7 +176,7 @@ class GPUKernels:
             return 0
         if not isinstance(state, torch.Tensor):
             raise ValueError(f"{what}: n_slots is needed beside an address")
-        return state.numel() // per_slot
+        return state.numel() // max(per_slot, 1)
 
     def _launch(self, name: str, *args) -> None:
         stream = _raw_stream(self._index) if self.stream is None else current_stream(self.stream, self.device)
@@ -217,7 +217,7 @@ class GPUKernels:
         code = _type_of(out, dtype, "out")
         po, so = self._rows(out, tokens, channels, code, "out")
         px, sx = self._rows(x, tokens, channels, code, "x")
-        ns = self._slots_of(state, (width - 1) * channels or 1, n_slots, "state")
+        ns = self._slots_of(state, (width - 1) * channels, n_slots, "state")
         self._launch("ervf_conv1d_prompt", px, sx, self._flat(w, channels * width, _F32, "w"),
                      self._flat(bias, channels, _F32, "bias"),
                      self._flat(state, ns * (width - 1) * channels, _CODE_TYPES[code], "state"), ns,

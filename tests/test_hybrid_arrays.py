@@ -94,3 +94,12 @@ def test_a_stream_of_any_kind(k, monkeypatch, stream, handle):
     k.gated_norm(AT, AT, None, AT, 3, 2, 2, dtype=torch.float32)
     k.mv_bf16(AT, AT, AT, 8, 8)
     assert seen == [handle, handle]
+
+
+def test_sizes_of_nothing_are_refused_beside_a_state(k):
+    state, f32 = torch.zeros(4, 4), torch.float32
+    for call in (lambda: k.ssm_prompt(AT, AT, AT, AT, AT, AT, None, None, state, AT, 1, 3, 0, 64, 1, 64, dtype=f32),
+                 lambda: k.ssm_token(AT, AT, AT, AT, None, AT, AT, None, None, state, 1, 4, 64, 1, 0, 4, dtype=f32),
+                 lambda: k.conv1d_prompt(AT, AT, AT, None, state, AT, 1, 3, 0, 4, dtype=f32)):
+        with pytest.raises(ValueError):
+            call()
