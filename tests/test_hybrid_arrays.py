@@ -103,3 +103,39 @@ def test_sizes_of_nothing_are_refused_beside_a_state(k):
                  lambda: k.conv1d_prompt(AT, AT, AT, None, state, AT, 1, 3, 0, 4, dtype=f32)):
         with pytest.raises(ValueError):
             call()
+
+
+WIDE = 2 ** 32 + 8  # 8 in 32 bits
+
+
+@pytest.mark.parametrize("size", [WIDE, 2 ** 31, -WIDE])
+def test_sizes_that_pass_32_bits_are_refused(k, monkeypatch, size):
+    """Cut to 32 bits they would be other sizes, and most of the output would stay as it was."""
+    seen = Launches(monkeypatch).seen
+    f32 = torch.float32
+
+    def linear(rows=8, cols=8, tokens=3):
+        k.linear_bf16(AT, AT, AT, rows, cols, tokens, dtype=f32)
+
+    def conv(seqs=1, tokens=3, channels=8, width=4, n_slots=1):
+        k.conv1d_prompt(AT, AT, AT, None, AT, AT, seqs, tokens, channels, width, n_slots=n_slots, dtype=f32)
+
+    def scan(seqs=1, tokens=3, heads=2, head_dim=2, groups=1, d_state=4, n_slots=1):
+        k.ssm_prompt(AT, AT, AT, AT, AT, AT, None, None, AT, AT, seqs, tokens, heads, head_dim, groups, d_state,
+                     n_slots=n_slots, dtype=f32)
+
+    def token(seqs=1, heads=2, head_dim=2, groups=1, d_state=4, width=4, n_slots=1):
+        k.ssm_token(AT, AT, AT, AT, None, AT, AT, None, None, AT, seqs, heads, head_dim, groups, d_state, width,
+                    n_slots=n_slots, dtype=f32)
+
+    def norm(tokens=3, groups=1, group_size=8):
+        k.gated_norm(AT, AT, None, AT, tokens, groups, group_size, dtype=f32)
+
+    for call in (linear, conv, scan, token, norm):
+        for name in call.__code__.co_varnames[:call.__code__.co_argcount]:
+            with pytest.raises(ValueError):
+                call(**{name: size})
+    assert not seen
+    for call in (linear, conv, scan, token, norm):
+        call()
+    assert len(seen) == 5
