@@ -585,8 +585,9 @@ ERVF_API int ervf_cache_fetch(const uint8_t* bank_c, const uint8_t* bank_s, uint
  * elements apart; bias f32.  bias, resid may be NULL; resid may be out
  * itself (then with its stride), x must not overlap out.  Sums and epilogue
  * in f32, one rounding to out_type, the same bits on every call; the tensor
- * core's own sums are off by up to 3e-6 (relative, 4096 columns) beyond 64
- * tokens, a quarter of that up to 64.  cols and x_stride multiples of 8, W and
+ * core's own sums truncate: over 4096 columns they are off by 4.4e-6 of the
+ * results' norm beyond 64 tokens and by 1.0e-6 up to 64 (normal W and x; it
+ * grows with cols).  cols and x_stride multiples of 8, W and
  * x 16-byte aligned; any rows and tokens (out rows of 16-byte alignment are
  * fastest).  tokens = 0 does nothing.
  * The reference projects one token at a time (gpu_kernels.py:21-49). */
