@@ -60,7 +60,8 @@ def _type_of(a, dtype, what: str) -> int:
 
 
 def _fit(*sizes) -> None:
-    """Sizes reach the C ABI as 32-bit numbers, to which ctypes would cut them without a word."""
+    """Sizes reach the C ABI as 32-bit numbers, to which ctypes would cut them without a word.
+    Called where one of them has a bit above the 31st (or a sign, which the C ABI refuses)."""
     if max(sizes) > 0x7FFFFFFF or min(sizes) < -0x80000000:
         raise ValueError(f"unsupported shape: sizes {sizes} pass 32 bits")
 
@@ -202,7 +203,8 @@ class GPUKernels:
         epilogue, one rounding, the same bits on every call."""
         if act not in _ACTS:
             raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
-        _fit(rows, cols, tokens)
+        if (rows | cols | tokens) >> 31:
+            _fit(rows, cols, tokens)
         code = _type_of(out, dtype, "out")
         po, so = self._rows(out, tokens, rows, code, "out")
         px, sx = self._rows(x, tokens, cols, _lib.BF16, "x")
@@ -222,7 +224,8 @@ class GPUKernels:
         sequence carries any): row slots[i] (None: i) holds the inputs before
         sequence i where has_state[i], and its last inputs afterwards; a slot
         outside the array is no state.  No slot may be named twice."""
-        _fit(seqs, tokens, channels, width)
+        if (seqs | tokens | channels | width) >> 31:
+            _fit(seqs, tokens, channels, width)
         code = _type_of(out, dtype, "out")
         po, so = self._rows(out, tokens, channels, code, "out")
         px, sx = self._rows(x, tokens, channels, code, "x")
@@ -243,7 +246,8 @@ class GPUKernels:
         cu_seqlens, slots and has_state as in conv1d_prompt.  A is not above 0.
         bf16 with head_dim 64 and d_state 64 or 128 runs in chunks on the tensor
         cores, everything else token by token."""
-        _fit(seqs, tokens, heads, head_dim, groups, d_state)
+        if (seqs | tokens | heads | head_dim | groups | d_state) >> 31:
+            _fit(seqs, tokens, heads, head_dim, groups, d_state)
         code = _type_of(y, dtype, "y")
         inner, bc = heads * head_dim, groups * d_state
         py, sy = self._rows(y, tokens, inner, code, "y")
@@ -268,7 +272,8 @@ class GPUKernels:
         scan and gated_norm (z None: no gate, norm_w None: no norm), in one
         launch; conv_state and state are updated in place.  A sequence whose
         slot is outside the arrays starts from zero and stores nothing."""
-        _fit(seqs, heads, head_dim, groups, d_state, width)
+        if (seqs | heads | head_dim | groups | d_state | width) >> 31:
+            _fit(seqs, heads, head_dim, groups, d_state, width)
         code = _type_of(out, dtype, "out")
         inner = heads * head_dim
         ch = inner + 2 * groups * d_state
@@ -290,7 +295,8 @@ class GPUKernels:
                    dtype=None) -> None:
         """out = w g / sqrt(mean(g^2) + eps) with g = y silu(z) (z None: y), the mean per
         group of channels.  out may be y or z itself."""
-        _fit(tokens, groups, group_size)
+        if (tokens | groups | group_size) >> 31:
+            _fit(tokens, groups, group_size)
         code = _type_of(out, dtype, "out")
         n = groups * group_size
         po, so = self._rows(out, tokens, n, code, "out")
