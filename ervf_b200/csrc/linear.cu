@@ -254,7 +254,9 @@ struct LinEdge {
 };
 
 // 16 features r.. of a warp's tokens t0 .. t0 + 31 where rows have any
-// alignment: from shared memory, 16 lanes to a token.
+// alignment: from shared memory, 16 lanes to a token, an element each.  Against
+// tensor stores: 509 x 3712 x 2688 21 us instead of 17, 8192 x 2688 x 3712 134 instead
+// of 115 in bf16, 150 instead of 116 in f32 (GPU time).
 template <typename T>
 __device__ __noinline__ void lin_ragged(const LinTile& a, int t0, int r, const float* stage) {
   const int lane = threadIdx.x & 31;

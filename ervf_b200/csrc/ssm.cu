@@ -80,7 +80,7 @@ struct Raw {
 // y_t = act(bias + sum_j w[j] x[t - width + 1 + j]) for each channel.  A
 // thread owns V channels of one tile of a sequence, keeps the window in
 // registers and the next tokens' loads in flight while it works on as many
-// (eight of bf16: 8192 tokens of 6144 channels 52 -> 47 us, 4.3 TB/s; four of
+// (eight of bf16: 8192 tokens of 6144 channels in 45 us, 4.5 TB/s; four of
 // f32, which at eight ran short of registers).
 // Bound by HBM and, near it, by the two special-function operations of each
 // silu: every input is read once (and `width - 1` rows again per tile, from
@@ -209,7 +209,8 @@ bool vec_ok(const void* p, long long stride, size_t elem, unsigned bytes = 16) {
 // head's state, NL columns each (columns n with (n / 4) % 4 == lane part), in
 // registers; B, C, x and the steps of kSeqTile tokens at a time lie in shared
 // memory.  Serves every type and size; its time is the length of a sequence
-// times the latency of one step.  PAD: fewer state columns than 4 NL; those
+// times the latency of one step: 8192 tokens of 64 heads of 64 with 128 states
+// take 3.7 ms in f32 and 4.7 in bf16, where HBM would need 0.05 and 0.03.  PAD: fewer state columns than 4 NL; those
 // behind them take no part in a step, whose x may be infinite (0 times it is NaN).
 constexpr int kSeqRows = 32, kSeqThreads = 4 * kSeqRows, kSeqTile = 16;
 
@@ -600,6 +601,8 @@ __global__ void __launch_bounds__(kNormThreads, NV <= 2 ? 8 : 4) gated_norm_warp
 }
 
 // Any size and alignment: one CTA per (token, group), two passes over a row.
+// 8192 x 4096 in bf16: 77 us off 16-byte rows in groups of 512, 72 as one group (a
+// warp per group: 37), f32 as one group 108 (63).
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads) gated_norm_kernel(NormArgs a) {
   __shared__ float red[kNormThreads / 32];

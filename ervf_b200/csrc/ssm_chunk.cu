@@ -41,8 +41,8 @@
 // memory take its whole bandwidth (128 bytes a clock); with W, the split state
 // and the tiles a step moves 740 KB there, 5800 clocks; its warps issue 5100
 // instructions a scheduler.  Measured: 11000 clocks, of which P takes 3500, P x
-// 1300 and y 3600 one after the other (64 heads, 8192 tokens: 148 us in all,
-// 27 of them pass 1).  Waits are short and loops little
+// 1300 and y 3600 one after the other (64 heads, 8192 tokens: 151 to 156 us in
+// all, 27 of them pass 1, which spills 116 bytes at 128 states).  Waits are short and loops little
 // unrolled on purpose: seven roles' code has to share the instruction cache
 // (waits that watched the clock and unrolled MMA loops: 97 KB, 179 us).  Tried
 // without gain: y of the second head by the W warps, S C ahead of the state's
@@ -1142,8 +1142,13 @@ bool rows16(const void* p, long long stride) {
 }
 
 // The chunked form takes bf16, head_dim 64 and 64 or 128 state columns; and
-// enough tokens: below, the token-by-token kernel's time (0.55 us a token)
-// is less than three launches and a chunk's latency.  And no more than
+// enough tokens: below, the token-by-token kernel's time (0.4 us a token of one
+// sequence) is less than four launches and a chunk's latency.  One sequence of 33
+// tokens takes 18 us in chunks and 17 token by token, of 64 tokens 18 and 28 (64
+// heads, 128 states).  The rule looks at the tokens of the whole call, while a
+// sequence costs a chunk's step however short it is: 8 sequences of 5 take 27 us
+// in chunks and 18 token by token, 32 of 8 63 and 66, 96 of 2 161 and 122, 256
+// of 16 421 and 752.  And no more than
 // kMaxChunkSeqs sequences: pass 0 walks all offsets for every chunk, and every
 // role of passes 1 and 3 steps through empty sequences one by one while the
 // others' waits, which are bounded, run.

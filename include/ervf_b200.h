@@ -627,9 +627,14 @@ ERVF_API int ervf_conv1d_prompt(const void* x, long long x_stride, const float* 
  * cleared; calls that share it must not overlap on the GPU.  y must not
  * overlap an input.
  * bf16 with head_dim 64, d_state 64 or 128 and rows of x, B, C, y of 16-byte
- * alignment runs in chunks of 128 tokens on the tensor cores (above 32
- * tokens); everything else token by token, whose time grows with the longest
- * sequence.  A NaN or infinity reaches what the recurrence lets it reach, in
+ * alignment runs in chunks of 128 tokens on the tensor cores (above 32 tokens,
+ * up to 16384 sequences); everything else token by token in f32, whose time
+ * grows with the longest sequence: 0.45 us a token in f32 and 0.57 in bf16 for 64
+ * heads of 64 with 128 states, 25 to 30 times the chunks' for a prompt of
+ * thousands of tokens.  In chunks the weights (C_t . B_s) exp(c_t - c_s) d_s of
+ * the tokens of one chunk are rounded to bf16 (2^-8 of each term of y at most,
+ * as y's own rounding; measured 1.8e-3 of y's norm in all instead of 1.7e-3), and
+ * the state before the chunk meets C with 2^-16; states stay f32.  A NaN or infinity reaches what the recurrence lets it reach, in
  * both forms; in chunks an infinity may become NaN on the way.  The reference: softplus and ssm, one token at a time. */
 ERVF_API int ervf_ssm_prompt(const void* x, long long x_stride, const void* dt, long long dt_stride,
                              const float* A, const void* B, long long b_stride, const void* C,
