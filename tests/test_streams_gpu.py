@@ -38,7 +38,7 @@ def test_scan_on_a_stream_of_any_kind(cuda, kind):
                 "external": torch.cuda.ExternalStream(handle)}[kind]
     if kind != "legacy default":
         with torch.cuda.stream(side):
-            torch.cuda._sleep(20_000_000)  # the call stands behind this on its stream
+            torch.cuda._sleep(200_000_000)  # the call stands behind this on its stream
     call(k, *outs[1])
     if kind != "legacy default":
         torch.cuda.current_stream().synchronize()
