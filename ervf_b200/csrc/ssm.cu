@@ -210,8 +210,9 @@ bool vec_ok(const void* p, long long stride, size_t elem, unsigned bytes = 16) {
 // registers; B, C, x and the steps of kSeqTile tokens at a time lie in shared
 // memory.  Serves every type and size; its time is the length of a sequence
 // times the latency of one step: 8192 tokens of 64 heads of 64 with 128 states
-// take 3.7 ms in f32 and 4.7 in bf16, where HBM would need 0.05 and 0.03.  PAD: fewer state columns than 4 NL; those
-// behind them take no part in a step, whose x may be infinite (0 times it is NaN).
+// take 3.7 ms in f32 and 4.7 in bf16, where HBM would need 0.05 and 0.03.
+// PAD: fewer state columns than 4 NL; those behind them take no part in a step,
+// whose x may be infinite (0 times it is NaN).
 constexpr int kSeqRows = 32, kSeqThreads = 4 * kSeqRows, kSeqTile = 16;
 
 template <typename T, int NL, bool PAD>

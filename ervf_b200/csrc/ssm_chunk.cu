@@ -42,11 +42,12 @@
 // and the tiles a step moves 740 KB there, 5800 clocks; its warps issue 5100
 // instructions a scheduler.  Measured: 11000 clocks, of which P takes 3500, P x
 // 1300 and y 3600 one after the other (64 heads, 8192 tokens: 151 to 156 us in
-// all, 27 of them pass 1, which spills 116 bytes at 128 states).  Waits are short and loops little
-// unrolled on purpose: seven roles' code has to share the instruction cache
-// (waits that watched the clock and unrolled MMA loops: 97 KB, 179 us).  Tried
-// without gain: y of the second head by the W warps, S C ahead of the state's
-// new terms, W pieces of 16 tokens, C B^T pieces loaded once for both heads.
+// all, 27 of them pass 1, which spills 116 bytes at 128 states).  Waits are short
+// and loops little unrolled on purpose: seven roles' code has to share the
+// instruction cache (waits that watched the clock and unrolled MMA loops: 97 KB,
+// 179 us).  Tried without gain: y of the second head by the W warps, S C ahead of
+// the state's new terms, W pieces of 16 tokens, C B^T pieces loaded once for both
+// heads.
 // In pass 1 warps 0..7 do W's work too.  y's test for sums that a NaN or an
 // infinity behind their token has spoiled costs 1% (causal_rows).
 // Every wait is bounded: one that runs out records kErrTimeout, marks the CTA
